@@ -34,7 +34,7 @@ typedef enum quik_status {
                               per map outside the capture).  Nothing was launched. */
 } quik_status;
 
-typedef enum quik_dtype { QUIK_F16 = 0, QUIK_BF16 = 1 } quik_dtype;
+typedef enum quik_dtype { QUIK_F16 = 0, QUIK_BF16 = 1, QUIK_F32 = 2 /* row scales only */ } quik_dtype;
 
 const char *quik_status_string(int status);
 const char *quik_last_hip_error(void);
@@ -384,6 +384,39 @@ int quik_mixed_linear_fwd(const void *qx, const void *qw, const void *meta,
                           const void *fp_w, const void *bias, int dtype, int64_t M,
                           int64_t N, int64_t K, int64_t F, int bits, void *out,
                           void *stream);
+
+/* ---- rows in 8 bits, made where a decoder block makes them ------------------------------------------
+ * No counterpart in the reference, whose norm and activation stay in torch and whose symmetric.quantize takes a
+ * scale that is known before.  One launch each, one pass over the row:
+ *   rms_norm:  h = dtype(x + residual) (written to `sum`; residual NULL: h = x and sum is not written),
+ *              u = h * gain, value = u / sqrt(mean(h^2) + eps)
+ *   silu_mul:  value = u = gate / (1 + exp(-gate)) * up
+ *   q [rows, cols] int8 = rne(u * (127 / max|u|)), scale [rows] of scale_type (QUIK_F32, QUIK_F16 or QUIK_BF16), so that
+ *   value ~ q * scale: |value - q * scale| <= scale / 2 before the scale is rounded to its type.
+ * fp32 arithmetic; the norm's codes are those of the expression evaluated operation by operation.  A row of zeros has codes 0 and
+ * scale 0; a row that holds a NaN or an infinity (in h, u or a factor of u), or whose squares pass fp32's range, codes 0 and a NaN scale.
+ * The pitches are the distances of rows in elements (>= cols; not used with one row); q, sum and scale are contiguous.  Any cols
+ * and any alignment of whole elements; 16-byte aligned rows of a multiple of 8 columns take wide accesses.
+ * sum may be x or residual if its pitch is cols: every element is read before it is written. */
+int quik_rms_norm_quantize(const void *x, int64_t x_pitch, const void *residual, int64_t residual_pitch,
+                           const void *gain, float eps, int dtype, int64_t rows, int64_t cols, void *sum, int8_t *q,
+                           void *scale, int scale_type, void *stream);
+int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up, int64_t up_pitch, int dtype,
+                           int64_t rows, int64_t cols, int8_t *q, void *scale, int scale_type, void *stream);
+
+/* ---- 4-bit weights with a scale per group ------------------------------------------------------------
+ * No counterpart in the reference, whose weights have one scale per output column.
+ *   out[m,n] = dtype( s_row[m] * sum_g scales[n,g] * sum_{k in group g} x[m,k] * (q[n,k] - zeros[n,g]) + bias[n] )
+ *   x       x_bits 16: [M, K] of dtype, scale_row not used; x_bits 8: [M, K] int8 with scale_row [M] fp32
+ *   w       [N, K/2] uint8, signed int4 codes, low nibble = even k (MixedQLinear.int_weight, pack_to_i4)
+ *   scales  [N, ceil(K / group)] dtype; zeros the same shape in units of a code (any number, not only whole ones), or NULL
+ *   bias    [N] dtype or NULL; out [M, N] dtype
+ * K % 32 == 0, group % 32 == 0 (a group >= K: one scale per output column; the last group may be shorter); x and w 16-byte
+ * aligned.  A group's product is summed in fp32 (int8: exactly) and scaled in fp32; one rounding to dtype.  A row of x that
+ * holds an infinity gives infinities or NaNs. */
+int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const void *scales, const void *zeros,
+                           const float *scale_row, const void *bias, int dtype, int64_t M, int64_t N, int64_t K,
+                           int64_t group, void *out, void *stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libquik_hip.so")
 
-QUIK_F16, QUIK_BF16 = 0, 1
+QUIK_F16, QUIK_BF16, QUIK_F32 = 0, 1, 2
 
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 
@@ -69,6 +69,9 @@ SIGNATURES = {
     "quik_int8_matmul": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "quik_mixed_linear_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _int,
                                      _vp, _vp]),
+    "quik_rms_norm_quantize": (_int, [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _int, _i64, _i64, _vp, _vp, _vp, _int, _vp]),
+    "quik_silu_mul_quantize": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _vp, _int, _vp]),
+    "quik_int4_group_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp]),
 }
 
 TILED_4 = 0x344C5451    # QUIK_TILED_4: operand buffers, tiled weights of 4 bits
@@ -191,6 +194,16 @@ def dtype_id(t: torch.Tensor, op: str, allow_bf16: bool) -> int:
 def check_cuda_contiguous(op: str, **tensors):
     """The checks the reference's host functions make before launching:
     torch::checkAllContiguous and torch::checkDeviceType(..., CUDA)."""
+    return _check_cuda(op, lambda t: t.is_contiguous(), "contiguous", tensors)
+
+
+def check_cuda_rows(op: str, **tensors):
+    """As check_cuda_contiguous for matrices whose rows may lie apart (column views of a wider one)."""
+    return _check_cuda(op, lambda t: t.dim() == 2 and (t.stride(1) == 1 or t.size(1) <= 1) and
+                       (t.stride(0) >= t.size(1) or t.size(0) <= 1), "a matrix with contiguous rows that do not overlap", tensors)
+
+
+def _check_cuda(op, laid_out, layout, tensors):
     dev = None
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
@@ -198,8 +211,8 @@ def check_cuda_contiguous(op: str, **tensors):
         if not t.is_cuda:
             raise RuntimeError(f"{op}: expected tensor for argument '{name}' to be on a CUDA (HIP) device, "
                                f"but it is on {t.device}")
-        if not t.is_contiguous():
-            raise RuntimeError(f"{op}: expected tensor for argument '{name}' to be contiguous")
+        if not laid_out(t):
+            raise RuntimeError(f"{op}: expected tensor for argument '{name}' to be {layout}")
         if dev is None:
             dev = t.device
         elif t.device != dev:

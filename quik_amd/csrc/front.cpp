@@ -16,10 +16,12 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <optional>
 #include <utility>
@@ -165,14 +167,28 @@ constexpr c10::DispatchKeySet kInterposedKeys({c10::DispatchKey::FuncTorchBatche
                                                c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
                                                c10::DispatchKey::BatchedNestedTensor});
 
-// A plain contiguous tensor on the current GPU, or null.
-const at::Tensor *plain(PyObject *o, c10::DeviceIndex dev) {
+// A plain strided tensor on the current GPU, or null.
+const at::Tensor *strided(PyObject *o, c10::DeviceIndex dev) {
   if (!THPVariable_CheckExact(o) || c10::impl::TorchDispatchModeTLS::any_modes_set()) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(o);
-  if (!t.defined() || t.key_set().has_any(kInterposedKeys) || !t.has_storage() || !t.is_cuda() || t.get_device() != dev || t.layout() != at::kStrided || !t.is_contiguous() ||
+  if (!t.defined() || t.key_set().has_any(kInterposedKeys) || !t.has_storage() || !t.is_cuda() || t.get_device() != dev || t.layout() != at::kStrided ||
       t.is_conj() || t.is_neg())
     return nullptr;
   return &t;
+}
+
+// A plain contiguous one, or null.
+const at::Tensor *plain(PyObject *o, c10::DeviceIndex dev) {
+  const at::Tensor *t = strided(o, dev);
+  return t && t->is_contiguous() ? t : nullptr;
+}
+
+// A matrix with values whose rows are contiguous and do not overlap, or null.
+const at::Tensor *matrix(PyObject *o, c10::DeviceIndex dev) {
+  const at::Tensor *t = strided(o, dev);
+  return t && t->dim() == 2 && t->numel() != 0 && (t->stride(1) == 1 || t->size(1) == 1) && (t->stride(0) >= t->size(1) || t->size(0) == 1)
+             ? t
+             : nullptr;
 }
 
 // The layer's forward on x through its plan: output [rows, N] in `out` (given the shape `shape`).  False: not served
@@ -580,6 +596,109 @@ PyObject *py_fused_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
   });
 }
 
+// the type of row scales that a dtype object names; -1: another one
+int scale_type_of(PyObject *o, at::ScalarType &type) {
+  if (!THPDtype_Check(o)) return -1;
+  type = reinterpret_cast<THPDtype *>(o)->scalar_type;
+  return type == at::kFloat ? QUIK_F32 : type == at::kHalf ? QUIK_F16 : type == at::kBFloat16 ? QUIK_BF16 : -1;
+}
+
+// a tuple of `n` tensors, an undefined one as None
+PyObject *tuple_of(std::initializer_list<at::Tensor> v) {
+  PyObject *t = PyTuple_New(static_cast<Py_ssize_t>(v.size()));
+  if (!t) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor &x : v) {
+    PyObject *o = x.defined() ? THPVariable_Wrap(x) : (Py_INCREF(Py_None), Py_None);
+    if (!o) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, i++, o);
+  }
+  return t;
+}
+
+// rms_norm_quantize(x, weight, eps, residual, scale_dtype) -> (q, scale, sum or None) or None
+PyObject *py_rms_norm_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *x = matrix(args[0], dev), *w = plain(args[1], dev), *r = nullptr;
+  if (!x || !w || (args[3] != Py_None && !(r = matrix(args[3], dev)))) Py_RETURN_NONE;
+  at::ScalarType scales;
+  const int dt = dtype_of(*x), st = scale_type_of(args[4], scales);
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const int64_t rows = x->size(0), cols = x->size(1);
+  if (dt < 0 || st < 0 || !(eps >= 0) || w->dim() != 1 || w->size(0) != cols || w->scalar_type() != x->scalar_type() ||
+      (r && (r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = new_empty({rows, cols}, at::kChar, dev), scale = new_empty({rows, 1}, scales, dev), sum;
+    if (r) sum = new_empty({rows, cols}, x->scalar_type(), dev);
+    const int rc = quik_rms_norm_quantize(data_of(*x), x->stride(0), r ? data_of(*r) : nullptr, r ? r->stride(0) : 0, data_of(*w),
+                                          static_cast<float>(eps), dt, rows, cols, r ? out_ptr(sum) : nullptr,
+                                          static_cast<int8_t *>(out_ptr(q)), out_ptr(scale), st, stream_of(dev));
+    if (rc != QUIK_OK) return fail("rms_norm_quantize", rc);
+    return tuple_of({q, scale, sum});
+  });
+}
+
+// silu_mul_quantize(gate, up, scale_dtype) -> (q, scale) or None
+PyObject *py_silu_mul_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 3) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *g = matrix(args[0], dev), *u = matrix(args[1], dev);
+  if (!g || !u) Py_RETURN_NONE;
+  at::ScalarType scales;
+  const int dt = dtype_of(*g), st = scale_type_of(args[2], scales);
+  if (dt < 0 || st < 0 || u->scalar_type() != g->scalar_type() || u->sizes() != g->sizes()) Py_RETURN_NONE;
+  const int64_t rows = g->size(0), cols = g->size(1);
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = new_empty({rows, cols}, at::kChar, dev), scale = new_empty({rows, 1}, scales, dev);
+    const int rc = quik_silu_mul_quantize(data_of(*g), g->stride(0), data_of(*u), u->stride(0), dt, rows, cols,
+                                          static_cast<int8_t *>(out_ptr(q)), out_ptr(scale), st, stream_of(dev));
+    if (rc != QUIK_OK) return fail("silu_mul_quantize", rc);
+    return tuple_of({q, scale});
+  });
+}
+
+// int4_group_matmul(x, weight, scales, group_size, zeros, scale_row, bias) -> out or None
+PyObject *py_int4_group_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *x = plain(args[0], dev), *w = plain(args[1], dev), *s = plain(args[2], dev), *z = nullptr, *sr = nullptr, *b = nullptr;
+  if (!x || !w || !s || !PyLong_Check(args[3]) || (args[4] != Py_None && !(z = plain(args[4], dev))) ||
+      (args[5] != Py_None && !(sr = plain(args[5], dev))) || (args[6] != Py_None && !(b = plain(args[6], dev))))
+    Py_RETURN_NONE;
+  const int64_t group = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const int dt = dtype_of(*s);
+  const bool codes = x->scalar_type() == at::kChar;
+  if (dt < 0 || w->scalar_type() != at::kByte || (!codes && x->scalar_type() != s->scalar_type()) || codes != (sr != nullptr) || x->dim() != 2 ||
+      w->dim() != 2 || s->dim() != 2 || x->numel() == 0 || w->numel() == 0 || x->size(1) != 2 * w->size(1) || group <= 0 || group % 32 != 0)
+    Py_RETURN_NONE;
+  const int64_t M = x->size(0), K = x->size(1), N = w->size(0);
+  if (K % 32 != 0 || s->size(0) != N || s->size(1) != K / group + (K % group != 0) ||
+      (z && (z->scalar_type() != s->scalar_type() || z->sizes() != s->sizes())) ||
+      (sr && (sr->scalar_type() != at::kFloat || sr->numel() != M)) || (b && (b->scalar_type() != s->scalar_type() || b->numel() != N)))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor out = new_empty({M, N}, s->scalar_type(), dev);
+    const int rc = quik_int4_group_matmul(data_of(*x), codes ? 8 : 16, static_cast<const uint8_t *>(data_of(*w)), data_of(*s),
+                                          z ? data_of(*z) : nullptr, sr ? static_cast<const float *>(data_of(*sr)) : nullptr,
+                                          b ? data_of(*b) : nullptr, dt, M, N, K, group, out_ptr(out), stream_of(dev));
+    if (rc != QUIK_OK) return fail("int4GroupMatmul", rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_forward)), METH_FASTCALL, nullptr},
     {"group_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_group_forward)), METH_FASTCALL, nullptr},
@@ -589,6 +708,9 @@ PyMethodDef kMethods[] = {
     {"matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_matmul)), METH_FASTCALL, nullptr},
     {"dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequantize)), METH_FASTCALL, nullptr},
     {"fused_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_fused_dequantize)), METH_FASTCALL, nullptr},
+    {"rms_norm_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rms_norm_quantize)), METH_FASTCALL, nullptr},
+    {"silu_mul_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_silu_mul_quantize)), METH_FASTCALL, nullptr},
+    {"int4_group_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_int4_group_matmul)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_front", "Host front end of quik_amd's hot calls.", -1, kMethods,

@@ -1,0 +1,284 @@
+// Rows of a decoder block in 8 bits: the two places where a block makes the input of its next product itself.
+//   rms_norm  h = x + residual, rounded to the 16-bit type (and stored: it is the next residual; no residual: h = x)
+//             u = h * gain;  value = u / sqrt(mean(h^2) + eps)
+//   silu_mul  u = gate / (1 + exp(-gate)) * up;  value = u
+// Output: q = rne(u * (127 / top)) with top = max |u| of the row, and scale = top / 127 (/ sqrt(mean(h^2) + eps)), so that
+// value ~ q * scale.  The norm's factor is the same for a whole row and leaves the codes alone: largest magnitude and sum of
+// squares come from the same single pass, and a norm's codes do not depend on the order of a sum.  u is exact in fp32 (products of
+// 8 or 11 bits); every other step of the norm is one IEEE operation in fp32.  A row of zeros has codes 0 and scale 0; a row that
+// holds a NaN or an infinity, or whose squares pass the range of fp32, has codes 0 and a NaN as its scale.
+#include "common.h"
+
+namespace quik {
+namespace {
+
+enum RowOp { kNorm, kNormAdd, kSiluMul };
+
+struct RowArgs {
+  const uint16_t *a, *b, *gain;  // norm: x, residual, gain; silu_mul: gate, up
+  int64_t rows, cols, pitch_a, pitch_b;
+  float eps;
+  uint16_t *sum;  // norm with a residual: h [rows, cols]
+  int8_t *q;
+  void *scale;  // of scale_type
+  int scale_type;
+};
+
+template <bool BF16, RowOp OP>
+__device__ __forceinline__ float row_value(float a, float b, float gain, uint16_t &h, float &square) {
+  if constexpr (OP == kSiluMul) {
+    // exp and the quotient by the hardware's exp2 and reciprocal (1 ulp each): some 4e-7 of a value, 5e-5 of a code's step
+    const float e = __builtin_amdgcn_exp2f(a * -1.44269504088896340736f);
+    return a * __builtin_amdgcn_rcpf(1.0f + e) * b;
+  } else {
+    if constexpr (OP == kNormAdd) {
+      h = from_f32<BF16>(a + b);
+      a = to_f32<BF16>(h);
+    }
+    square += a * a;
+    return a * gain;
+  }
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// what is the same for the row: factor of the codes, scale
+template <RowOp OP>
+__device__ __forceinline__ void row_scale(uint32_t top_bits, float square, int64_t cols, float eps, float &pre, float &inv, float &scale) {
+  const float top = __uint_as_float(top_bits);
+  // (127 / top must not overflow: rows of tiny numbers are made larger by a power of two first)
+  pre = top < 0x1p-100f ? 0x1p100f : 1.0f;
+  const bool bad = top_bits >= kInfBits || !(square < __builtin_inff());
+  inv = bad || top_bits == 0 ? 0.0f : 127.0f / (top * pre);
+  scale = top / 127.0f;
+  if constexpr (OP != kSiluMul) scale = scale * (1.0f / sqrtf(square / static_cast<float>(cols) + eps));
+  if (bad) scale = __builtin_nanf("");
+}
+
+// (the codes go by the row's largest value, not by what a 16-bit scale rounds to: its half a step of 2^-11 or 2^-8 is in every
+// value of the row alike)
+__device__ __forceinline__ void store_scale(const RowArgs &p, int64_t row, float scale) {
+  if (p.scale_type == QUIK_F32) static_cast<float *>(p.scale)[row] = scale;
+  else static_cast<uint16_t *>(p.scale)[row] = p.scale_type == QUIK_BF16 ? from_f32<true>(scale) : from_f32<false>(scale);
+}
+
+// q in the low byte: |u * inv| <= 127 (1 + 2^-23), and adding 1.5 * 2^23 rounds to nearest even at 1
+__device__ __forceinline__ uint32_t code_bits(float u, float inv) { return __float_as_uint(u * inv + 12582912.0f); }
+
+__device__ __forceinline__ float wave_sum_f(float v) {
+  v += dpp_move<kDppSwap1>(v);
+  v += dpp_move<kDppSwap2>(v);
+  v += dpp_move<kDppHalfMirror>(v);
+  v += dpp_move<kDppMirror>(v);
+  const int b = __builtin_bit_cast(int, v);
+  return (__builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16))) +
+         (__builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48)));
+}
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = umax(v, static_cast<uint32_t>(dpp_move_i<kDppSwap1>(static_cast<int>(v))));
+  v = umax(v, static_cast<uint32_t>(dpp_move_i<kDppSwap2>(static_cast<int>(v))));
+  v = umax(v, static_cast<uint32_t>(dpp_move_i<kDppHalfMirror>(static_cast<int>(v))));
+  v = umax(v, static_cast<uint32_t>(dpp_move_i<kDppMirror>(static_cast<int>(v))));
+  const uint32_t r0 = __builtin_amdgcn_readlane(v, 0), r1 = __builtin_amdgcn_readlane(v, 16), r2 = __builtin_amdgcn_readlane(v, 32),
+                 r3 = __builtin_amdgcn_readlane(v, 48);
+  return umax(umax(r0, r1), umax(r2, r3));
+}
+
+// top and square over the workgroup; `red` is free again when the next row's call comes (two barriers)
+template <int T>
+__device__ __forceinline__ void block_reduce(uint32_t &top, float &square, uint32_t *red) {
+  top = wave_max_u(top);
+  square = wave_sum_f(square);
+  if constexpr (T > 64) {
+    constexpr int W = T / 64;
+    float *reds = reinterpret_cast<float *>(red + W);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6] = top;
+      reds[threadIdx.x >> 6] = square;
+    }
+    __syncthreads();
+    top = red[0];
+    square = reds[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      top = umax(top, red[w]);
+      square += reds[w];
+    }
+  }
+}
+
+// One row per workgroup, held in registers: V chunks of VEC columns per thread (VEC 8: 16-byte accesses; 1: any alignment).
+template <bool BF16, RowOp OP, int T, int VEC, int V>
+__global__ __launch_bounds__(T) void rows8_kernel(RowArgs p) {
+  __shared__ uint32_t red[2 * (T / 64)];
+  const int tid = threadIdx.x;
+  const int chunks = static_cast<int>(p.cols / VEC);
+  const int64_t row = blockIdx.x;
+  const uint16_t *a = p.a + row * p.pitch_a;
+  const uint16_t *b = OP == kNorm ? nullptr : p.b + row * p.pitch_b;
+  float u[V][VEC];
+  uint32_t top = 0;
+  float square = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = tid + j * T;
+    if (c < chunks) {
+      alignas(16) uint16_t va[VEC], vb[VEC], vg[VEC], vh[VEC];
+      if constexpr (VEC == 8) {
+        *reinterpret_cast<uint4 *>(va) = *reinterpret_cast<const uint4 *>(a + c * 8);
+        if constexpr (OP != kNorm) *reinterpret_cast<uint4 *>(vb) = *reinterpret_cast<const uint4 *>(b + c * 8);
+        if constexpr (OP != kSiluMul) *reinterpret_cast<uint4 *>(vg) = *reinterpret_cast<const uint4 *>(p.gain + c * 8);
+      } else {
+        va[0] = a[c];
+        if constexpr (OP != kNorm) vb[0] = b[c];
+        if constexpr (OP != kSiluMul) vg[0] = p.gain[c];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        u[j][e] = row_value<BF16, OP>(to_f32<BF16>(va[e]), OP == kNorm ? 0.0f : to_f32<BF16>(vb[e]), OP == kSiluMul ? 0.0f : to_f32<BF16>(vg[e]),
+                                      vh[e], square);
+        top = umax(top, __float_as_uint(u[j][e]) & 0x7FFFFFFFu);
+      }
+      if constexpr (OP == kNormAdd) {
+        uint16_t *s = p.sum + row * p.cols + static_cast<int64_t>(c) * VEC;
+        if constexpr (VEC == 8)
+          *reinterpret_cast<uint4 *>(s) = *reinterpret_cast<const uint4 *>(vh);
+        else
+          s[0] = vh[0];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) u[j][e] = 0.0f;
+    }
+  }
+  block_reduce<T>(top, square, red);
+  float pre, inv, scale;
+  row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
+  if (tid == 0) store_scale(p, row, scale);
+  if (pre != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) u[j][e] *= pre;
+  }
+  if (inv == 0.0f) {  // (NaNs and infinities among the values: codes 0)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) u[j][e] = 0.0f;
+  }
+  int8_t *q = p.q + row * p.cols;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = tid + j * T;
+    if (c < chunks) {
+      if constexpr (VEC == 8) {
+        uint32_t w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float *v = &u[j][4 * k];
+          const uint32_t lo = __builtin_amdgcn_perm(code_bits(v[1], inv), code_bits(v[0], inv), 0x0C0C0400u);
+          const uint32_t hi = __builtin_amdgcn_perm(code_bits(v[3], inv), code_bits(v[2], inv), 0x04000C0Cu);
+          w[k] = lo | hi;
+        }
+        *reinterpret_cast<uint2 *>(q + c * 8) = make_uint2(w[0], w[1]);
+      } else {
+        q[c] = static_cast<int8_t>(code_bits(u[j][0], inv) & 0xFFu);
+      }
+    }
+  }
+}
+
+// Rows that no instance of the kernel above holds in registers: the row is read twice, the second time from the caches.
+template <bool BF16, RowOp OP>
+__global__ __launch_bounds__(1024) void rows8_long_kernel(RowArgs p) {
+  __shared__ uint32_t red[2 * 16];
+  const int64_t row = blockIdx.x;
+  const uint16_t *a = p.a + row * p.pitch_a;
+  const uint16_t *b = OP == kNorm ? nullptr : p.b + row * p.pitch_b;
+  uint32_t top = 0;
+  float square = 0.0f, unused = 0.0f;
+  uint16_t h = 0;
+  auto value = [&](int64_t c, float &sq) {
+    return row_value<BF16, OP>(to_f32<BF16>(a[c]), OP == kNorm ? 0.0f : to_f32<BF16>(b[c]), OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, sq);
+  };
+  for (int64_t c = threadIdx.x; c < p.cols; c += 1024) {
+    top = umax(top, __float_as_uint(value(c, square)) & 0x7FFFFFFFu);
+    if constexpr (OP == kNormAdd) p.sum[row * p.cols + c] = h;
+  }
+  block_reduce<1024>(top, square, red);
+  float pre, inv, scale;
+  row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
+  if (threadIdx.x == 0) store_scale(p, row, scale);
+  for (int64_t c = threadIdx.x; c < p.cols; c += 1024)
+    p.q[row * p.cols + c] = inv == 0.0f ? int8_t{0} : static_cast<int8_t>(code_bits(value(c, unused) * pre, inv) & 0xFFu);
+}
+
+template <bool BF16, RowOp OP>
+int launch(const RowArgs &p, bool wide, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.rows));
+  const int64_t chunks = p.cols / 8;
+#define QUIK_ROWS(T, VEC, V) hipLaunchKernelGGL((rows8_kernel<BF16, OP, T, VEC, V>), grid, dim3(T), 0, st, p)
+  if (wide && chunks <= 64) QUIK_ROWS(64, 8, 1);
+  else if (wide && chunks <= 128) QUIK_ROWS(128, 8, 1);
+  else if (wide && chunks <= 256) QUIK_ROWS(256, 8, 1);
+  else if (wide && chunks <= 512) QUIK_ROWS(512, 8, 1);
+  else if (wide && chunks <= 1024) QUIK_ROWS(1024, 8, 1);
+  else if (wide && chunks <= 2048) QUIK_ROWS(1024, 8, 2);
+  else if (wide && chunks <= 4096) QUIK_ROWS(1024, 8, 4);
+  else if (p.cols <= 256) QUIK_ROWS(64, 1, 4);
+  else if (p.cols <= 4096) QUIK_ROWS(256, 1, 16);
+  else if (p.cols <= 32768) QUIK_ROWS(1024, 1, 32);
+  else hipLaunchKernelGGL((rows8_long_kernel<BF16, OP>), grid, dim3(1024), 0, st, p);
+#undef QUIK_ROWS
+  return check_launch();
+}
+
+template <RowOp OP>
+int launch_typed(const RowArgs &p, int dtype, bool wide, hipStream_t st) {
+  return dtype == QUIK_BF16 ? launch<true, OP>(p, wide, st) : launch<false, OP>(p, wide, st);
+}
+
+bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// sizes that both operations check: rows in one grid, offsets of a row's elements in 63 bits
+int check_rows(int dtype, int scale_type, int64_t rows, int64_t cols, int64_t pitch_a, int64_t pitch_b) {
+  if (dtype != QUIK_F16 && dtype != QUIK_BF16) return QUIK_ERR_DTYPE;
+  if (scale_type != QUIK_F16 && scale_type != QUIK_BF16 && scale_type != QUIK_F32) return QUIK_ERR_DTYPE;
+  if (rows < 0 || cols <= 0 || (rows > 1 && (pitch_a < cols || pitch_b < cols))) return QUIK_ERR_SHAPE;
+  if (rows > INT32_MAX || cols > INT32_MAX) return QUIK_ERR_RANGE;
+  return QUIK_OK;
+}
+}  // namespace
+}  // namespace quik
+
+using namespace quik;
+
+extern "C" int quik_rms_norm_quantize(const void *x, int64_t x_pitch, const void *residual, int64_t residual_pitch, const void *gain,
+                                      float eps, int dtype, int64_t rows, int64_t cols, void *sum, int8_t *q, void *scale, int scale_type, void *stream) {
+  if (int rc = check_rows(dtype, scale_type, rows, cols, x_pitch, residual ? residual_pitch : cols)) return rc;
+  if (!(eps >= 0.0f)) return QUIK_ERR_RANGE;
+  if (rows == 0) return QUIK_OK;
+  if (!x || !gain || !q || !scale || (residual && !sum)) return QUIK_ERR_NULL;
+  if (!aligned(x, 2) || !aligned(residual, 2) || !aligned(gain, 2) || !aligned(sum, 2) || !aligned(scale, scale_type == QUIK_F32 ? 4 : 2)) return QUIK_ERR_ALIGN;
+  const RowArgs p{static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(residual), static_cast<const uint16_t *>(gain), rows, cols,
+                  x_pitch, residual_pitch, eps, static_cast<uint16_t *>(sum), q, scale, scale_type};
+  const bool wide = cols % 8 == 0 && aligned(x, 16) && aligned(gain, 16) && aligned(q, 8) && (rows == 1 || x_pitch % 8 == 0) &&
+                    (!residual || (aligned(residual, 16) && aligned(sum, 16) && (rows == 1 || residual_pitch % 8 == 0)));
+  return residual ? launch_typed<kNormAdd>(p, dtype, wide, as_stream(stream)) : launch_typed<kNorm>(p, dtype, wide, as_stream(stream));
+}
+
+extern "C" int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up, int64_t up_pitch, int dtype, int64_t rows,
+                                      int64_t cols, int8_t *q, void *scale, int scale_type, void *stream) {
+  if (int rc = check_rows(dtype, scale_type, rows, cols, gate_pitch, up_pitch)) return rc;
+  if (rows == 0) return QUIK_OK;
+  if (!gate || !up || !q || !scale) return QUIK_ERR_NULL;
+  if (!aligned(gate, 2) || !aligned(up, 2) || !aligned(scale, scale_type == QUIK_F32 ? 4 : 2)) return QUIK_ERR_ALIGN;
+  const RowArgs p{static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up), nullptr, rows, cols, gate_pitch, up_pitch, 0.0f,
+                  nullptr, q, scale, scale_type};
+  const bool wide = cols % 8 == 0 && aligned(gate, 16) && aligned(up, 16) && aligned(q, 8) &&
+                    (rows == 1 || (gate_pitch % 8 == 0 && up_pitch % 8 == 0));
+  return launch_typed<kSiluMul>(p, dtype, wide, as_stream(stream));
+}

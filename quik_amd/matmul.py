@@ -16,7 +16,7 @@ from . import _lib as L
 
 __all__ = ["int4Matmul", "int8Matmul", "mixed_linear", "pack_weight_fp6", "mixed_linear_fp6", "mixed_linear_tile4",
            "pack_weight_tile8",
-           "mixed_linear_tile8"]
+           "mixed_linear_tile8", "int4GroupMatmul"]
 
 
 def _matmul(op, A, B, want_dtype, sym, kmul):
@@ -315,4 +315,52 @@ def mixed_linear_tile8(x8, w8, meta, weights_scales, reduced_w, bias, M, N, K, F
                                                    L.ptr(tensors.get("reduced_w")), L.ptr(tensors.get("bias")), dt, M, N,
                                                    K, F, L.ptr(out), L.ptr(ws), ws_bytes, L.stream()),
                 "mixed_linear_tile8")
+    return out
+
+
+def int4GroupMatmul(x, weight, scales, group_size, zeros=None, scale_row=None, bias=None):
+    """4-bit weights with one scale (and zero) per group_size columns of a row:
+    out[m, n] = sum_k x[m, k] * (q[n, k] - zeros[n, g]) * scales[n, g] (* scale_row[m]) (+ bias[n]), g = k // group_size.
+
+    x [M, K] of the scales' type, or int8 with scale_row [M, 1] float32 (symmetric.rms_norm_quantize, silu_mul_quantize); weight [N,
+    K/2] uint8, signed codes, low nibble = even k (qlinear.pack_to_i4); scales [N, ceil(K / group_size)] fp16 or bf16; zeros the
+    same shape and type; bias [N].  K and group_size are multiples of 32; the last group may be shorter.  Returns [M, N] of the
+    scales' type; sums in fp32, one rounding."""
+    op = "int4GroupMatmul"
+    out = L.front().int4_group_matmul(x, weight, scales, group_size, zeros, scale_row, bias)
+    if out is not None:
+        return out
+    tensors = dict(x=x, weight=weight, scales=scales)
+    tensors.update((name, t) for name, t in (("zeros", zeros), ("scale_row", scale_row), ("bias", bias)) if t is not None)
+    dev = L.check_cuda_contiguous(op, **tensors)
+    dt = L.dtype_id(scales, op, allow_bf16=True)
+    if weight.dtype != torch.uint8:
+        raise RuntimeError(f"{op}: expected weight of dtype torch.uint8 but got {weight.dtype}")
+    if x.dtype != scales.dtype and x.dtype != torch.int8:
+        raise RuntimeError(f"{op}: expected x of dtype {scales.dtype} or torch.int8 but got {x.dtype}")
+    if (x.dtype == torch.int8) != (scale_row is not None):
+        raise RuntimeError(f"{op}: scale_row belongs to int8 activations (x is {x.dtype}, scale_row is "
+                           f"{'missing' if scale_row is None else 'given'})")
+    if scale_row is not None and scale_row.dtype != torch.float32:
+        raise RuntimeError(f"{op}: expected scale_row of dtype torch.float32 but got {scale_row.dtype}")
+    for name, t in (("zeros", zeros), ("bias", bias)):
+        if t is not None and t.dtype != scales.dtype:
+            raise RuntimeError(f"{op}: expected {name} of dtype {scales.dtype} but got {t.dtype}")
+    if x.dim() != 2 or weight.dim() != 2 or x.size(1) != 2 * weight.size(1):
+        raise RuntimeError(f"{op}: x [M, K] and weight [N, K/2] must agree in K, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    (M, K), N = x.shape, weight.size(0)
+    if K == 0 or K % 32 or group_size <= 0 or group_size % 32:
+        raise RuntimeError(f"{op}: K and group_size must be multiples of 32, got {K} and {group_size}")
+    for name, t, shape in (("scales", scales, (N, -(-K // group_size))), ("zeros", zeros, (N, -(-K // group_size)))):
+        if t is not None and t.shape != torch.Size(shape):
+            raise RuntimeError(f"{op}: expected {name} to have size {shape}, got {tuple(t.shape)}")
+    if scale_row is not None and scale_row.numel() != M:
+        raise RuntimeError(f"{op}: expected scale_row to have {M} elements but got {scale_row.numel()}")
+    if bias is not None and bias.numel() != N:
+        raise RuntimeError(f"{op}: expected bias to have {N} elements but got {bias.numel()}")
+    lib = L.load()
+    with L.device_guard(dev):
+        out = torch.empty((M, N), dtype=scales.dtype, device=dev)
+        L.check(lib.quik_int4_group_matmul(L.ptr(x), 8 if x.dtype == torch.int8 else 16, L.ptr(weight), L.ptr(scales), L.ptr(zeros),
+                                           L.ptr(scale_row), L.ptr(bias), dt, M, N, K, group_size, L.ptr(out), L.stream()), op)
     return out

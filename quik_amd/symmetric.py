@@ -11,7 +11,8 @@ import torch
 
 from . import _lib as L
 
-__all__ = ["quantize", "dequantize", "int4FusedDequantize", "int8FusedDequantize", "quantize_mapped"]
+__all__ = ["quantize", "dequantize", "int4FusedDequantize", "int8FusedDequantize", "quantize_mapped", "rms_norm_quantize",
+           "silu_mul_quantize"]
 
 
 def quantize(src: torch.Tensor, scale: torch.Tensor, bits: int = 4) -> torch.Tensor:
@@ -134,3 +135,78 @@ def quantize_mapped(src: torch.Tensor, colmap: torch.Tensor, num_int: int, num_f
                                              L.ptr(fp_x) if fp_x is not None and num_fp else None, L.stream()),
                 "quantize")
     return dst, scale, fp_x
+
+
+_SCALE_TYPE = {torch.float32: L.QUIK_F32, torch.float16: L.QUIK_F16, torch.bfloat16: L.QUIK_BF16}
+
+
+def _scale_type(op, scale_dtype):
+    if scale_dtype not in _SCALE_TYPE:
+        raise RuntimeError(f"{op}: expected scale_dtype to be float32, float16 or bfloat16 but got {scale_dtype}")
+    return _SCALE_TYPE[scale_dtype]
+
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor = None,
+                      scale_dtype: torch.dtype = torch.float32):
+    """Root-mean-square norm with 8-bit rows as its output, in one launch: h = x + residual (rounded to x's type; residual None:
+    h = x), value = h / sqrt(mean(h^2) + eps) * weight; q int8 [rows, cols] and scale [rows, 1] with value ~ q * scale, a row's
+    largest magnitude at 127.  Returns (q, scale, h), h None without a residual; h is the next residual.
+
+    x, residual [rows, cols] fp16 or bf16 (rows may lie apart), weight [cols] of the same type.  The scale is fp32;
+    scale_dtype=torch.float16 gives what int8FusedDequantize and dequantize take.  A row with a NaN or an infinity has codes 0 and
+    a NaN scale."""
+    op = "rms_norm_quantize"
+    out = L.front().rms_norm_quantize(x, weight, eps, residual, scale_dtype)
+    if out is not None:
+        return out
+    rows_of = dict(x=x) if residual is None else dict(x=x, residual=residual)
+    dev = L.check_cuda_rows(op, **rows_of)
+    if L.check_cuda_contiguous(op, weight=weight) != dev:
+        raise RuntimeError(f"{op}: expected all tensors on the same GPU, but 'weight' is on {weight.device} and x is on {dev}")
+    dt = L.dtype_id(x, op, allow_bf16=True)
+    rows, cols = x.shape
+    for name, t, shape in (("residual", residual, x.shape), ("weight", weight, (cols,))):
+        if t is not None and t.dtype != x.dtype:
+            raise RuntimeError(f"{op}: expected {name} of dtype {x.dtype} but got {t.dtype}")
+        if t is not None and t.shape != torch.Size(shape):
+            raise RuntimeError(f"{op}: expected {name} to have size {tuple(shape)}, got {tuple(t.shape)}")
+    if cols == 0:
+        raise RuntimeError(f"{op}: rows of no columns have no norm")
+    if not eps >= 0:
+        raise RuntimeError(f"{op}: expected eps to be at least 0 but got {eps}")
+    st = _scale_type(op, scale_dtype)
+    lib = L.load()
+    with L.device_guard(dev):
+        q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+        scale = torch.empty((rows, 1), dtype=scale_dtype, device=dev)
+        h = None if residual is None else torch.empty((rows, cols), dtype=x.dtype, device=dev)
+        L.check(lib.quik_rms_norm_quantize(L.ptr(x), x.stride(0), L.ptr(residual), 0 if residual is None else residual.stride(0),
+                                           L.ptr(weight), eps, dt, rows, cols, L.ptr(h), L.ptr(q), L.ptr(scale), st, L.stream()), op)
+    return q, scale, h
+
+
+def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor, scale_dtype: torch.dtype = torch.float32):
+    """value = gate * sigmoid(gate) * up in 8-bit rows, in one launch: returns (q int8 [rows, cols], scale [rows, 1]) with value ~
+    q * scale, a row's largest magnitude at 127.  gate and up [rows, cols] of one type, fp16 or bf16; their rows may lie apart
+    (the two halves of one product).  scale_dtype and rows with a NaN or an infinity as in rms_norm_quantize."""
+    op = "silu_mul_quantize"
+    out = L.front().silu_mul_quantize(gate, up, scale_dtype)
+    if out is not None:
+        return out
+    dev = L.check_cuda_rows(op, gate=gate, up=up)
+    dt = L.dtype_id(gate, op, allow_bf16=True)
+    if up.dtype != gate.dtype:
+        raise RuntimeError(f"{op}: expected up of dtype {gate.dtype} but got {up.dtype}")
+    if up.shape != gate.shape:
+        raise RuntimeError(f"{op}: expected gate and up to have the same size, got {tuple(gate.shape)} and {tuple(up.shape)}")
+    rows, cols = gate.shape
+    if cols == 0:
+        raise RuntimeError(f"{op}: rows of no columns have no scale")
+    st = _scale_type(op, scale_dtype)
+    lib = L.load()
+    with L.device_guard(dev):
+        q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+        scale = torch.empty((rows, 1), dtype=scale_dtype, device=dev)
+        L.check(lib.quik_silu_mul_quantize(L.ptr(gate), gate.stride(0), L.ptr(up), up.stride(0), dt, rows, cols, L.ptr(q),
+                                           L.ptr(scale), st, L.stream()), op)
+    return q, scale

@@ -1,0 +1,139 @@
+"""matmul.int4GroupMatmul against its formula in 64 bits.
+
+Tolerance of one value: half a step of the result's type, and the roundings of the sums.  A group's 32-column steps and the groups
+themselves are added one after the other in fp32, each product exact: at most `32 + K / 32 + 24` additions of 2^-24 each of
+sum |x| (|q| + c) s, with c the constant that the widened codes carry and zero points add: 136 for bf16 (its codes are widened to 136 +
+q), |z| for zeros.  int8 activations: the groups' sums are exact, the groups are added in fp32."""
+import numpy as np
+import pytest
+import torch
+
+import quik
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def make(M, N, K, G, acts, dtype, zeros=False, bias=False, seed=0, whole=True):
+    g = torch.Generator().manual_seed(seed + M + N + K + G)
+    groups = -(-K // G)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    s = (torch.rand(N, groups, generator=g) * 0.009 + 0.001).to(dtype)
+    z = None
+    if zeros:
+        z = torch.randint(-8, 8, (N, groups), generator=g).to(dtype) if whole else (torch.rand(N, groups, generator=g) * 16 - 8).to(dtype)
+    sr = None
+    if acts == torch.int8:
+        x = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8)
+        sr = torch.rand(M, 1, generator=g) * 0.02 + 0.01
+    else:
+        x = torch.randn(M, K, generator=g)
+        x[:, ::128] *= 10
+        x = x.to(acts)
+    b = torch.randn(N, generator=g).to(dtype) if bias else None
+    move = lambda t: None if t is None else t.to(DEV)
+    return tuple(move(t) for t in (x, w, s, z, sr, b))
+
+
+def oracle(x, w, s, z, sr, b, G):
+    """(value, sum of magnitudes) in 64 bits"""
+    up = lambda t: t.double().cpu().numpy()
+    by = w.cpu().numpy()
+    q = np.empty((by.shape[0], 2 * by.shape[1]))
+    q[:, 0::2], q[:, 1::2] = ((by & 15) ^ 8).astype(int) - 8, ((by >> 4) ^ 8).astype(int) - 8
+    at = np.arange(q.shape[1]) // G
+    zz = 0 if z is None else up(z)[:, at]
+    extra = (136 if x.dtype == torch.bfloat16 else 0) + np.abs(zz)
+    y = up(x) @ ((q - zz) * up(s)[:, at]).T
+    size = np.abs(up(x)) @ ((np.abs(q) + extra) * up(s)[:, at]).T
+    if sr is not None:
+        y, size = y * up(sr).reshape(-1, 1), size * up(sr).reshape(-1, 1)
+    if b is not None:
+        y = y + up(b)
+    return y, size
+
+
+def check(out, args, G):
+    y, size = oracle(*args, G)
+    K = args[0].shape[1]
+    half = torch.finfo(out.dtype).eps / 2
+    got = out.double().cpu().numpy()
+    assert got.shape == y.shape
+    adds = 32 + K / 32 + 24 if args[0].dtype != torch.int8 else K / 32 + 24
+    assert (np.abs(got - y) <= half * np.abs(y) + adds * 2.0 ** -24 * (size + np.abs(y))).all()
+    if y.size > 64:
+        assert np.linalg.norm(got - y) <= half * np.linalg.norm(y)
+
+
+def call(args, G):
+    x, w, s, z, sr, b = args
+    return quik.matmul.int4GroupMatmul(x, w, s, G, zeros=z, scale_row=sr, bias=b)
+
+
+# every number of token rows per matrix tile and its ends; columns that fill no tile; K that ends inside a block of 128
+SIZES = [(1, 1, 32), (1, 16, 128), (1, 33, 4096), (2, 100, 160), (3, 7, 1024), (4, 64, 992), (5, 40, 256), (8, 200, 2080), (9, 31, 512),
+         (16, 65, 1056), (17, 48, 640), (32, 130, 384), (33, 17, 96), (63, 129, 1184), (64, 512, 256), (65, 70, 544), (100, 300, 1024),
+         (128, 128, 2048), (129, 257, 416), (300, 141, 768), (515, 96, 1280)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_sizes(M, N, K, codes, dtype):
+    args = make(M, N, K, 128, torch.int8 if codes else dtype, dtype)
+    check(call(args, 128), args, 128)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("G", [32, 64, 96, 128, 160, 256, 384, 1 << 20])
+@pytest.mark.parametrize("M,N,K", [(1, 50, 1120), (6, 80, 2048), (13, 33, 352), (40, 96, 1184), (150, 130, 1120)])
+def test_groups(M, N, K, G, zeros, codes, dtype):
+    args = make(M, N, K, G, torch.int8 if codes else dtype, dtype, zeros, bias=G == 64)
+    check(call(args, G), args, G)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("M,N,K", [(1, 257, 11008), (16, 128, 13824), (70, 160, 8192)])
+def test_long_rows_zeros_between_codes_and_bias(M, N, K, codes, dtype):
+    args = make(M, N, K, 128, torch.int8 if codes else dtype, dtype, True, True, whole=False)
+    check(call(args, 128), args, 128)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("M", [1, 4, 12, 50, 200])
+def test_extreme_codes(M, codes):
+    """Every code at its lowest: the largest sums that there are; and rows of zeros."""
+    x, w, s, z, sr, b = make(M, 40, 2048, 128, torch.int8 if codes else torch.float16, torch.float16)
+    w.fill_(0x88)
+    x.fill_(-128 if codes else 2)
+    s.fill_(0.0009765625)
+    if codes:
+        sr.fill_(0.015625)
+    out = call((x, w, s, z, sr, b), 128)
+    want = 8 * 128 * 2048 / 1024 / 64 if codes else -8 * 2 * 2048 / 1024
+    assert (out == want).all()
+    assert not call((torch.zeros_like(x), w, s, z, sr, b), 128).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 7, 16, 60, 140])
+def test_a_row_that_is_no_number_stays_alone(M, dtype):
+    args = make(M, 70, 608, 128, dtype, dtype, True)
+    want = call(args, 128)
+    for bad in (float("nan"), float("inf")):
+        x = args[0].clone()
+        x[M // 2, 607] = bad
+        got = call((x,) + args[1:], 128)
+        assert not got[M // 2].isfinite().any()
+        keep = torch.arange(M, device=DEV) != M // 2
+        assert torch.equal(got[keep], want[keep])
+
+
+def test_empty():
+    args = make(1, 40, 128, 128, torch.float16, torch.float16)
+    assert call((args[0][:0],) + args[1:], 128).shape == (0, 40)
+    assert call((args[0], args[1][:0], args[2][:0], None, None, None), 128).shape == (1, 0)
