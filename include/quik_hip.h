@@ -411,12 +411,16 @@ int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up,
  *   w       [N, K/2] uint8, signed int4 codes, low nibble = even k (MixedQLinear.int_weight, pack_to_i4)
  *   scales  [N, ceil(K / group)] dtype; zeros the same shape in units of a code (any number, not only whole ones), or NULL
  *   bias    [N] dtype or NULL; out [M, N] dtype
- * K % 32 == 0, group % 32 == 0 (a group >= K: one scale per output column; the last group may be shorter); x and w 16-byte
+ * K % 32 == 0, K <= 2^20, group % 32 == 0 (a group >= K: one scale per output column; the last group may be shorter); x and w 16-byte
  * aligned.  A group's product is summed in fp32 (int8: exactly) and scaled in fp32; one rounding to dtype.  A row of x that
  * holds an infinity gives infinities or NaNs. */
 int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const void *scales, const void *zeros,
                            const float *scale_row, const void *bias, int dtype, int64_t M, int64_t N, int64_t K,
-                           int64_t group, void *out, void *stream);
+                           int64_t group, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+/* Calls of more than 16 rows whose tiles leave CUs idle split K: workspace (16-byte aligned, not to be shared by calls that may
+ * overlap, free again behind the call on the stream) then holds the sums of each part, which a second launch adds in order.  Bytes
+ * that such a call makes use of, 0: none.  With NULL or fewer bytes K is not split: slower, the same result within its rounding. */
+int64_t quik_int4_group_matmul_workspace_bytes(int x_bits, int dtype, int64_t M, int64_t N, int64_t K);
 
 #ifdef __cplusplus
 }

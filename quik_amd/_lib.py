@@ -71,7 +71,8 @@ SIGNATURES = {
                                      _vp, _vp]),
     "quik_rms_norm_quantize": (_int, [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _int, _i64, _i64, _vp, _vp, _vp, _int, _vp]),
     "quik_silu_mul_quantize": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _vp, _int, _vp]),
-    "quik_int4_group_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "quik_int4_group_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "quik_int4_group_matmul_workspace_bytes": (_i64, [_int, _int, _i64, _i64, _i64]),
 }
 
 TILED_4 = 0x344C5451    # QUIK_TILED_4: operand buffers, tiled weights of 4 bits

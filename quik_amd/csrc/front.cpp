@@ -691,9 +691,12 @@ PyObject *py_int4_group_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) 
     Py_RETURN_NONE;
   return guarded([&]() -> PyObject * {
     at::Tensor out = new_empty({M, N}, s->scalar_type(), dev);
+    const int64_t need = quik_int4_group_matmul_workspace_bytes(codes ? 8 : 16, dt, M, N, K);
+    c10::DataPtr ws;
+    if (need) ws = c10::hip::HIPCachingAllocator::get()->allocate(static_cast<size_t>(need));
     const int rc = quik_int4_group_matmul(data_of(*x), codes ? 8 : 16, static_cast<const uint8_t *>(data_of(*w)), data_of(*s),
                                           z ? data_of(*z) : nullptr, sr ? static_cast<const float *>(data_of(*sr)) : nullptr,
-                                          b ? data_of(*b) : nullptr, dt, M, N, K, group, out_ptr(out), stream_of(dev));
+                                          b ? data_of(*b) : nullptr, dt, M, N, K, group, out_ptr(out), ws.get(), need, stream_of(dev));
     if (rc != QUIK_OK) return fail("int4GroupMatmul", rc);
     return THPVariable_Wrap(std::move(out));
   });

@@ -361,6 +361,9 @@ def int4GroupMatmul(x, weight, scales, group_size, zeros=None, scale_row=None, b
     lib = L.load()
     with L.device_guard(dev):
         out = torch.empty((M, N), dtype=scales.dtype, device=dev)
-        L.check(lib.quik_int4_group_matmul(L.ptr(x), 8 if x.dtype == torch.int8 else 16, L.ptr(weight), L.ptr(scales), L.ptr(zeros),
-                                           L.ptr(scale_row), L.ptr(bias), dt, M, N, K, group_size, L.ptr(out), L.stream()), op)
+        bits = 8 if x.dtype == torch.int8 else 16
+        need = lib.quik_int4_group_matmul_workspace_bytes(bits, dt, M, N, K)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        L.check(lib.quik_int4_group_matmul(L.ptr(x), bits, L.ptr(weight), L.ptr(scales), L.ptr(zeros), L.ptr(scale_row), L.ptr(bias), dt, M,
+                                           N, K, group_size, L.ptr(out), L.ptr(ws), need, L.stream()), op)
     return out

@@ -36,16 +36,16 @@ def test_activation_checks_its_arguments():
 
 
 def test_product_checks_its_arguments():
-    def f(x=one, bits=16, w=one, s=one, z=null, sr=null, b=null, dt=0, M=4, N=8, K=256, G=128, out=one):
-        return _lib().quik_int4_group_matmul(x, bits, w, s, z, sr, b, dt, M, N, K, G, out, null)
+    def f(x=one, bits=16, w=one, s=one, z=null, sr=null, b=null, dt=0, M=4, N=8, K=256, G=128, out=one, ws=null):
+        return _lib().quik_int4_group_matmul(x, bits, w, s, z, sr, b, dt, M, N, K, G, out, ws, 0, null)
     assert f(M=0) == 0 and f(N=0) == 0
     assert f(bits=4) == -1 and f(dt=2) == -3
     assert f(M=-1) == -2 and f(N=-1) == -2 and f(K=0) == -2 and f(G=0) == -2 and f(G=-32) == -2
     assert f(K=240) == -4 and f(G=48) == -4
-    assert f(K=1 << 31) == -6 and f(N=1 << 31) == -6 and f(M=1 << 31) == -6
+    assert f(K=(1 << 20) + 32) == -6 and f(N=1 << 31) == -6 and f(M=1 << 31) == -6
     assert f(x=null) == -5 and f(w=null) == -5 and f(s=null) == -5 and f(out=null) == -5 and f(bits=8) == -5
     at8 = ctypes.c_void_p(264)
-    assert f(x=at8) == -4 and f(w=at8) == -4 and f(s=odd) == -4 and f(z=odd) == -4 and f(b=odd) == -4 and f(out=odd) == -4
+    assert f(x=at8) == -4 and f(w=at8) == -4 and f(s=odd) == -4 and f(z=odd) == -4 and f(b=odd) == -4 and f(out=odd) == -4 and f(ws=at8) == -4
     assert f(bits=8, sr=ctypes.c_void_p(258)) == -4
 
 
@@ -88,3 +88,11 @@ def test_shapes_types_and_layouts():
     shifted = torch.zeros(2 * 64 + 1, dtype=torch.float16, device=dev)[1:].view(2, 64)
     with pytest.raises(RuntimeError, match="alignment"):
         quik.matmul.int4GroupMatmul(shifted, p, s, 64)
+
+
+def test_product_says_what_it_makes_use_of():
+    f = _lib().quik_int4_group_matmul_workspace_bytes
+    assert f(16, 0, 16, 4096, 4096) == 0 and f(16, 0, 0, 4096, 4096) == 0 and f(8, 0, 64, 0, 4096) == 0
+    assert f(16, 0, 2048, 8192, 8192) == 0                        # tiles for every CU
+    n = f(8, 1, 64, 5121, 13824)                                  # few tiles, long rows: whole parts of [64, 5124] sums
+    assert n > 0 and n % (64 * 5124 * 4) == 0

@@ -103,6 +103,37 @@ def test_long_rows_zeros_between_codes_and_bias(M, N, K, codes, dtype):
     check(call(args, 128), args, 128)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("G,zeros", [(128, False), (64, True), (32, True)])
+def test_the_widest_tiles(G, zeros, codes, dtype):
+    """Rows and columns for the tiles of 128 x 256, ending inside one on both sides; K that ends inside a block."""
+    args = make(1030, 8197, 2080, G, torch.int8 if codes else dtype, dtype, zeros)
+    check(call(args, G), args, G)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("M,N,K,G", [(20, 130, 4096, 128), (64, 516, 8224, 64), (90, 257, 6016, 128)])
+def test_split_rows(M, N, K, G, codes, dtype):
+    """K split over workgroups, and the same call without the memory for it."""
+    from quik_amd import _lib as L
+    args = make(M, N, K, G, torch.int8 if codes else dtype, dtype, True, True)
+    x, w, s, z, sr, b = args
+    lib, dt, bits = L.load(), L.dtype_id(s, "", True), 8 if codes else 16
+    need = lib.quik_int4_group_matmul_workspace_bytes(bits, dt, M, N, K)
+    assert need > 0
+    split = call(args, G)
+    check(split, args, G)
+    out = torch.empty_like(split)
+    for ws, size in ((None, 0), (torch.empty(need, dtype=torch.uint8, device=DEV), need - 1)):
+        out.fill_(7)
+        L.check(lib.quik_int4_group_matmul(L.ptr(x), bits, L.ptr(w), L.ptr(s), L.ptr(z), L.ptr(sr), L.ptr(b), dt, M, N, K, G, L.ptr(out), L.ptr(ws),
+                                           size, L.stream()), "")
+        check(out, args, G)
+    assert torch.equal(split, call(args, G))
+
+
 @pytest.mark.parametrize("codes", [False, True])
 @pytest.mark.parametrize("M", [1, 4, 12, 50, 200])
 def test_extreme_codes(M, codes):
