@@ -403,13 +403,20 @@ struct TileShape {
   static constexpr int kMyX = (kX + kW - 1) / kW, kMyW = (kWt + kW - 1) / kW, kMyS = (kS + kW - 1) / kW;
   static constexpr int kCopies = kMyX + kMyW + kMyS * (ZEROS ? 2 : 1);
   static constexpr int kReduce = WK > 1 ? WM * WN * WK * RM * RN * 1024 : 0;
-  static constexpr int kLds = D * kStage > kReduce ? D * kStage : kReduce;
+  static constexpr bool kSums = ZEROS || XT == kBF16;
+  // Sums of the activations: of eight row tiles the waves side by side make one each and take the others' a step later (us at 2048 x 4096 ->
+  // 11008, each wave all of them and this: bf16 267, 256, fp16 with zeros 292, 258); of fewer each wave makes all that it needs (64 x 4096
+  // -> 11008 bf16 with zeros, so and shared: 22.7, 26.3).
+  static constexpr bool kShared = kSums && RM >= 8, kOwnSums = kSums && !kShared;
+  static constexpr int kAtSums = D * kStage, kRings = kAtSums + (kShared ? 2 * WK * PARTS * kBM * 4 : 0);  // of two steps
+  static constexpr int kLds = kRings > kReduce ? kRings : kReduce;
+  static_assert(!kShared || WN >= RM, "");
 };
 
 template <int XT, int RM, int RN, int WM, int WN, int WK, int D, int PARTS, bool ZEROS>
 __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArgs p) {
   using S = TileShape<XT, RM, RN, WM, WN, WK, D, PARTS, ZEROS>;
-  constexpr bool kSums = ZEROS || XT == kBF16;
+  constexpr bool kShared = S::kShared, kOwnSums = S::kOwnSums;
   constexpr bool kTurn = PARTS > 1;  // matrix step s: columns 32 s .. of the block; else columns 8 s .. of each lane row's 32
   constexpr int kRowPieces = S::kRowBytes / 16, kSize = is_i8(XT) ? 1 : 2;
   extern __shared__ float red[];
@@ -517,6 +524,44 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier: what was read of LDS is read)
   };
+  // Sums of the activations of a part (columns of one group), by a matrix of ones: what the zeros and the offset of widened bf16 codes are
+  // multiplied by.
+  float *const sums = reinterpret_cast<float *>(lds + S::kAtSums);
+  float less[kShared ? PARTS : 1][RN][4];  // -scale * (offset + zero) of the step before
+  auto sums_of = [&](int step, int part) { return sums + (((step & 1) * WK + wk) * PARTS + part) * S::kBM + wm * 16 * RM + col; };
+  auto add_ones = [&](auto x, Acc<XT> v) {
+    if constexpr (sizeof(x) == 8) return __builtin_amdgcn_mfma_i32_16x16x32_i8(0x0101010101010101l, __builtin_bit_cast(long, x), v, 0, 0, 0);
+    else if constexpr (is_i8(XT)) return __builtin_amdgcn_mfma_i32_16x16x64_i8(i32x4{0x01010101, 0x01010101, 0x01010101, 0x01010101}, __builtin_bit_cast(i32x4, x), v, 0, 0, 0);
+    else return mfma32<XT>(XT == kBF16 ? u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u} : u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}, __builtin_bit_cast(u32x4, x), v);
+  };
+  auto sum = [&](const uint8_t *from, int step, int part, int64_t k0) {
+    const int own = wn % RM;
+    Acc<XT> v = Acc<XT>{0, 0, 0, 0};
+    constexpr int kSteps = is_i8(XT) && !kTurn ? 2 : 4;
+#pragma unroll
+    for (int s = part * kSteps / PARTS; s < (part + 1) * kSteps / PARTS; ++s) {
+      if (PARTS == 2 && k0 + 32 * s >= p.K) break;
+      if constexpr (is_i8(XT) && kTurn) v = add_ones(x_half(from, own, s), v);
+      else v = add_ones(x_piece_of(from, own, s), v);
+    }
+    if (kg == 0) sums_of(step, part)[16 * own] = static_cast<float>(v[0]);
+  };
+  auto correct = [&](int step) {
+    const int64_t k0 = (static_cast<int64_t>(step) * WK + wk) * 128;
+    if (WK > 1 && k0 >= p.K) return;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      if (kTurn && k0 + 128 / PARTS * part >= p.K) break;
+#pragma unroll
+      for (int t = 0; t < RM; ++t) {
+        const float v = sums_of(step, part)[16 * t];
+#pragma unroll
+        for (int f = 0; f < RN; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) total[t][f][r] = __builtin_fmaf(less[part][f][r], v, total[t][f][r]);
+      }
+    }
+  };
   auto multiply = [&](int step) {
     const int64_t k0 = (static_cast<int64_t>(step) * WK + wk) * 128;
     if (WK > 1 && k0 >= p.K) return;
@@ -530,10 +575,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
         if (kTurn && k0 + 128 / PARTS * part >= p.K) break;
-        Acc<XT> acc[RM][RN], sums[RM];
+        if constexpr (kShared) sum(from, step, part, k0);
+        Acc<XT> acc[RM][RN], own[kOwnSums ? RM : 1];
+        __builtin_amdgcn_s_setprio(1);  // a wave among its products before one that widens codes for its next
 #pragma unroll
         for (int t = 0; t < RM; ++t) {
-          sums[t] = Acc<XT>{0, 0, 0, 0};
+          if constexpr (kOwnSums) own[t] = Acc<XT>{0, 0, 0, 0};
 #pragma unroll
           for (int f = 0; f < RN; ++f) acc[t][f] = Acc<XT>{0, 0, 0, 0};
         }
@@ -545,7 +592,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = __builtin_bit_cast(long, x_half(from, t, s));
-              if constexpr (kSums) sums[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(0x0101010101010101l, xa[t], sums[t], 0, 0, 0);
+              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -555,14 +602,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
             }
           }
         } else if constexpr (is_i8(XT)) {
-          const int one = 0x01010101;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             i32x4 xa[RM];
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = __builtin_bit_cast(i32x4, x_piece_of(from, t, s));
-              if constexpr (kSums) sums[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(i32x4{one, one, one, one}, xa[t], sums[t], 0, 0, 0);
+              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -573,7 +619,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
             }
           }
         } else {
-          const uint32_t one = XT == kBF16 ? 0x3F803F80u : 0x3C003C00u;
 #pragma unroll
           for (int s = part * 4 / PARTS; s < (part + 1) * 4 / PARTS; ++s) {
             if (PARTS == 2 && k0 + 32 * s >= p.K) break;
@@ -581,7 +626,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = x_piece_of(from, t, s);
-              if constexpr (kSums) sums[t] = mfma32<XT>(u32x4{one, one, one, one}, xa[t], sums[t]);
+              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -591,28 +636,32 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
             }
           }
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int f = 0; f < RN; ++f) {
           // (four bytes each, the value in the low half; kTurn: 16 columns at the block's four units of 32)
           const int at = (kTurn ? (wk * (S::kBN / 16) + wn * RN + f) * 64 + part * (64 / PARTS) : wk * (S::kS / WK) * 64 + (wn * RN + f) * 16) + 4 * kg;
           const u32x4 sw = *reinterpret_cast<const u32x4 *>(from_s + 4 * at);
-          float s[4], z[4];
+          float s[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[r] = from16(sw[r], sbf);
-            z[r] = XT == kBF16 ? 136.0f : 0.0f;
-          }
+          for (int r = 0; r < 4; ++r) s[r] = from16(sw[r], sbf);
+          constexpr float kOffset = XT == kBF16 ? 136.0f : 0.0f, kUnit = is_i8(XT) ? 16.0f : 1.0f;
+          float z[4] = {kOffset, kOffset, kOffset, kOffset};
           if constexpr (ZEROS) {
             const u32x4 zw = *reinterpret_cast<const u32x4 *>(from_s + (S::kAtZ - S::kAtS) + 4 * at);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[r] += from16(zw[r], sbf) * (is_i8(XT) ? 16.0f : 1.0f);
+            for (int r = 0; r < 4; ++r) z[r] += kUnit * from16(zw[r], sbf);
+          }
+          if constexpr (kShared) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) less[part][f][r] = -s[r] * z[r];
           }
 #pragma unroll
           for (int t = 0; t < RM; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               float d = static_cast<float>(acc[t][f][r]);
-              if constexpr (kSums) d = __builtin_fmaf(-z[r], static_cast<float>(sums[t][0]), d);
+              if constexpr (kOwnSums) d = __builtin_fmaf(-z[r], static_cast<float>(own[t][0]), d);
               total[t][f][r] = __builtin_fmaf(s[r], d, total[t][f][r]);
             }
         }
@@ -624,7 +673,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   for (int step = first; step < steps; ++step) {
     arrive(step);
     if (step + D - 1 < steps) copy(step + D - 1);
+    if (kShared && step > first) correct(step - 1);
     multiply(step);
+  }
+  if constexpr (kShared) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier: the last step's sums are there)
+    correct(steps - 1);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wait only)
   const bool quads = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;  // four columns of a row in one store
