@@ -30,6 +30,7 @@ struct GroupArgs {
   void *out;
   int64_t M, N, K;
   int32_t G, groups;
+  int32_t width;   // columns per tile of the kernel of few rows
   float *partial;  // K split: sums [splits][M][N rounded up to 4]
   int32_t splits;
   uint32_t group_factor;  // ceil(2^31 / (G / 32)): group of a unit of 32 columns = unit * group_factor >> 31
@@ -117,7 +118,8 @@ __device__ __forceinline__ u32x4 order_f16(u32x4 a, u32x4 b, uint32_t sel) {
                __builtin_amdgcn_perm(b[3], b[1], sel)};
 }
 
-// Up to 16 token rows (4 * RR of them in the result registers 0 .. RR - 1).  A workgroup takes tiles of 16 * FT output columns; its W
+// Up to 16 token rows (4 * RR of them in the result registers 0 .. RR - 1).  A workgroup takes tiles of p.width <= 16 * FT output columns, which
+// deals all columns evenly to the CUs (the matrix columns behind them repeat the last one's codes, which are not read from memory again); its W
 // waves take the 128-column blocks of K in turn and add their sums through LDS at a tile's end.  Codes, activations, scales and
 // zeros come to LDS by direct copies, D - 1 blocks ahead and on into the next tile, into a ring of the wave's own (no barrier
 // but at a tile's end): a matrix operand wants 16 rows side by side, of which four neighbouring lanes that loaded it to registers
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(64 * W) void group4_decode_kernel(GroupArgs p) {
   extern __shared__ float red[];  // W * kRegs * 64 sums, then the rings
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
   constexpr bool sbf = is_bf16(XT);
-  const int blocks = static_cast<int>((p.K + 127) >> 7), tiles = static_cast<int>((p.N + 16 * FT - 1) / (16 * FT));
+  const int blocks = static_cast<int>((p.K + 127) >> 7), tiles = static_cast<int>((p.N + p.width - 1) / p.width);
   uint8_t *ring = reinterpret_cast<uint8_t *>(red) + W * kRegs * 256 + wave * (D * kStage);
   const uint32_t ring_at = lds_address(ring);
 
@@ -154,8 +156,8 @@ __global__ __launch_bounds__(64 * W) void group4_decode_kernel(GroupArgs p) {
   }
   uint32_t from_w[FT], from_s[kCopiesS];
   const uint8_t *wbase, *sbase, *zbase;
-  auto aim = [&](int tile) {  // at a tile's columns (the last tile's past the end: the last column)
-    const int64_t n0 = static_cast<int64_t>(tile) * (16 * FT), left = p.N - 1 - n0;
+  auto aim = [&](int tile) {  // at a tile's columns (past its end: the last one)
+    const int64_t n0 = static_cast<int64_t>(tile) * p.width, left = (p.N - n0 < p.width ? p.N - n0 : p.width) - 1;
     wbase = p.w + n0 * (p.K / 2);
     sbase = static_cast<const uint8_t *>(p.scales) + n0 * p.groups * 2;
     zbase = static_cast<const uint8_t *>(p.zeros) + n0 * p.groups * 2;
@@ -353,14 +355,14 @@ __global__ __launch_bounds__(64 * W) void group4_decode_kernel(GroupArgs p) {
 #pragma unroll
       for (int r = 0; r < RR; ++r) red[(wave * kRegs + f * RR + r) * 64 + lane] = total[f][r];
     __syncthreads();
-    const int64_t n0 = static_cast<int64_t>(tile) * (16 * FT);
+    const int64_t n0 = static_cast<int64_t>(tile) * p.width;
     for (int e = threadIdx.x; e < kRegs * 64; e += 64 * W) {
       float v = 0.0f;
 #pragma unroll
       for (int i = 0; i < W; ++i) v += red[i * kRegs * 64 + e];
       const int l = e & 63, r = (e >> 6) % RR, f = (e >> 6) / RR;
       const int64_t n = n0 + 16 * f + (l & 15), m = (l >> 4) * RR + r;
-      if (n < p.N && m < p.M) {
+      if (16 * f + (l & 15) < p.width && n < p.N && m < p.M) {
         if constexpr (is_i8(XT)) v *= p.scale_row[m] * 0.0625f;
         if (p.bias) v += load16(p.bias, n, sbf);
         static_cast<uint16_t *>(p.out)[m * p.N + n] = sbf ? from_f32<true>(v) : from_f32<false>(v);
@@ -383,9 +385,9 @@ int launch_decode(const GroupArgs &p, hipStream_t st) {
   static_assert(smem <= kLdsBytes, "");
   auto kern = group4_decode_kernel<XT, RR, FT, W, D, SMALL, ZEROS>;
   if (int rc = prepare(kern, smem)) return rc;
-  // as many workgroups as run at a time
-  const int per_cu = kLdsBytes / smem < 32 / W ? kLdsBytes / smem : 32 / W;
-  const int64_t tiles = (p.N + 16 * FT - 1) / (16 * FT), slots = static_cast<int64_t>(num_cus()) * per_cu;
+  // as many workgroups as run at a time, two of eight waves per CU at most (1 x 8192 -> 28672 fp16, 16 columns: 27.2 us, three 29.0)
+  const int per_cu = kLdsBytes / smem < 16 / W ? kLdsBytes / smem : 16 / W;
+  const int64_t tiles = (p.N + p.width - 1) / p.width, slots = static_cast<int64_t>(num_cus()) * per_cu;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles < slots ? tiles : slots)), dim3(64 * W), smem, st, p);
   return check_launch();
 }
@@ -768,21 +770,31 @@ int launch_tile(const GroupArgs &p, hipStream_t st) {
   return check_launch();
 }
 
-// Columns per workgroup for up to 16 rows: the time goes as the tiles of the busiest CU, and a tile of 16 * FT columns costs FT and the
-// activations' share (measured, of 16 columns' codes: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16 bits).  us at 1 x
-// 8192 -> 28672, FT 1 and 2: 27.5, 29.5; 1 x 4096 -> 22016 int8: 11.0, 10.5; 16 x 8192 -> 28672, FT 1, 2 and 4: 51, 43, 38.
+// Columns per workgroup for up to 16 rows: with FT matrix tiles side by side, the rounds that all CUs need, and the columns of a round dealt
+// to them evenly.  A round's time goes half as the columns that are read, half as the matrix tiles that are computed, and as the activations'
+// share (of 16 columns: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16 bits, half of it for int8).  us with the rule's FT and
+// the next best: 1 x 4096 -> 4096 4.4 (1), 5.3 (2); 1 x 8192 -> 28672 27.5 (1), 29.3 (2); 1 x 4096 -> 22016 int8 10.2 (2), 11.0 (1); 16 x 13824 -> 5120
+// int8 10.7 (2), 14.1 (1); 16 x 8192 -> 28672 37.3 (4), 43 (2).
 template <int XT, int RR, bool SMALL, bool ZEROS>
-int by_columns(const GroupArgs &p, hipStream_t st) {
+int by_columns(GroupArgs p, hipStream_t st) {
   const double share = (RR == 1 ? 0.1 : RR == 2 ? 0.3 : 1.0) * (is_i8(XT) ? 0.5 : 1.0);
+  const int64_t cus = num_cus();
+  auto width = [&](int ft) {
+    const int64_t most = 16 * ft, rounds = ((p.N + most - 1) / most + cus - 1) / cus;
+    return static_cast<int>((p.N + rounds * cus - 1) / (rounds * cus));
+  };
   auto cost = [&](int ft) {
-    const int64_t tiles = (p.N + 16 * ft - 1) / (16 * ft), cus = num_cus();
-    return static_cast<double>((tiles + cus - 1) / cus) * (ft + share);
+    const int w = width(ft);
+    const int64_t rounds = ((p.N + w - 1) / w + cus - 1) / cus;
+    return static_cast<double>(rounds) * (0.5 * w / 16.0 + 0.5 * ft + share);
   };
   const double c1 = cost(1), c2 = cost(2), c4 = RR == 4 ? cost(4) : 1e30;
   if (c4 < c2 && c4 < c1) {
+    p.width = width(4);
     if constexpr (RR == 4) return launch_decode<XT, RR, 4, 4, 2, SMALL, ZEROS>(p, st);
   }
-  if (c2 <= c1) return launch_decode<XT, RR, 2, 8, 2, SMALL, ZEROS>(p, st);
+  p.width = width(c2 < c1 ? 2 : 1);
+  if (c2 < c1) return launch_decode<XT, RR, 2, 8, 2, SMALL, ZEROS>(p, st);
   return launch_decode<XT, RR, 1, 8, 2, SMALL, ZEROS>(p, st);
 }
 
@@ -873,7 +885,7 @@ extern "C" int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *
 
   const int64_t g = group < K ? group : (K + 31) / 32 * 32;
   const GroupArgs p{x, w, scales, zeros, x_bits == 8 ? scale_row : nullptr, bias, out, M, N, K, static_cast<int32_t>(g),
-                    static_cast<int32_t>((K + g - 1) / g), static_cast<float *>(workspace), 1, static_cast<uint32_t>(((int64_t{1} << 31) + g / 32 - 1) / (g / 32))};
+                    static_cast<int32_t>((K + g - 1) / g), 0, static_cast<float *>(workspace), 1, static_cast<uint32_t>(((int64_t{1} << 31) + g / 32 - 1) / (g / 32))};
   if (x_bits == 8) return dtype == QUIK_BF16 ? by_groups<kI8BF16>(p, workspace_bytes, as_stream(stream)) : by_groups<kI8F16>(p, workspace_bytes, as_stream(stream));
   return dtype == QUIK_BF16 ? by_groups<kBF16>(p, workspace_bytes, as_stream(stream)) : by_groups<kF16>(p, workspace_bytes, as_stream(stream));
 }
