@@ -397,7 +397,7 @@ int quik_mixed_linear_fwd(const void *qx, const void *qw, const void *meta,
  * scale 0; a row that holds a NaN or an infinity (in h, u or a factor of u), or whose squares pass fp32's range, codes 0 and a NaN scale.
  * The pitches are the distances of rows in elements (>= cols; not used with one row); q, sum and scale are contiguous.  Any cols
  * and any alignment of whole elements; 16-byte aligned rows of a multiple of 8 columns take wide accesses.
- * sum may be x or residual if its pitch is cols: every element is read before it is written. */
+ * sum may be x or residual itself where that one's rows are contiguous (pitch cols); it may not overlap them otherwise. */
 int quik_rms_norm_quantize(const void *x, int64_t x_pitch, const void *residual, int64_t residual_pitch,
                            const void *gain, float eps, int dtype, int64_t rows, int64_t cols, void *sum, int8_t *q,
                            void *scale, int scale_type, void *stream);

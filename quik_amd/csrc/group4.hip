@@ -771,13 +771,13 @@ int launch_tile(const GroupArgs &p, hipStream_t st) {
 }
 
 // Columns per workgroup for up to 16 rows: with FT matrix tiles side by side, the rounds that all CUs need, and the columns of a round dealt
-// to them evenly.  A round's time goes half as the columns that are read, half as the matrix tiles that are computed, and as the activations'
-// share (of 16 columns: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16 bits, half of it for int8).  us with the rule's FT and
-// the next best: 1 x 4096 -> 4096 4.4 (1), 5.3 (2); 1 x 8192 -> 28672 27.5 (1), 29.3 (2); 1 x 4096 -> 22016 int8 10.2 (2), 11.0 (1); 16 x 13824 -> 5120
-// int8 10.7 (2), 14.1 (1); 16 x 8192 -> 28672 37.3 (4), 43 (2).
+// to them evenly.  A round's time goes as the columns that are read, as the matrix tiles that are computed (a quarter of it; half where sums of
+// the activations come in), and as the activations' share (of 16 columns: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16
+// bits, half of it for int8).  us with the rule's FT and the next best, in turn on one card: 1 x 4096 -> 4096 5.3 (1), 6.1 (2); 1 x 8192 -> 28672 28.8
+// (2), 31.3 (1), bf16 with zeros 31.0 (1), 33.7 (2); 1 x 4096 -> 22016 int8 10.1 (2), 11.7 (1); 1 x 5120 -> 13824 10.6 (2), 12.6 (1).
 template <int XT, int RR, bool SMALL, bool ZEROS>
 int by_columns(GroupArgs p, hipStream_t st) {
-  const double share = (RR == 1 ? 0.1 : RR == 2 ? 0.3 : 1.0) * (is_i8(XT) ? 0.5 : 1.0);
+  const double share = (RR == 1 ? 0.1 : RR == 2 ? 0.3 : 1.0) * (is_i8(XT) ? 0.5 : 1.0), products = ZEROS || XT == kBF16 ? 0.5 : 0.25;
   const int64_t cus = num_cus();
   auto width = [&](int ft) {
     const int64_t most = 16 * ft, rounds = ((p.N + most - 1) / most + cus - 1) / cus;
@@ -786,7 +786,7 @@ int by_columns(GroupArgs p, hipStream_t st) {
   auto cost = [&](int ft) {
     const int w = width(ft);
     const int64_t rounds = ((p.N + w - 1) / w + cus - 1) / cus;
-    return static_cast<double>(rounds) * (0.5 * w / 16.0 + 0.5 * ft + share);
+    return static_cast<double>(rounds) * ((1.0 - products) * w / 16.0 + products * ft + share);
   };
   const double c1 = cost(1), c2 = cost(2), c4 = RR == 4 ? cost(4) : 1e30;
   if (c4 < c2 && c4 < c1) {

@@ -9,6 +9,8 @@
 // holds a NaN or an infinity, or whose squares pass the range of fp32, has codes 0 and a NaN as its scale.
 #include "common.h"
 
+#include <type_traits>
+
 namespace quik {
 namespace {
 
@@ -16,7 +18,7 @@ enum RowOp { kNorm, kNormAdd, kSiluMul };
 
 struct RowArgs {
   const uint16_t *a, *b, *gain;  // norm: x, residual, gain; silu_mul: gate, up
-  int64_t rows, cols, pitch_a, pitch_b;
+  int64_t first, rows, cols, pitch_a, pitch_b;  // first: of this launch's rows
   float eps;
   uint16_t *sum;  // norm with a residual: h [rows, cols]
   int8_t *q;
@@ -85,75 +87,98 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   return umax(umax(r0, r1), umax(r2, r3));
 }
 
-// top and square over the workgroup; `red` is free again when the next row's call comes (two barriers)
-template <int T>
+// top and square over the workgroup (up to 16 waves)
 __device__ __forceinline__ void block_reduce(uint32_t &top, float &square, uint32_t *red) {
   top = wave_max_u(top);
   square = wave_sum_f(square);
-  if constexpr (T > 64) {
-    constexpr int W = T / 64;
-    float *reds = reinterpret_cast<float *>(red + W);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-      red[threadIdx.x >> 6] = top;
-      reds[threadIdx.x >> 6] = square;
-    }
-    __syncthreads();
-    top = red[0];
-    square = reds[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-      top = umax(top, red[w]);
-      square += reds[w];
-    }
+  const int waves = static_cast<int>(blockDim.x >> 6);
+  if (waves == 1) return;
+  float *reds = reinterpret_cast<float *>(red + 16);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = top;
+    reds[threadIdx.x >> 6] = square;
+  }
+  __syncthreads();
+  top = red[0];
+  square = reds[0];
+  for (int w = 1; w < waves; ++w) {
+    top = umax(top, red[w]);
+    square += reds[w];
   }
 }
 
-// One row per workgroup, held in registers: V chunks of VEC columns per thread (VEC 8: 16-byte accesses; 1: any alignment).
-template <bool BF16, RowOp OP, int T, int VEC, int V>
-__global__ __launch_bounds__(T) void rows8_kernel(RowArgs p) {
-  __shared__ uint32_t red[2 * (T / 64)];
-  const int tid = threadIdx.x;
-  const int chunks = static_cast<int>(p.cols / VEC);
-  const int64_t row = blockIdx.x;
+// Sixteen bytes at the alignment of one element (global memory takes any), eight codes at any.
+typedef uint32_t loose4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(1)));
+
+// One row per workgroup of as many waves as it takes, held in registers: V chunks of eight columns per thread.  WIDE: rows are multiples of
+// eight columns at 16-byte addresses; else the last chunk is as many columns as there are left.
+template <bool BF16, RowOp OP, bool WIDE, int V>
+__global__ __launch_bounds__(1024) void rows8_kernel(RowArgs p) {
+  __shared__ uint32_t red[2 * 16];
+  const int tid = threadIdx.x, T = static_cast<int>(blockDim.x);
+  const int chunks = static_cast<int>((p.cols + 7) / 8), last = WIDE ? 8 : static_cast<int>(p.cols - (chunks - 1) * int64_t{8});
+  const int64_t row = p.first + blockIdx.x;
   const uint16_t *a = p.a + row * p.pitch_a;
   const uint16_t *b = OP == kNorm ? nullptr : p.b + row * p.pitch_b;
-  float u[V][VEC];
+  using Eight = std::conditional_t<WIDE, uint4, loose4>;
+  // A thread reads a column before it writes it: the sum may lie where x or the residual lies.  So no load moves up past a store by itself,
+  // and what is read of the row is requested in front of the first store where the registers allow it.  (Where there is no store the compiler
+  // does better: all of 2048 x 28672 bf16 silu_mul first takes 66.5 us, half the workgroups per CU, so 54.9.)
+  constexpr bool kFirst = OP == kNormAdd && V <= 2;
+  alignas(16) uint16_t va[V][8], vb[V][8], vg[V][8];
+  auto get = [&](int j) {
+    const int c = tid + j * T;
+    if (c >= chunks) return;
+    if (WIDE || c < chunks - 1 || last == 8) {
+      *reinterpret_cast<Eight *>(va[j]) = *reinterpret_cast<const Eight *>(a + c * int64_t{8});
+      if constexpr (OP != kNorm) *reinterpret_cast<Eight *>(vb[j]) = *reinterpret_cast<const Eight *>(b + c * int64_t{8});
+      if constexpr (OP != kSiluMul) *reinterpret_cast<Eight *>(vg[j]) = *reinterpret_cast<const Eight *>(p.gain + c * int64_t{8});
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // (zeros behind the end: they change neither maximum nor sum)
+        const int64_t at = c * int64_t{8} + e;
+        va[j][e] = e < last ? a[at] : 0;
+        if constexpr (OP != kNorm) vb[j][e] = e < last ? b[at] : 0;
+        if constexpr (OP != kSiluMul) vg[j][e] = e < last ? p.gain[at] : 0;
+      }
+    }
+  };
+  if constexpr (kFirst) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) get(j);
+  }
+  float u[V][8];
   uint32_t top = 0;
   float square = 0.0f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int c = tid + j * T;
     if (c < chunks) {
-      alignas(16) uint16_t va[VEC], vb[VEC], vg[VEC], vh[VEC];
-      if constexpr (VEC == 8) {
-        *reinterpret_cast<uint4 *>(va) = *reinterpret_cast<const uint4 *>(a + c * 8);
-        if constexpr (OP != kNorm) *reinterpret_cast<uint4 *>(vb) = *reinterpret_cast<const uint4 *>(b + c * 8);
-        if constexpr (OP != kSiluMul) *reinterpret_cast<uint4 *>(vg) = *reinterpret_cast<const uint4 *>(p.gain + c * 8);
-      } else {
-        va[0] = a[c];
-        if constexpr (OP != kNorm) vb[0] = b[c];
-        if constexpr (OP != kSiluMul) vg[0] = p.gain[c];
-      }
+      if constexpr (!kFirst) get(j);
+      alignas(16) uint16_t vh[8];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        u[j][e] = row_value<BF16, OP>(to_f32<BF16>(va[e]), OP == kNorm ? 0.0f : to_f32<BF16>(vb[e]), OP == kSiluMul ? 0.0f : to_f32<BF16>(vg[e]),
+      for (int e = 0; e < 8; ++e) {
+        u[j][e] = row_value<BF16, OP>(to_f32<BF16>(va[j][e]), OP == kNorm ? 0.0f : to_f32<BF16>(vb[j][e]), OP == kSiluMul ? 0.0f : to_f32<BF16>(vg[j][e]),
                                       vh[e], square);
         top = umax(top, __float_as_uint(u[j][e]) & 0x7FFFFFFFu);
       }
       if constexpr (OP == kNormAdd) {
-        uint16_t *s = p.sum + row * p.cols + static_cast<int64_t>(c) * VEC;
-        if constexpr (VEC == 8)
-          *reinterpret_cast<uint4 *>(s) = *reinterpret_cast<const uint4 *>(vh);
-        else
-          s[0] = vh[0];
+        uint16_t *s = p.sum + row * p.cols + c * int64_t{8};
+        if (WIDE || c < chunks - 1 || last == 8) {
+          *reinterpret_cast<Eight *>(s) = *reinterpret_cast<const Eight *>(vh);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < last) s[e] = vh[e];
+        }
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) u[j][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) u[j][e] = 0.0f;
     }
   }
-  block_reduce<T>(top, square, red);
+  block_reduce(top, square, red);
   float pre, inv, scale;
   row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
   if (tid == 0) store_scale(p, row, scale);
@@ -161,79 +186,98 @@ __global__ __launch_bounds__(T) void rows8_kernel(RowArgs p) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) u[j][e] *= pre;
+      for (int e = 0; e < 8; ++e) u[j][e] *= pre;
   }
   if (inv == 0.0f) {  // (NaNs and infinities among the values: codes 0)
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) u[j][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) u[j][e] = 0.0f;
   }
   int8_t *q = p.q + row * p.cols;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int c = tid + j * T;
     if (c < chunks) {
-      if constexpr (VEC == 8) {
-        uint32_t w[2];
+      uint32_t w[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float *v = &u[j][4 * k];
-          const uint32_t lo = __builtin_amdgcn_perm(code_bits(v[1], inv), code_bits(v[0], inv), 0x0C0C0400u);
-          const uint32_t hi = __builtin_amdgcn_perm(code_bits(v[3], inv), code_bits(v[2], inv), 0x04000C0Cu);
-          w[k] = lo | hi;
-        }
-        *reinterpret_cast<uint2 *>(q + c * 8) = make_uint2(w[0], w[1]);
+      for (int k = 0; k < 2; ++k) {
+        const float *v = &u[j][4 * k];
+        const uint32_t lo = __builtin_amdgcn_perm(code_bits(v[1], inv), code_bits(v[0], inv), 0x0C0C0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(code_bits(v[3], inv), code_bits(v[2], inv), 0x04000C0Cu);
+        w[k] = lo | hi;
+      }
+      int8_t *to = q + c * int64_t{8};
+      if (WIDE) {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+      } else if (c < chunks - 1 || last == 8) {
+        *reinterpret_cast<loose2 *>(to) = loose2{w[0], w[1]};
       } else {
-        q[c] = static_cast<int8_t>(code_bits(u[j][0], inv) & 0xFFu);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < last) to[e] = static_cast<int8_t>(w[e >> 2] >> (8 * (e & 3)));
       }
     }
   }
 }
 
-// Rows that no instance of the kernel above holds in registers: the row is read twice, the second time from the caches.
+// Rows that no instance of the kernel above holds in registers: the row is read twice, the second time from the caches (with a residual, its
+// sum: it may lie where x or the residual lies).
 template <bool BF16, RowOp OP>
 __global__ __launch_bounds__(1024) void rows8_long_kernel(RowArgs p) {
   __shared__ uint32_t red[2 * 16];
-  const int64_t row = blockIdx.x;
+  const int64_t row = p.first + blockIdx.x;
   const uint16_t *a = p.a + row * p.pitch_a;
   const uint16_t *b = OP == kNorm ? nullptr : p.b + row * p.pitch_b;
+  uint16_t *sum = OP == kNormAdd ? p.sum + row * p.cols : nullptr;
   uint32_t top = 0;
-  float square = 0.0f, unused = 0.0f;
-  uint16_t h = 0;
-  auto value = [&](int64_t c, float &sq) {
-    return row_value<BF16, OP>(to_f32<BF16>(a[c]), OP == kNorm ? 0.0f : to_f32<BF16>(b[c]), OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, sq);
-  };
+  float square = 0.0f;
   for (int64_t c = threadIdx.x; c < p.cols; c += 1024) {
-    top = umax(top, __float_as_uint(value(c, square)) & 0x7FFFFFFFu);
-    if constexpr (OP == kNormAdd) p.sum[row * p.cols + c] = h;
+    uint16_t h = 0;
+    const float u = row_value<BF16, OP>(to_f32<BF16>(a[c]), OP == kNorm ? 0.0f : to_f32<BF16>(b[c]), OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, square);
+    top = umax(top, __float_as_uint(u) & 0x7FFFFFFFu);
+    if constexpr (OP == kNormAdd) sum[c] = h;
   }
-  block_reduce<1024>(top, square, red);
+  block_reduce(top, square, red);
   float pre, inv, scale;
   row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
   if (threadIdx.x == 0) store_scale(p, row, scale);
-  for (int64_t c = threadIdx.x; c < p.cols; c += 1024)
-    p.q[row * p.cols + c] = inv == 0.0f ? int8_t{0} : static_cast<int8_t>(code_bits(value(c, unused) * pre, inv) & 0xFFu);
+  for (int64_t c = threadIdx.x; c < p.cols; c += 1024) {  // (a thread's own columns: what it has written of the sum)
+    uint16_t h = 0;
+    float unused = 0.0f;
+    constexpr RowOp kAgain = OP == kNormAdd ? kNorm : OP;
+    const float u = row_value<BF16, kAgain>(to_f32<BF16>(OP == kNormAdd ? sum[c] : a[c]), OP == kSiluMul ? to_f32<BF16>(b[c]) : 0.0f,
+                                            OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, unused);
+    p.q[row * p.cols + c] = inv == 0.0f ? int8_t{0} : static_cast<int8_t>(code_bits(u * pre, inv) & 0xFFu);
+  }
 }
 
 template <bool BF16, RowOp OP>
-int launch(const RowArgs &p, bool wide, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.rows));
-  const int64_t chunks = p.cols / 8;
-#define QUIK_ROWS(T, VEC, V) hipLaunchKernelGGL((rows8_kernel<BF16, OP, T, VEC, V>), grid, dim3(T), 0, st, p)
-  if (wide && chunks <= 64) QUIK_ROWS(64, 8, 1);
-  else if (wide && chunks <= 128) QUIK_ROWS(128, 8, 1);
-  else if (wide && chunks <= 256) QUIK_ROWS(256, 8, 1);
-  else if (wide && chunks <= 512) QUIK_ROWS(512, 8, 1);
-  else if (wide && chunks <= 1024) QUIK_ROWS(1024, 8, 1);
-  else if (wide && chunks <= 2048) QUIK_ROWS(1024, 8, 2);
-  else if (wide && chunks <= 4096) QUIK_ROWS(1024, 8, 4);
-  else if (p.cols <= 256) QUIK_ROWS(64, 1, 4);
-  else if (p.cols <= 4096) QUIK_ROWS(256, 1, 16);
-  else if (p.cols <= 32768) QUIK_ROWS(1024, 1, 32);
-  else hipLaunchKernelGGL((rows8_long_kernel<BF16, OP>), grid, dim3(1024), 0, st, p);
+int launch_rows(const RowArgs &p, int64_t rows, bool wide, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(rows));
+  // Chunks per thread: one where a row's time is a chain of latencies, more where many rows' memory is what takes the time.  us with one, two
+  // and four: 1 x 4096 fp16 with a residual 3.2, 3.4, 3.75; 777 x 5120 fp16 5.9, 5.1, 5.3; 4096 x 8192 bf16 with a residual 43.8, 40.1, 38.6.
+  const int64_t chunks = (p.cols + 7) / 8, cus = num_cus();
+  const int v = rows > 8 * cus || chunks > 2048 ? 4 : rows > cus || chunks > 1024 ? 2 : 1;
+#define QUIK_ROWS(WIDE, V) hipLaunchKernelGGL((rows8_kernel<BF16, OP, WIDE, V>), grid, dim3(static_cast<unsigned>((chunks + 64 * V - 1) / (64 * V) * 64)), 0, st, p)
+  if (chunks > 4096) hipLaunchKernelGGL((rows8_long_kernel<BF16, OP>), grid, dim3(1024), 0, st, p);
+  else if (wide && v == 1) QUIK_ROWS(true, 1);
+  else if (wide && v == 2) QUIK_ROWS(true, 2);
+  else if (wide) QUIK_ROWS(true, 4);
+  else if (v == 1) QUIK_ROWS(false, 1);
+  else if (v == 2) QUIK_ROWS(false, 2);
+  else QUIK_ROWS(false, 4);
 #undef QUIK_ROWS
   return check_launch();
+}
+
+// 2^20 rows per launch (a grid has less than 2^32 threads).  A loop over rows in the kernel costs registers: 2048 x 28672 bf16 silu_mul 55
+// -> 61.5 us.
+template <bool BF16, RowOp OP>
+int launch(RowArgs p, bool wide, hipStream_t st) {
+  for (; p.first < p.rows; p.first += 1 << 20)
+    if (int rc = launch_rows<BF16, OP>(p, p.rows - p.first < 1 << 20 ? p.rows - p.first : 1 << 20, wide, st)) return rc;
+  return QUIK_OK;
 }
 
 template <RowOp OP>
@@ -263,7 +307,7 @@ extern "C" int quik_rms_norm_quantize(const void *x, int64_t x_pitch, const void
   if (rows == 0) return QUIK_OK;
   if (!x || !gain || !q || !scale || (residual && !sum)) return QUIK_ERR_NULL;
   if (!aligned(x, 2) || !aligned(residual, 2) || !aligned(gain, 2) || !aligned(sum, 2) || !aligned(scale, scale_type == QUIK_F32 ? 4 : 2)) return QUIK_ERR_ALIGN;
-  const RowArgs p{static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(residual), static_cast<const uint16_t *>(gain), rows, cols,
+  const RowArgs p{static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(residual), static_cast<const uint16_t *>(gain), 0, rows, cols,
                   x_pitch, residual_pitch, eps, static_cast<uint16_t *>(sum), q, scale, scale_type};
   const bool wide = cols % 8 == 0 && aligned(x, 16) && aligned(gain, 16) && aligned(q, 8) && (rows == 1 || x_pitch % 8 == 0) &&
                     (!residual || (aligned(residual, 16) && aligned(sum, 16) && (rows == 1 || residual_pitch % 8 == 0)));
@@ -276,7 +320,7 @@ extern "C" int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, cons
   if (rows == 0) return QUIK_OK;
   if (!gate || !up || !q || !scale) return QUIK_ERR_NULL;
   if (!aligned(gate, 2) || !aligned(up, 2) || !aligned(scale, scale_type == QUIK_F32 ? 4 : 2)) return QUIK_ERR_ALIGN;
-  const RowArgs p{static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up), nullptr, rows, cols, gate_pitch, up_pitch, 0.0f,
+  const RowArgs p{static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up), nullptr, 0, rows, cols, gate_pitch, up_pitch, 0.0f,
                   nullptr, q, scale, scale_type};
   const bool wide = cols % 8 == 0 && aligned(gate, 16) && aligned(up, 16) && aligned(q, 8) &&
                     (rows == 1 || (gate_pitch % 8 == 0 && up_pitch % 8 == 0));

@@ -30,8 +30,8 @@ from ._lib import device_guard
 
 _front = None     # the native front end; set when the first plan is made (only plans lead into it)
 
-__all__ = ["MixedQLinear", "SharedQuantizedInput", "FusedMixedQLinearGroup", "Linear4bit", "Linear8bit", "pack_to_i4",
-           "two_compl"]
+__all__ = ["MixedQLinear", "SharedQuantizedInput", "FusedMixedQLinearGroup", "Linear4bit", "Linear8bit", "GroupLinear4bit",
+           "pack_to_i4", "two_compl"]
 
 
 def two_compl(x: Tensor, bits: int) -> Tensor:
@@ -811,3 +811,52 @@ class Linear4bit(torch.nn.Module):
         x_int4 = x[:, :x.size(1) // 2].to(torch.uint8).contiguous()
         out = matmul.int4Matmul(x_int4, self.int_weight).to(torch.float16)
         return out if self.bias is None else out.add(self.bias)
+
+
+class GroupLinear4bit(torch.nn.Module):
+    """4-bit weights with one scale (and zero) per `group_size` input columns of a row, for 16-bit activations or 8-bit rows.
+
+    int_weight [out, in/2] holds signed codes as Linear4bit's, scales [out, ceil(in / group_size)]; with `zeros` a code stands for
+    (code - zero) * scale.  forward(x) takes x of the scales' type; forward(q, scale) int8 rows and their scales as
+    symmetric.rms_norm_quantize and silu_mul_quantize give them.  No counterpart in the reference."""
+
+    def __init__(self, in_features, out_features, group_size=128, zeros=False, bias=False, dtype=torch.float16):
+        super().__init__()
+        if in_features % 32 or group_size % 32 or in_features <= 0 or group_size <= 0:
+            raise ValueError(f"GroupLinear4bit: in_features and group_size must be multiples of 32, got {in_features} and {group_size}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group_size = group_size
+        groups = (in_features + group_size - 1) // group_size
+        self.register_buffer('int_weight', torch.zeros((out_features, in_features // 2), dtype=torch.uint8))
+        self.register_buffer('scales', torch.ones((out_features, groups), dtype=dtype))
+        self.register_buffer('zeros', torch.zeros((out_features, groups), dtype=dtype) if zeros else None)
+        self.register_buffer('bias', torch.zeros((out_features,), dtype=dtype) if bias else None)
+
+    @staticmethod
+    @torch.no_grad()
+    def from_float(module, group_size=128, symm=True):
+        """Round-to-nearest codes of a torch.nn.Linear, group by group: symmetric (largest magnitude at 7), or over [min, max] with a whole
+        zero.  The scales have the weight's type (16 bits: fp16 where the module is fp32)."""
+        w = module.weight
+        dtype = w.dtype if w.dtype in (torch.float16, torch.bfloat16) else torch.float16
+        mod = GroupLinear4bit(module.in_features, module.out_features, group_size, not symm, module.bias is not None, dtype).to(w.device)
+        for g in range(mod.scales.shape[1]):
+            part = w[:, g * group_size:(g + 1) * group_size].float()
+            lo, hi = part.amin(1, keepdim=True).clamp(max=0), part.amax(1, keepdim=True).clamp(min=0)
+            scale = (torch.maximum(-lo, hi) / 7 if symm else (hi - lo) / 15).to(dtype).float()
+            scale = torch.where(scale > 0, scale, torch.ones_like(scale))
+            zero = torch.zeros_like(scale) if symm else (-8 - lo / scale).round()
+            codes = (part / scale + zero).round().clamp(-8, 7).to(torch.int8)
+            mod.int_weight[:, g * group_size // 2:g * group_size // 2 + part.shape[1] // 2] = pack_to_i4(codes)
+            mod.scales[:, g:g + 1] = scale
+            if not symm:
+                mod.zeros[:, g:g + 1] = zero
+        if module.bias is not None:
+            mod.bias.copy_(module.bias)
+        return mod
+
+    def forward(self, x, scale=None):
+        out = matmul.int4GroupMatmul(x.reshape(-1, x.shape[-1]), self.int_weight, self.scales, self.group_size, zeros=self.zeros,
+                                     scale_row=scale, bias=self.bias)
+        return out.reshape(*x.shape[:-1], self.out_features)

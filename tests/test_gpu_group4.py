@@ -168,3 +168,40 @@ def test_empty():
     args = make(1, 40, 128, 128, torch.float16, torch.float16)
     assert call((args[0][:0],) + args[1:], 128).shape == (0, 40)
     assert call((args[0], args[1][:0], args[2][:0], None, None, None), 128).shape == (1, 0)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_offsets_past_32_bits(codes):
+    """Activations, results and weights of more than 2^31 elements and bytes."""
+    x, w, s, z, sr, b = make(8, 48, 16384, 128, torch.int8 if codes else torch.float16, torch.float16)
+    rows = (1 << 17) + 8
+    many = torch.zeros(rows, 16384, dtype=x.dtype, device=DEV)
+    many[-8:] = x
+    scale = None if sr is None else torch.ones(rows, 1, device=DEV)
+    if scale is not None:
+        scale[-8:] = sr
+    out = call((many, w, s, z, scale, b), 128)
+    check(out[-8:], (x, w, s, z, sr, b), 128)
+    assert not out[:-8].any()
+    del many, out
+    cols = (1 << 18) + 48
+    wide = torch.full((cols, 8192), 0x88, dtype=torch.uint8, device=DEV)
+    wide[-48:] = w
+    scales = torch.zeros(cols, 128, dtype=torch.float16, device=DEV)
+    scales[-48:] = s
+    for rows in (8, 24):
+        xx = x.repeat(3, 1)[:rows]
+        ss = None if sr is None else sr.repeat(3, 1)[:rows]
+        out = call((xx, wide, scales, None, ss, None), 128)
+        check(out[:, -48:], (xx, w, s, None, ss, None), 128)
+        assert not out[:, :-48].any()
+
+
+def test_one_group_of_all_columns_and_long_rows():
+    """The longest rows there are."""
+    K = 1 << 20
+    for M in (1, 20):
+        for G in (K, 64):
+            args = make(M, 18, K, G, torch.int8, torch.float16, True)
+            args[2].mul_(2.0 ** -9)
+            check(call(args, G), args, G)

@@ -38,12 +38,12 @@ def _norm_oracle(x, weight, eps, residual):
         u = _f32(h) * _f32(weight)
         top = np.abs(u).max(1, keepdims=True)
         inv = np.where(top > 0, np.float32(127) / top, np.float32(0)).astype(np.float32)
-        q = np.rint(u * inv)
+        q = np.nan_to_num(np.rint(u * inv))
         scale = top.astype(np.float64) / 127 / np.sqrt((_up(h) ** 2).mean(1, keepdims=True) + np.float64(np.float32(eps)))
     bad = ~np.isfinite(u).all(1) | ~np.isfinite(_f32(h)).all(1)
     q[bad] = 0
     scale[bad] = np.nan
-    return q.astype(np.int8), scale, h
+    return np.clip(q, -127, 127).astype(np.int8), scale, h
 
 
 def _check_scale(got, want, tol):
@@ -168,6 +168,42 @@ def test_scales_of_16_bits(dtype, scale_dtype):
     q, s = quik.symmetric.silu_mul_quantize(x, x)
     q16, s16 = quik.symmetric.silu_mul_quantize(x, x, scale_dtype=scale_dtype)
     assert torch.equal(q, q16) and torch.equal(s.to(scale_dtype), s16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [64, 1001, 4096, 16384, 30000, 40000])
+def test_sum_in_the_place_of_an_input(cols, dtype):
+    from quik_amd import _lib as L
+    rows, x, r, w = 5, _input(5, cols, dtype, 19), _input(5, cols, dtype, 20), _input(1, cols, dtype, 21)[0]
+    wq, ws, wh = quik.symmetric.rms_norm_quantize(x, w, residual=r)
+    for place in (0, 1):
+        both = [x.clone(), r.clone()]
+        q, scale = torch.empty_like(wq), torch.empty_like(ws)
+        L.check(L.load().quik_rms_norm_quantize(L.ptr(both[0]), cols, L.ptr(both[1]), cols, L.ptr(w), 1e-6, L.dtype_id(x, "", True), rows, cols,
+                                                L.ptr(both[place]), L.ptr(q), L.ptr(scale), L.QUIK_F32, L.stream()), "")
+        assert torch.equal(both[place], wh) and torch.equal(q, wq) and torch.equal(scale, ws)
+        assert torch.equal(both[1 - place], (r, x)[place])
+
+
+def test_more_rows_than_workgroups_and_offsets_past_32_bits():
+    w = _input(1, 8, torch.float16, 22)[0]
+    x = torch.ones((1 << 20) + 3, 8, dtype=torch.float16, device=DEV)
+    x[-1] = _input(1, 8, torch.float16, 23)[0]
+    q, scale, _ = quik.symmetric.rms_norm_quantize(x, w)
+    for i in (0, 1 << 20, -1):
+        one = quik.symmetric.rms_norm_quantize(x[i:][:1], w)
+        assert torch.equal(q[i], one[0][0]) and torch.equal(scale[i], one[1][0])
+    cols, rows = 32768, (1 << 16) + 2                 # 2^31 and some elements
+    g = torch.zeros(rows, cols, dtype=torch.bfloat16, device=DEV)
+    g[-2:] = _input(2, cols, torch.bfloat16, 24)
+    w = _input(1, cols, torch.bfloat16, 25)[0]
+    q, scale, h = quik.symmetric.rms_norm_quantize(g, w, residual=g)
+    a, b, c = quik.symmetric.rms_norm_quantize(g[-2:], w, residual=g[-2:])
+    assert torch.equal(q[-2:], a) and torch.equal(scale[-2:], b) and torch.equal(h[-2:], c) and not scale[:-2].any()
+    del h
+    q, scale = quik.symmetric.silu_mul_quantize(g, g)
+    a, b = quik.symmetric.silu_mul_quantize(g[-2:], g[-2:])
+    assert torch.equal(q[-2:], a) and torch.equal(scale[-2:], b) and not scale[:-2].any()
 
 
 def test_empty_batch():
