@@ -445,13 +445,20 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   const uint8_t *sbase = static_cast<const uint8_t *>(p.scales) + n0 * p.groups * 2, *zbase = static_cast<const uint8_t *>(p.zeros) + n0 * p.groups * 2;
   const int64_t left_m = p.M - 1 - m0, left_n = p.N - 1 - n0;
   const int last_w = static_cast<int>(p.K / 32) - 1, last_x = static_cast<int>(p.K * kSize / 16) - 1;
+  // Where a row's 16-byte pieces lie in LDS: at the row's number exclusive-or the piece's; in wide tiles with the piece's two fields (lane row,
+  // matrix step) changed over where a lane reads neighbouring pieces in its steps.  A 16-byte read goes by lanes 0 .. 3, 12 .. 15, 20 .. 27 and
+  // so on, which are at different banks then (else half as many cycles again per read: 2048 x 4096 -> 11008 int8 151 us, so 140, bf16
+  // 236, 229).  Copies in that order cost more than the banks in small tiles (64 x 8192 -> 8192 fp16 35.1 us, 36.5).
+  constexpr bool kSwap = !kTurn && RM >= 8;
+  auto place_of = [](int piece) { return !kSwap ? piece : is_i8(XT) ? (piece & 1) * 4 + (piece >> 1) : (piece & 3) * 4 + (piece >> 2); };
+  auto piece_at = [](int place) { return !kSwap ? place : is_i8(XT) ? (place & 3) * 2 + (place >> 2) : (place & 3) * 4 + (place >> 2); };
   // this wave's copies: which of the step's, the row's offset and the piece of the step that this lane takes
   uint32_t x_row[S::kMyX], w_row[S::kMyW], s_row[S::kMyS];
   int x_piece[S::kMyX], w_piece[S::kMyW], s_unit[S::kMyS];
 #pragma unroll
   for (int i = 0; i < S::kMyX; ++i) {
     const int c = (wave + i * S::kW) % S::kX, part = c / (S::kX / WK), row = (c % (S::kX / WK)) * (64 / kRowPieces) + lane / kRowPieces;
-    x_piece[i] = part * kRowPieces + ((lane % kRowPieces) ^ (row % kRowPieces));
+    x_piece[i] = part * kRowPieces + piece_at((lane % kRowPieces) ^ (row % kRowPieces));
     x_row[i] = static_cast<uint32_t>((row < left_m ? row : left_m) * p.K * kSize);
   }
 #pragma unroll
@@ -507,7 +514,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   auto x_row_at = [&](const uint8_t *from, int t) { return from + (wk * S::kBM + wm * 16 * RM + 16 * t + col) * S::kRowBytes; };
   auto x_piece_of = [&](const uint8_t *from, int t, int s) {
     const int piece = is_i8(XT) ? 2 * kg + s : kTurn ? 4 * s + kg : 4 * kg + s;
-    return *reinterpret_cast<const u32x4 *>(x_row_at(from, t) + ((piece ^ (col % kRowPieces)) * 16));
+    return *reinterpret_cast<const u32x4 *>(x_row_at(from, t) + ((place_of(piece) ^ (col % kRowPieces)) * 16));
   };
   auto x_half = [&](const uint8_t *from, int t, int s) {
     return *reinterpret_cast<const u32x2 *>(x_row_at(from, t) + (((2 * s + kg / 2) ^ (col % kRowPieces)) * 16 + (kg & 1) * 8));
