@@ -478,30 +478,39 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   auto group_of = [&](int unit) { return static_cast<uint32_t>((static_cast<uint64_t>(static_cast<uint32_t>(unit)) * p.group_factor) >> 31); };
   auto copy = [&](int step) {
     const uint32_t to = lds_at + step % D * S::kStage;
-    const bool whole = (static_cast<int64_t>(step) + 1) * (128 * WK) <= p.K;
     const int xp0 = step * (WK * kRowPieces), wp0 = step * (WK * 4);
+    if ((static_cast<int64_t>(step) + 1) * (128 * WK) <= p.K) {  // (what goes on along K in scalar registers)
+      const uint8_t *xfrom = xbase + xp0 * 16, *wfrom = wbase + wp0 * 16;
 #pragma unroll
-    for (int i = 0; i < S::kMyX; ++i) {  // (pieces past the end of a row come from its last one)
-      const int c = (wave + i * S::kW) % S::kX;
-      int piece = xp0 + x_piece[i];
-      if (!whole) piece = piece < last_x ? piece : last_x;
-      dma_load16(xbase, x_row[i] + static_cast<uint32_t>(piece) * 16, to + c * 1024);
-    }
+      for (int i = 0; i < S::kMyX; ++i) dma_load16(xfrom, x_row[i] + x_piece[i] * 16, to + (wave + i * S::kW) % S::kX * 1024);
 #pragma unroll
-    for (int i = 0; i < S::kMyW; ++i) {
-      const int c = (wave + i * S::kW) % S::kWt;
-      int piece = wp0 + w_piece[i];
-      if (!whole) piece = piece < last_w ? piece : last_w;
-      dma_load16(wbase, w_row[i] + static_cast<uint32_t>(piece) * 16, to + S::kAtW + c * 1024);
+      for (int i = 0; i < S::kMyW; ++i) dma_load16(wfrom, w_row[i] + w_piece[i] * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
+    } else {  // pieces past the end of a row come from its last one
+#pragma unroll
+      for (int i = 0; i < S::kMyX; ++i) {
+        const int piece = xp0 + x_piece[i];
+        dma_load16(xbase, x_row[i] + static_cast<uint32_t>(piece < last_x ? piece : last_x) * 16, to + (wave + i * S::kW) % S::kX * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < S::kMyW; ++i) {
+        const int piece = wp0 + w_piece[i];
+        dma_load16(wbase, w_row[i] + static_cast<uint32_t>(piece < last_w ? piece : last_w) * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
+      }
     }
 #pragma unroll
     for (int i = 0; i < S::kMyS; ++i) {
       const int c = (wave + i * S::kW) % S::kS;
-      int unit = wp0 + s_unit[i];
-      unit = unit < last_w ? unit : last_w;
-      const uint32_t at = s_row[i] + 2 * group_of(unit);
-      dma_load_u16(sbase, at, to + S::kAtS + c * 256);
-      if constexpr (ZEROS) dma_load_u16(zbase, at, to + S::kAtZ + c * 256);
+      if constexpr (kTurn) {
+        const int unit = wp0 + s_unit[i];
+        const uint32_t at = s_row[i] + 2 * group_of(unit < last_w ? unit : last_w);
+        dma_load_u16(sbase, at, to + S::kAtS + c * 256);
+        if constexpr (ZEROS) dma_load_u16(zbase, at, to + S::kAtZ + c * 256);
+      } else {
+        const int unit = wp0 + c / (S::kS / WK) * 4;
+        const uint32_t g = 2 * group_of(unit < last_w ? unit : last_w);
+        dma_load_u16(sbase + g, s_row[i], to + S::kAtS + c * 256);
+        if constexpr (ZEROS) dma_load_u16(zbase + g, s_row[i], to + S::kAtZ + c * 256);
+      }
     }
   };
   f32x4 total[RM][RN];
@@ -811,14 +820,14 @@ struct TilePlan {
   int rows, cols, depth;
   double step[3], round;  // round: what first copies and stores of a workgroup take, where one runs per CU
 };
-constexpr TilePlan kPlans[3] = {{32, 128, 256, {0.94, 1.37, 0.72}, 0}, {64, 128, 256, {1.35, 1.9, 0.9}, 0}, {128, 256, 128, {1.95, 2.4, 1.3}, 6}};
+constexpr TilePlan kPlans[3] = {{32, 128, 256, {0.94, 1.37, 0.72}, 0}, {64, 128, 256, {1.35, 1.9, 0.9}, 0}, {128, 256, 128, {1.9, 2.1, 1.2}, 6}};
 
 struct Choice {
   int plan, splits;
 };
 // The cheapest tiles and K split: rounds of the busiest CU, 4 us around them, and for a split the second launch (3 us) and its sums, written
 // and read.  us, as the rule has it and measured: 64 x 13824 -> 5120 int8, 64 rows, K in 6: 18.2, 19.7 (not split: 53); 64 x 8192 -> 8192
-// fp16, K in 4: 21.2, 21.7 (47); 128 x 13824 -> 5120 int8, K in 3: 26.3, 26.9 (53); 2048 x 4096 -> 11008 int8, 128 rows: 147, 149 (64
+// fp16, K in 4: 21.2, 21.7 (47); 128 x 13824 -> 5120 int8, K in 3: 26.3, 26.9 (53); 2048 x 4096 -> 11008 int8, 128 rows: 137, 137 (64
 // rows: 153).
 Choice choose(int64_t M, int64_t N, int64_t K, int acts, bool may_split) {
   Choice best{1, 1};
