@@ -413,7 +413,7 @@ int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up,
  *   bias    [N] dtype or NULL; out [M, N] dtype
  * K % 32 == 0, K <= 2^20, group % 32 == 0 (a group >= K: one scale per output column; the last group may be shorter); x and w 16-byte
  * aligned.  A group's product is summed in fp32 (int8: exactly) and scaled in fp32; one rounding to dtype.  A row of x that
- * holds an infinity gives infinities or NaNs. */
+ * holds an infinity, or a bf16 value of 2^110 or more, gives infinities or NaNs where the sums pass fp32's range. */
 int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const void *scales, const void *zeros,
                            const float *scale_row, const void *bias, int dtype, int64_t M, int64_t N, int64_t K,
                            int64_t group, void *out, void *workspace, int64_t workspace_bytes, void *stream);

@@ -417,6 +417,9 @@ struct TileShape {
   // 11008, each wave all of them and this: bf16 267, 256, fp16 with zeros 292, 258); of fewer each wave makes all that it needs (64 x 4096
   // -> 11008 bf16 with zeros, so and shared: 22.7, 26.3).
   static constexpr bool kShared = kSums && RM >= 8, kOwnSums = kSums && !kShared;
+  // Groups of 32 and the like: what the sums are multiplied by is a matrix product of its own, of 16 columns and 16 rows over the block's four
+  // units of 32 columns, in fp32 (300 x 4544 -> 4541 int8, groups of 32 with zeros: 65 us, so 56; groups of 64 lose 1 - 7 %).
+  static constexpr bool kUnits = kOwnSums && PARTS == 4;
   static constexpr int kAtSums = D * kStage, kRings = kAtSums + (kShared ? 2 * WK * PARTS * kBM * 4 : 0);  // of two steps
   static constexpr int kLds = kRings > kReduce ? kRings : kReduce;
   static_assert(!kShared || WN >= RM, "");
@@ -425,7 +428,7 @@ struct TileShape {
 template <int XT, int RM, int RN, int WM, int WN, int WK, int D, int PARTS, bool ZEROS>
 __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArgs p) {
   using S = TileShape<XT, RM, RN, WM, WN, WK, D, PARTS, ZEROS>;
-  constexpr bool kShared = S::kShared, kOwnSums = S::kOwnSums;
+  constexpr bool kShared = S::kShared, kOwnSums = S::kOwnSums, kUnits = S::kUnits;
   constexpr bool kTurn = PARTS > 1;  // matrix step s: columns 32 s .. of the block; else columns 8 s .. of each lane row's 32
   constexpr int kRowPieces = S::kRowBytes / 16, kSize = is_i8(XT) ? 1 : 2;
   extern __shared__ float red[];
@@ -551,6 +554,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   };
   // Sums of the activations of a part (columns of one group), by a matrix of ones: what the zeros and the offset of widened bf16 codes are
   // multiplied by.
+  constexpr float kOffset = XT == kBF16 ? 136.0f : 0.0f, kUnit = is_i8(XT) ? 16.0f : 1.0f;
   float *const sums = reinterpret_cast<float *>(lds + S::kAtSums);
   float less[kShared ? PARTS : 1][RN][4];  // -scale * (offset + zero) of the step before
   auto sums_of = [&](int step, int part) { return sums + (((step & 1) * WK + wk) * PARTS + part) * S::kBM + wm * 16 * RM + col; };
@@ -597,15 +601,20 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
       w[f] = *reinterpret_cast<const u32x4 *>(from + S::kAtW + (wk * (S::kBN / 16) + wn * RN + f) * 1024 + w_slot);
       if constexpr (kTurn) transpose4(w[f]);
     }
+    Acc<XT> units[kUnits ? RM : 1];  // (kUnits: first value, of the lane row's 32 columns)
+    if constexpr (kUnits) {
+#pragma unroll
+      for (int t = 0; t < RM; ++t) units[t] = Acc<XT>{0, 0, 0, 0};
+    }
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
         if (kTurn && k0 + 128 / PARTS * part >= p.K) break;
         if constexpr (kShared) sum(from, step, part, k0);
-        Acc<XT> acc[RM][RN], own[kOwnSums ? RM : 1];
+        Acc<XT> acc[RM][RN], own[kOwnSums && !kUnits ? RM : 1];
         __builtin_amdgcn_s_setprio(1);  // a wave among its products before one that widens codes for its next
 #pragma unroll
         for (int t = 0; t < RM; ++t) {
-          if constexpr (kOwnSums) own[t] = Acc<XT>{0, 0, 0, 0};
+          if constexpr (kOwnSums && !kUnits) own[t] = Acc<XT>{0, 0, 0, 0};
 #pragma unroll
           for (int f = 0; f < RN; ++f) acc[t][f] = Acc<XT>{0, 0, 0, 0};
         }
@@ -617,7 +626,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = __builtin_bit_cast(long, x_half(from, t, s));
-              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
+              if constexpr (kUnits) {
+                const Acc<XT> v = add_ones(xa[t], Acc<XT>{0, 0, 0, 0});
+                units[t][0] = kg == s ? v[0] : units[t][0];
+              } else if constexpr (kOwnSums) {
+                own[t] = add_ones(xa[t], own[t]);
+              }
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -633,7 +647,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = __builtin_bit_cast(i32x4, x_piece_of(from, t, s));
-              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
+              if constexpr (kUnits) {
+                const Acc<XT> v = add_ones(xa[t], Acc<XT>{0, 0, 0, 0});
+                units[t][0] = kg == s ? v[0] : units[t][0];
+              } else if constexpr (kOwnSums) {
+                own[t] = add_ones(xa[t], own[t]);
+              }
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -651,7 +670,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = x_piece_of(from, t, s);
-              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
+              if constexpr (kUnits) {
+                const Acc<XT> v = add_ones(xa[t], Acc<XT>{0, 0, 0, 0});
+                units[t][0] = kg == s ? v[0] : units[t][0];
+              } else if constexpr (kOwnSums) {
+                own[t] = add_ones(xa[t], own[t]);
+              }
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
@@ -670,9 +694,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
           float s[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[r] = from16(sw[r], sbf);
-          constexpr float kOffset = XT == kBF16 ? 136.0f : 0.0f, kUnit = is_i8(XT) ? 16.0f : 1.0f;
           float z[4] = {kOffset, kOffset, kOffset, kOffset};
-          if constexpr (ZEROS) {
+          if constexpr (ZEROS && !kUnits) {
             const u32x4 zw = *reinterpret_cast<const u32x4 *>(from_s + (S::kAtZ - S::kAtS) + 4 * at);
 #pragma unroll
             for (int r = 0; r < 4; ++r) z[r] += kUnit * from16(zw[r], sbf);
@@ -686,11 +709,22 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               float d = static_cast<float>(acc[t][f][r]);
-              if constexpr (kOwnSums) d = __builtin_fmaf(-z[r], static_cast<float>(own[t][0]), d);
+              if constexpr (kOwnSums && !kUnits) d = __builtin_fmaf(-z[r], static_cast<float>(own[t][0]), d);
               total[t][f][r] = __builtin_fmaf(s[r], d, total[t][f][r]);
             }
         }
       }
+    if constexpr (kUnits) {
+#pragma unroll
+      for (int f = 0; f < RN; ++f) {
+        const int at = (wk * (S::kBN / 16) + wn * RN + f) * 64 + lane;
+        float z = kOffset;
+        if constexpr (ZEROS) z += kUnit * load16(from_s + (S::kAtZ - S::kAtS), 2 * at, sbf);
+        const float less_of = -load16(from_s, 2 * at, sbf) * z;
+#pragma unroll
+        for (int t = 0; t < RM; ++t) total[t][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(less_of, static_cast<float>(units[t][0]), total[t][f], 0, 0, 0);
+      }
+    }
   };
 #pragma unroll
   for (int d = 0; d < D - 1; ++d)
