@@ -486,41 +486,42 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
     s_row[i] = static_cast<uint32_t>((row < left_n ? row : left_n) * p.groups * 2);
   }
   auto group_of = [&](int unit) { return static_cast<uint32_t>((static_cast<uint64_t>(static_cast<uint32_t>(unit)) * p.group_factor) >> 31); };
-  auto copy = [&](int step) {
+  // Copies `from` .. `until` - 1 of this wave's S::kCopies of a step.
+  auto copy = [&](int step, int from, int until) {
     const uint32_t to = lds_at + step % D * S::kStage;
     const int xp0 = step * (WK * kRowPieces), wp0 = step * (WK * 4);
     if ((static_cast<int64_t>(step) + 1) * (128 * WK) <= p.K) {  // (what goes on along K in scalar registers)
       const uint8_t *xfrom = xbase + xp0 * 16, *wfrom = wbase + wp0 * 16;
 #pragma unroll
-      for (int i = 0; i < S::kMyX; ++i) dma_load16(xfrom, x_row[i] + x_piece[i] * 16, to + (wave + i * S::kW) % S::kX * 1024);
+      for (int i = 0; i < S::kMyX; ++i)
+        if (i >= from && i < until) dma_load16(xfrom, x_row[i] + x_piece[i] * 16, to + (wave + i * S::kW) % S::kX * 1024);
 #pragma unroll
-      for (int i = 0; i < S::kMyW; ++i) dma_load16(wfrom, w_row[i] + w_piece[i] * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
+      for (int i = 0; i < S::kMyW; ++i)
+        if (S::kMyX + i >= from && S::kMyX + i < until) dma_load16(wfrom, w_row[i] + w_piece[i] * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
     } else {  // pieces past the end of a row come from its last one
 #pragma unroll
       for (int i = 0; i < S::kMyX; ++i) {
         const int piece = xp0 + x_piece[i];
-        dma_load16(xbase, x_row[i] + static_cast<uint32_t>(piece < last_x ? piece : last_x) * 16, to + (wave + i * S::kW) % S::kX * 1024);
+        if (i >= from && i < until)
+          dma_load16(xbase, x_row[i] + static_cast<uint32_t>(piece < last_x ? piece : last_x) * 16, to + (wave + i * S::kW) % S::kX * 1024);
       }
 #pragma unroll
       for (int i = 0; i < S::kMyW; ++i) {
         const int piece = wp0 + w_piece[i];
-        dma_load16(wbase, w_row[i] + static_cast<uint32_t>(piece < last_w ? piece : last_w) * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
+        if (S::kMyX + i >= from && S::kMyX + i < until)
+          dma_load16(wbase, w_row[i] + static_cast<uint32_t>(piece < last_w ? piece : last_w) * 16, to + S::kAtW + (wave + i * S::kW) % S::kWt * 1024);
       }
     }
 #pragma unroll
     for (int i = 0; i < S::kMyS; ++i) {
-      const int c = (wave + i * S::kW) % S::kS;
-      if constexpr (kTurn) {
-        const int unit = wp0 + s_unit[i];
-        const uint32_t at = s_row[i] + 2 * group_of(unit < last_w ? unit : last_w);
-        dma_load_u16(sbase, at, to + S::kAtS + c * 256);
-        if constexpr (ZEROS) dma_load_u16(zbase, at, to + S::kAtZ + c * 256);
-      } else {
-        const int unit = wp0 + c / (S::kS / WK) * 4;
-        const uint32_t g = 2 * group_of(unit < last_w ? unit : last_w);
-        dma_load_u16(sbase + g, s_row[i], to + S::kAtS + c * 256);
-        if constexpr (ZEROS) dma_load_u16(zbase + g, s_row[i], to + S::kAtZ + c * 256);
-      }
+      const int nth = S::kMyX + S::kMyW + (ZEROS ? 2 * i : i), c = (wave + i * S::kW) % S::kS;
+      if (nth + (ZEROS ? 1 : 0) < from || nth >= until) continue;
+      const int unit = wp0 + (kTurn ? s_unit[i] : c / (S::kS / WK) * 4);
+      const uint32_t g = 2 * group_of(unit < last_w ? unit : last_w);
+      const uint8_t *sfrom = kTurn ? sbase : sbase + g, *zfrom = kTurn ? zbase : zbase + g;
+      const uint32_t at = kTurn ? s_row[i] + g : s_row[i];
+      if (nth >= from) dma_load_u16(sfrom, at, to + S::kAtS + c * 256);
+      if (ZEROS && nth + 1 >= from && nth + 1 < until) dma_load_u16(zfrom, at, to + S::kAtZ + c * 256);
     }
   };
   f32x4 total[RM][RN];
@@ -591,9 +592,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
       }
     }
   };
+  // The copies of the step D - 1 on: in front of the products, or dealt to the places between them, where all of them first hold a wave longer
+  // than they are late then (us, first and dealt: 300 x 4544 -> 4541 fp16, groups of 64 with zeros 49.0, 43.8; 2048 x 4096 -> 11008 fp16 212, 204, bf16
+  // 230, 218, int8 142, 140; 64 x 8192 -> 8192 fp16 34.2, 44.4).
+  constexpr bool kDealt = PARTS > 1 || RM >= 8;
+  constexpr int kSlots = (is_i8(XT) && !kTurn ? 2 : 4) * RN;
   auto multiply = [&](int step) {
     const int64_t k0 = (static_cast<int64_t>(step) * WK + wk) * 128;
-    if (WK > 1 && k0 >= p.K) return;
+    const bool more = step + D - 1 < steps;
+    auto slot = [&](int nth) {
+      if (kDealt && more) copy(step + D - 1, nth * S::kCopies / kSlots, (nth + 1) * S::kCopies / kSlots);
+    };
+    if (!kDealt && more) copy(step + D - 1, 0, S::kCopies);
+    if (WK > 1 && k0 >= p.K) return;  // (in the last step, which has no copies behind it)
     const uint8_t *from = lds + step % D * S::kStage, *from_s = from + S::kAtS;
     u32x4 w[RN];
 #pragma unroll
@@ -608,7 +619,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
     }
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
-        if (kTurn && k0 + 128 / PARTS * part >= p.K) break;
+        if (kTurn && k0 + 128 / PARTS * part >= p.K) break;  // (the last step, which has no copies behind it)
         if constexpr (kShared) sum(from, step, part, k0);
         Acc<XT> acc[RM][RN], own[kOwnSums && !kUnits ? RM : 1];
         __builtin_amdgcn_s_setprio(1);  // a wave among its products before one that widens codes for its next
@@ -638,6 +649,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
               const long wb = __builtin_bit_cast(long, widen8_in_order(w[f][s]));
 #pragma unroll
               for (int t = 0; t < RM; ++t) acc[t][f] = __builtin_amdgcn_mfma_i32_16x16x32_i8(wb, xa[t], acc[t][f], 0, 0, 0);
+              slot(s * RN + f);
             }
           }
         } else if constexpr (is_i8(XT)) {
@@ -660,6 +672,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
               const i32x4 wb = {static_cast<int>(wl[0]), static_cast<int>(wl[1]), static_cast<int>(wh[0]), static_cast<int>(wh[1])};
 #pragma unroll
               for (int t = 0; t < RM; ++t) acc[t][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wb, xa[t], acc[t][f], 0, 0, 0);
+              slot(s * RN + f);
             }
           }
         } else {
@@ -682,6 +695,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
               const u32x4 wb = XT == kBF16 ? widen_bf16(w[f][s]) : widen_f16(w[f][s]);
 #pragma unroll
               for (int t = 0; t < RM; ++t) acc[t][f] = mfma32<XT>(wb, xa[t], acc[t][f]);
+              slot(s * RN + f);
             }
           }
         }
@@ -728,10 +742,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   };
 #pragma unroll
   for (int d = 0; d < D - 1; ++d)
-    if (first + d < steps) copy(first + d);
+    if (first + d < steps) copy(first + d, 0, S::kCopies);
   for (int step = first; step < steps; ++step) {
     arrive(step);
-    if (step + D - 1 < steps) copy(step + D - 1);
     if (kShared && step > first) correct(step - 1);
     multiply(step);
   }
