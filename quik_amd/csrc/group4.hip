@@ -753,7 +753,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
     correct(steps - 1);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wait only)
-  const bool quads = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;  // four columns of a row in one store
+  typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(2)));  // four columns of a row in one store, at any of them
   float row_scale[RM];
 #pragma unroll
   for (int t = 0; t < RM; ++t) {
@@ -775,8 +775,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
       b[r] = sbf ? from_f32<true>(v[r]) : from_f32<false>(v[r]);
     }
     uint16_t *to = static_cast<uint16_t *>(p.out) + m * p.N + n;
-    if (quads) {
-      *reinterpret_cast<u32x2 *>(to) = u32x2{b[0] | b[1] << 16, b[2] | b[3] << 16};
+    if (n + 3 < p.N) {
+      *reinterpret_cast<loose2 *>(to) = loose2{b[0] | b[1] << 16, b[2] | b[3] << 16};
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
