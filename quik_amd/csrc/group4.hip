@@ -12,8 +12,8 @@
 // rounded to 16 bits.  sum x of a group comes from the same instruction with a matrix of ones.
 //
 // Up to 16 rows the stream of codes bounds it (group4_decode_kernel: 1 x 8192 -> 28672 fp16 29 us, 4.2 TB/s; bf16 with zeros 31; 16 x 13824 ->
-// 5120 int8 8.8; a copy on this card 5.2 TB/s).  Above, the issue of instructions does (group4_tile_kernel: 2048 x 4096 -> 11008 int8 137 us,
-// 1350 TOP/s, fp16 204 us, 905 TFLOP/s): per result and group a conversion (int8) and an fma beside the matrix instructions, and the
+// 5120 int8 8.8; a copy on this card 5.2 TB/s).  Above, the issue of instructions does (group4_tile_kernel: 2048 x 4096 -> 11008 int8 140 us,
+// 1320 TOP/s, fp16 204 us, 905 TFLOP/s): per result and group a conversion (int8) and an fma beside the matrix instructions, and the
 // widening, which a matrix instruction hides two to three of (measured: 16 cycles alone, 19 with two vector instructions beside it, 39 with
 // eight).  Widening less often is why the wide tiles are 128 rows per wave.
 #include "common.h"
@@ -881,7 +881,7 @@ struct Choice {
 };
 // The cheapest tiles and K split: rounds of the busiest CU, 4 us around them, and for a split the second launch (3 us) and its sums, written
 // and read.  us, as the rule has it and measured: 64 x 13824 -> 5120 int8, 64 rows, K in 6: 18.2, 19.7 (not split: 53); 64 x 8192 -> 8192
-// fp16, K in 4: 21.2, 21.7 (47); 128 x 13824 -> 5120 int8, K in 3: 26.3, 26.9 (53); 2048 x 4096 -> 11008 int8, 128 rows: 137, 137 (64
+// fp16, K in 4: 21.2, 21.7 (47); 128 x 13824 -> 5120 int8, K in 3: 26.3, 26.9 (53); 2048 x 4096 -> 11008 int8, 128 rows: 137, 140 (64
 // rows: 153).
 Choice choose(int64_t M, int64_t N, int64_t K, int acts, bool may_split) {
   Choice best{1, 1};
