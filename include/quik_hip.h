@@ -394,7 +394,7 @@ int quik_mixed_linear_fwd(const void *qx, const void *qw, const void *meta,
  *   q [rows, cols] int8 = rne(u * (127 / max|u|)), scale [rows] of scale_type (QUIK_F32, QUIK_F16 or QUIK_BF16), so that
  *   value ~ q * scale: |value - q * scale| <= scale / 2 before the scale is rounded to its type.
  * fp32 arithmetic; the norm's codes are those of the expression evaluated operation by operation.  A row of zeros has codes 0 and
- * scale 0; a row that holds a NaN or an infinity (in h, u or a factor of u), or whose squares pass fp32's range, codes 0 and a NaN scale.
+ * scale 0 (at an eps of 0 too); a row that holds a NaN or an infinity (in h, u or a factor of u), or whose squares pass fp32's range, codes 0 and a NaN scale.
  * The pitches are the distances of rows in elements (>= cols; not used with one row); q, sum and scale are contiguous.  Any cols
  * and any alignment of whole elements; 16-byte aligned rows of a multiple of 8 columns take wide accesses.
  * sum may be x or residual itself where that one's rows are contiguous (pitch cols); it may not overlap them otherwise. */

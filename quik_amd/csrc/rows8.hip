@@ -58,6 +58,7 @@ __device__ __forceinline__ void row_scale(uint32_t top_bits, float square, int64
   inv = bad || top_bits == 0 ? 0.0f : 127.0f / (top * pre);
   scale = top / 127.0f;
   if constexpr (OP != kSiluMul) scale = scale * (1.0f / sqrtf(square / static_cast<float>(cols) + eps));
+  if (top_bits == 0) scale = 0.0f;  // (a row of zeros at an eps of 0 has no finite factor)
   if (bad) scale = __builtin_nanf("");
 }
 
