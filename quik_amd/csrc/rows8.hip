@@ -6,7 +6,7 @@
 // value ~ q * scale.  The norm's factor is the same for a whole row and leaves the codes alone: largest magnitude and sum of
 // squares come from the same single pass, and a norm's codes do not depend on the order of a sum.  u is exact in fp32 (products of
 // 8 or 11 bits); every other step of the norm is one IEEE operation in fp32.  A row of zeros has codes 0 and scale 0; a row that
-// holds a NaN or an infinity, or whose squares pass the range of fp32, has codes 0 and a NaN as its scale.
+// holds a NaN or an infinity, or whose sum of squares passes the range of fp32, has codes 0 and a NaN as its scale.
 //
 // Bound by memory where there are many rows: 4096 x 8192 bf16 with a residual 40 us (235 MB, 5.9 TB/s), 2048 x 28672 bf16 silu_mul 56 us (294 MB,
 // 5.2 TB/s), a copy on this card 5.2.  One row is a chain of launch, one trip to memory, a reduction and a store: 2.4 us for 4096
@@ -48,16 +48,28 @@ __device__ __forceinline__ float row_value(float a, float b, float gain, uint16_
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
+// Rows of tiny bf16 numbers: where mean(h^2) + eps is below kTiny, squares may lie below fp32's smallest numbers, and the sum is made again
+// of h * kLift (2^-133 and more: squares from 2^-74 up; (2^31 columns) * kTiny * kLift^2 = 2^123).  fp16 squares are 2^-48 and more.
+constexpr float kTiny = 0x1p-100f, kLift = 0x1p96f;
+template <bool BF16, RowOp OP>
+__device__ __forceinline__ bool tiny_squares(uint32_t top_bits, float square, int64_t cols, float eps) {
+  return BF16 && OP != kSiluMul && top_bits != 0 && square < (kTiny - eps) * static_cast<float>(cols);
+}
+// the norm's factor from the sum of the squares of h * lift, over lift
+__device__ __forceinline__ float norm_factor(float square, int64_t cols, float eps, float lift) {
+  return 1.0f / sqrtf(square / static_cast<float>(cols) + eps * lift * lift);
+}
+
 // what is the same for the row: factor of the codes, scale
 template <RowOp OP>
-__device__ __forceinline__ void row_scale(uint32_t top_bits, float square, int64_t cols, float eps, float &pre, float &inv, float &scale) {
+__device__ __forceinline__ void row_scale(uint32_t top_bits, float square, int64_t cols, float eps, float lift, float &pre, float &inv, float &scale) {
   const float top = __uint_as_float(top_bits);
-  // (127 / top must not overflow: rows of tiny numbers are made larger by a power of two first)
+  // (127 / top must not overflow, top / 127 not lose bits: rows of tiny numbers are made larger by a power of two first)
   pre = top < 0x1p-100f ? 0x1p100f : 1.0f;
   const bool bad = top_bits >= kInfBits || !(square < __builtin_inff());
   inv = bad || top_bits == 0 ? 0.0f : 127.0f / (top * pre);
-  scale = top / 127.0f;
-  if constexpr (OP != kSiluMul) scale = scale * (1.0f / sqrtf(square / static_cast<float>(cols) + eps));
+  if constexpr (OP == kSiluMul) scale = top / 127.0f;
+  else scale = top * pre / 127.0f * norm_factor(square, cols, eps, lift) * (pre == 1.0f ? lift : lift * 0x1p-100f);
   if (top_bits == 0) scale = 0.0f;  // (a row of zeros at an eps of 0 has no finite factor)
   if (bad) scale = __builtin_nanf("");
 }
@@ -110,6 +122,13 @@ __device__ __forceinline__ void block_reduce(uint32_t &top, float &square, uint3
     top = umax(top, red[w]);
     square += reds[w];
   }
+}
+
+// a further sum of the workgroup's
+__device__ __forceinline__ void block_sum(float &v, uint32_t *red) {
+  __syncthreads();  // (the sums before are read)
+  uint32_t none = 0;
+  block_reduce(none, v, red);
 }
 
 // Sixteen bytes at the alignment of one element (global memory takes any), eight codes at any.
@@ -184,8 +203,16 @@ __global__ __launch_bounds__(1024) void rows8_kernel(RowArgs p) {
     }
   }
   block_reduce(top, square, red);
-  float pre, inv, scale;
-  row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
+  float lift = 1.0f, pre, inv, scale;
+  if (tiny_squares<BF16, OP>(top, square, p.cols, p.eps)) {
+    const uint16_t *h = OP == kNormAdd ? p.sum + row * p.cols : a;  // (a thread's own columns: what it has written of the sum)
+    lift = kLift;
+    square = 0.0f;
+    for (int64_t at = tid * int64_t{8}; at < p.cols; at += T * int64_t{8})
+      for (int64_t c = at; c < at + 8 && c < p.cols; ++c) square += to_f32<BF16>(h[c]) * lift * (to_f32<BF16>(h[c]) * lift);
+    block_sum(square, red);
+  }
+  row_scale<OP>(top, square, p.cols, p.eps, lift, pre, inv, scale);
   if (tid == 0) store_scale(p, row, scale);
   if (pre != 1.0f) {
 #pragma unroll
@@ -244,8 +271,15 @@ __global__ __launch_bounds__(1024) void rows8_long_kernel(RowArgs p) {
     if constexpr (OP == kNormAdd) sum[c] = h;
   }
   block_reduce(top, square, red);
-  float pre, inv, scale;
-  row_scale<OP>(top, square, p.cols, p.eps, pre, inv, scale);
+  float lift = 1.0f, pre, inv, scale;
+  if (tiny_squares<BF16, OP>(top, square, p.cols, p.eps)) {
+    const uint16_t *h = OP == kNormAdd ? sum : a;  // (a thread's own columns: what it has written of the sum)
+    lift = kLift;
+    square = 0.0f;
+    for (int64_t c = threadIdx.x; c < p.cols; c += 1024) square += to_f32<BF16>(h[c]) * lift * (to_f32<BF16>(h[c]) * lift);
+    block_sum(square, red);
+  }
+  row_scale<OP>(top, square, p.cols, p.eps, lift, pre, inv, scale);
   if (threadIdx.x == 0) store_scale(p, row, scale);
   for (int64_t c = threadIdx.x; c < p.cols; c += 1024) {  // (a thread's own columns: what it has written of the sum)
     uint16_t h = 0;
