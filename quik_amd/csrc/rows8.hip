@@ -30,12 +30,23 @@ struct RowArgs {
   int scale_type;
 };
 
-template <bool BF16, RowOp OP>
+// gate / (1 + exp(-gate)) * up.  exp2 and reciprocal are the hardware's, good to 1 ulp; with the rounding of exp2's argument a value is off by
+// (1.5 |gate| + 10) 2^-24 of it (6e-7 at gates around 0, 3e-6 at -30).  From kFar down exp(-gate) nears the end of fp32's range, where a
+// large up still makes a number of the value (and a row of nothing else has a scale): such a gate's exponential comes in halves, on either
+// factor, until they are 0 from -175 on (a value below 2^-116 whatever up is); within the same bound.
+constexpr uint32_t kFarBits = 0xC2AC0000u;  // -86: bits above are gates below (and negative NaNs)
+__device__ __forceinline__ float gated(float gate, float up) {
+  return gate * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.44269504088896340736f)) * up;
+}
+__device__ __forceinline__ float gated_far(float gate, float up) {
+  const float half = __builtin_amdgcn_exp2f(gate * 0.72134752044448170368f);
+  return gate * half * (up * half);
+}
+
+template <bool BF16, RowOp OP, bool FAR>
 __device__ __forceinline__ float row_value(float a, float b, float gain, uint16_t &h, float &square) {
   if constexpr (OP == kSiluMul) {
-    // exp and the quotient by the hardware's exp2 and reciprocal (1 ulp each): some 4e-7 of a value, 5e-5 of a code's step
-    const float e = __builtin_amdgcn_exp2f(a * -1.44269504088896340736f);
-    return a * __builtin_amdgcn_rcpf(1.0f + e) * b;
+    return FAR && __float_as_uint(a) > kFarBits ? gated_far(a, b) : gated(a, b);
   } else {
     if constexpr (OP == kNormAdd) {
       h = from_f32<BF16>(a + b);
@@ -183,8 +194,23 @@ __global__ __launch_bounds__(1024) void rows8_kernel(RowArgs p) {
       alignas(16) uint16_t vh[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        u[j][e] = row_value<BF16, OP>(to_f32<BF16>(va[j][e]), OP == kNorm ? 0.0f : to_f32<BF16>(vb[j][e]), OP == kSiluMul ? 0.0f : to_f32<BF16>(vg[j][e]),
+        u[j][e] = row_value<BF16, OP, false>(to_f32<BF16>(va[j][e]), OP == kNorm ? 0.0f : to_f32<BF16>(vb[j][e]), OP == kSiluMul ? 0.0f : to_f32<BF16>(vg[j][e]),
                                       vh[e], square);
+      }
+      if constexpr (OP == kSiluMul) {
+        uint32_t low = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) low = umax(low, __float_as_uint(to_f32<BF16>(va[j][e])));
+        if (low > kFarBits) {  // (us for 2048 x 28672 bf16: without 54.1, so 54.8, halves for all gates 58.4; 512 x 40000 in the kernel below 39.2, 41.7)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float gate = to_f32<BF16>(va[j][e]);
+            if (__float_as_uint(gate) > kFarBits) u[j][e] = gated_far(gate, to_f32<BF16>(vb[j][e]));
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
         top = umax(top, __float_as_uint(u[j][e]) & 0x7FFFFFFFu);
       }
       if constexpr (OP == kNormAdd) {
@@ -266,7 +292,7 @@ __global__ __launch_bounds__(1024) void rows8_long_kernel(RowArgs p) {
   float square = 0.0f;
   for (int64_t c = threadIdx.x; c < p.cols; c += 1024) {
     uint16_t h = 0;
-    const float u = row_value<BF16, OP>(to_f32<BF16>(a[c]), OP == kNorm ? 0.0f : to_f32<BF16>(b[c]), OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, square);
+    const float u = row_value<BF16, OP, true>(to_f32<BF16>(a[c]), OP == kNorm ? 0.0f : to_f32<BF16>(b[c]), OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, square);
     top = umax(top, __float_as_uint(u) & 0x7FFFFFFFu);
     if constexpr (OP == kNormAdd) sum[c] = h;
   }
@@ -285,7 +311,7 @@ __global__ __launch_bounds__(1024) void rows8_long_kernel(RowArgs p) {
     uint16_t h = 0;
     float unused = 0.0f;
     constexpr RowOp kAgain = OP == kNormAdd ? kNorm : OP;
-    const float u = row_value<BF16, kAgain>(to_f32<BF16>(OP == kNormAdd ? sum[c] : a[c]), OP == kSiluMul ? to_f32<BF16>(b[c]) : 0.0f,
+    const float u = row_value<BF16, kAgain, true>(to_f32<BF16>(OP == kNormAdd ? sum[c] : a[c]), OP == kSiluMul ? to_f32<BF16>(b[c]) : 0.0f,
                                             OP == kSiluMul ? 0.0f : to_f32<BF16>(p.gain[c]), h, unused);
     p.q[row * p.cols + c] = inv == 0.0f ? int8_t{0} : static_cast<int8_t>(code_bits(u * pre, inv) & 0xFFu);
   }
