@@ -324,8 +324,9 @@ def int4GroupMatmul(x, weight, scales, group_size, zeros=None, scale_row=None, b
 
     x [M, K] of the scales' type, or int8 with scale_row [M, 1] float32 (symmetric.rms_norm_quantize, silu_mul_quantize); weight [N,
     K/2] uint8, signed codes, low nibble = even k (qlinear.pack_to_i4); scales [N, ceil(K / group_size)] fp16 or bf16; zeros the
-    same shape and type; bias [N].  K and group_size are multiples of 32; the last group may be shorter.  Returns [M, N] of the
-    scales' type; sums in fp32, one rounding."""
+    same shape and type; bias [N].  K and group_size are multiples of 32; the last group may be shorter; x and weight start at a multiple
+    of 16 bytes, as tensors that are no views do (GroupLinear4bit copies other activations).  Returns [M, N] of the scales' type; sums in
+    fp32, one rounding.  A row of x that holds an infinity, or a bf16 value of 2^110 or more, gives infinities or NaNs."""
     op = "int4GroupMatmul"
     out = L.front().int4_group_matmul(x, weight, scales, group_size, zeros, scale_row, bias)
     if out is not None:

@@ -857,6 +857,8 @@ class GroupLinear4bit(torch.nn.Module):
         return mod
 
     def forward(self, x, scale=None):
-        out = matmul.int4GroupMatmul(x.reshape(-1, x.shape[-1]).contiguous(), self.int_weight, self.scales, self.group_size, zeros=self.zeros,
-                                     scale_row=scale, bias=self.bias)
+        rows = x.reshape(-1, x.shape[-1]).contiguous()
+        if rows.is_cuda and rows.data_ptr() % 16:     # (a contiguous view that starts between)
+            rows = rows.clone()
+        out = matmul.int4GroupMatmul(rows, self.int_weight, self.scales, self.group_size, zeros=self.zeros, scale_row=scale, bias=self.bias)
         return out.reshape(*x.shape[:-1], self.out_features)
