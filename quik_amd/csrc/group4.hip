@@ -824,20 +824,29 @@ __global__ __launch_bounds__(256) void group4_join_kernel(GroupArgs p) {
   }
 }
 
+// (2^31 threads per launch: rows beyond are further launches, which follow each other and share the memory of the parts' sums)
 template <int XT, int RM, int RN, int WM, int WN, int WK, int D, int PARTS, bool ZEROS>
 int launch_tile(const GroupArgs &p, hipStream_t st) {
   using S = TileShape<XT, RM, RN, WM, WN, WK, D, PARTS, ZEROS>;
   static_assert(S::kLds <= kLdsBytes, "");
   auto kern = group4_tile_kernel<XT, RM, RN, WM, WN, WK, D, PARTS, ZEROS>;
   if (int rc = prepare(kern, S::kLds)) return rc;
-  const int64_t units = ((p.M + S::kBM - 1) / S::kBM) * ((p.N + S::kBN - 1) / S::kBN) * p.splits;
-  if (units * S::kW * 64 > INT32_MAX) return QUIK_ERR_RANGE;
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(units)), dim3(64 * S::kW), S::kLds, st, p);
-  if (p.splits > 1) {
+  const int64_t across = (p.N + S::kBN - 1) / S::kBN * p.splits, most = INT32_MAX / (S::kW * 64) / across * S::kBM;
+  if (most == 0) return QUIK_ERR_RANGE;
+  for (int64_t m = 0; m < p.M; m += most) {
+    GroupArgs q = p;
+    q.M = p.M - m < most ? p.M - m : most;
+    q.x = static_cast<const uint8_t *>(p.x) + m * p.K * (is_i8(XT) ? 1 : 2);
+    if (is_i8(XT)) q.scale_row = p.scale_row + m;
+    q.out = static_cast<uint16_t *>(p.out) + m * p.N;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((q.M + S::kBM - 1) / S::kBM * across)), dim3(64 * S::kW), S::kLds, st, q);
     if (int rc = check_launch()) return rc;
-    hipLaunchKernelGGL((group4_join_kernel<XT>), dim3(static_cast<unsigned>((p.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, p);
+    if (p.splits > 1) {
+      hipLaunchKernelGGL((group4_join_kernel<XT>), dim3(static_cast<unsigned>((q.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, q);
+      if (int rc = check_launch()) return rc;
+    }
   }
-  return check_launch();
+  return QUIK_OK;
 }
 
 // Columns per workgroup for up to 16 rows: with FT matrix tiles side by side, the rounds that all CUs need, and the columns of a round dealt
