@@ -653,18 +653,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
             }
           }
         } else if constexpr (is_i8(XT)) {
+          static_assert(!kUnits, "");  // (parts of 32 columns: kTurn)
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             i32x4 xa[RM];
 #pragma unroll
             for (int t = 0; t < RM; ++t) {
               xa[t] = __builtin_bit_cast(i32x4, x_piece_of(from, t, s));
-              if constexpr (kUnits) {
-                const Acc<XT> v = add_ones(xa[t], Acc<XT>{0, 0, 0, 0});
-                units[t][0] = kg == s ? v[0] : units[t][0];
-              } else if constexpr (kOwnSums) {
-                own[t] = add_ones(xa[t], own[t]);
-              }
+              if constexpr (kOwnSums) own[t] = add_ones(xa[t], own[t]);
             }
 #pragma unroll
             for (int f = 0; f < RN; ++f) {
