@@ -392,9 +392,12 @@ int quik_mixed_linear_fwd(const void *qx, const void *qw, const void *meta,
  *              u = h * gain, value = u / sqrt(mean(h^2) + eps)
  *   silu_mul:  value = u = gate / (1 + exp(-gate)) * up
  *   q [rows, cols] int8 = rne(u * (127 / max|u|)), scale [rows] of scale_type (QUIK_F32, QUIK_F16 or QUIK_BF16), so that
- *   value ~ q * scale: |value - q * scale| <= scale / 2 before the scale is rounded to its type.
- * fp32 arithmetic; the norm's codes are those of the expression evaluated operation by operation.  A row of zeros has codes 0 and
- * scale 0 (at an eps of 0 too); a row that holds a NaN or an infinity (in h, u or a factor of u), or whose squares pass fp32's range, codes 0 and a NaN scale.
+ *   value ~ q * scale: |value - q * scale| <= scale / 2 but for fp32's roundings, before the scale is rounded to its type (fp16: an
+ *   infinity above 65504, steps of 2^-24 below 2^-14).
+ * fp32 arithmetic; the norm's codes are those of the expression evaluated operation by operation; silu_mul's values are off by
+ * (1.5 |gate| + 10) 2^-24 of them at most, and gates of -175 and less count as shut (value 0).  A row of zeros has codes 0 and scale 0 (at an
+ * eps of 0 too); a row that holds a NaN or an infinity (in h, u or a factor of u), or whose sum of squares passes fp32's range, codes 0 and a
+ * NaN scale.
  * The pitches are the distances of rows in elements (>= cols; not used with one row); q, sum and scale are contiguous.  Any cols
  * and any alignment of whole elements; 16-byte aligned rows of a multiple of 8 columns take wide accesses.
  * sum may be x or residual itself where that one's rows are contiguous (pitch cols); it may not overlap them otherwise. */
@@ -412,7 +415,8 @@ int quik_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up,
  *   scales  [N, ceil(K / group)] dtype; zeros the same shape in units of a code (any number, not only whole ones), or NULL
  *   bias    [N] dtype or NULL; out [M, N] dtype
  * K % 32 == 0, K <= 2^20, group % 32 == 0 (a group >= K: one scale per output column; the last group may be shorter); x and w 16-byte
- * aligned.  A group's product is summed in fp32 (int8: exactly) and scaled in fp32; one rounding to dtype.  A row of x that
+ * aligned; N <= 2^29 with more than 16 rows (else QUIK_ERR_RANGE).  Products are summed in blocks of up to 128 columns of one group,
+ * in fp32 (int8: exactly); a block's sum is scaled and added to the others in fp32, and there is one rounding to dtype.  A row of x that
  * holds an infinity, or a bf16 value of 2^110 or more, gives infinities or NaNs where the sums pass fp32's range. */
 int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const void *scales, const void *zeros,
                            const float *scale_row, const void *bias, int dtype, int64_t M, int64_t N, int64_t K,
@@ -421,6 +425,9 @@ int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const vo
  * overlap, free again behind the call on the stream) then holds the sums of each part, which a second launch adds in order.  Bytes
  * that such a call makes use of, 0: none.  With NULL or fewer bytes K is not split: slower, the same result within its rounding. */
 int64_t quik_int4_group_matmul_workspace_bytes(int x_bits, int dtype, int64_t M, int64_t N, int64_t K);
+/* the tile of the result that a workgroup of such a call computes at a time, rows << 16 | columns.  Up to 16 rows: 4, 8 or 16 rows and the
+ * columns that are dealt to it, in one, two or four (only with 16 rows) matrix tiles of 16. */
+int quik_int4_group_matmul_tile(int x_bits, int dtype, int zeros, int64_t M, int64_t N, int64_t K, int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

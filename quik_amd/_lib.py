@@ -73,6 +73,7 @@ SIGNATURES = {
     "quik_silu_mul_quantize": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _vp, _int, _vp]),
     "quik_int4_group_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
     "quik_int4_group_matmul_workspace_bytes": (_i64, [_int, _int, _i64, _i64, _i64]),
+    "quik_int4_group_matmul_tile": (_int, [_int, _int, _int, _i64, _i64, _i64, _i64]),
 }
 
 TILED_4 = 0x344C5451    # QUIK_TILED_4: operand buffers, tiled weights of 4 bits

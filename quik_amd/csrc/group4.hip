@@ -8,8 +8,9 @@
 //         1024 is 1032 + q or 1152 + 16 q, and one packed fma leaves q.  All exact.
 //   bf16  a nibble under the bits of 128 is 136 + q (there is no packed bf16 subtraction): the 136 goes the way of the zeros
 //   int8  w & 0xF0F0F0F0 and (w << 4) & 0xF0F0F0F0 are 16 q; the 16 leaves with the scale
-// Each group's product is a matrix-core sum of its own (fp32; exact int32 for int8), scaled in fp32: no product of a scale and a code is
-// rounded to 16 bits.  sum x of a group comes from the same instruction with a matrix of ones.
+// The product of a block of up to 128 columns of one group (32 in the kernel of few rows where groups are no multiples of 128) is a
+// matrix-core sum of its own (fp32; exact int32 for int8), scaled and added to the others in fp32: no product of a scale and a code is rounded
+// to 16 bits.  sum x of a block comes from the same instruction with a matrix of ones.
 //
 // Up to 16 rows the stream of codes bounds it (group4_decode_kernel: 1 x 8192 -> 28672 fp16 29 us, 4.2 TB/s; bf16 with zeros 31; 16 x 13824 ->
 // 5120 int8 8.8; a copy on this card 5.2 TB/s).  Above, the issue of instructions does (group4_tile_kernel: 2048 x 4096 -> 11008 int8 140 us,
@@ -850,26 +851,33 @@ int launch_tile(const GroupArgs &p, hipStream_t st) {
 // the activations come in), and as the activations' share (of 16 columns: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16
 // bits, half of it for int8).  us with the rule's FT and the next best, in turn on one card: 1 x 4096 -> 4096 5.3 (1), 6.1 (2); 1 x 8192 -> 28672 28.8
 // (2), 31.3 (1), bf16 with zeros 31.0 (1), 33.7 (2); 1 x 4096 -> 22016 int8 10.1 (2), 11.7 (1); 1 x 5120 -> 13824 10.6 (2), 12.6 (1).
-template <int XT, int RR, bool SMALL, bool ZEROS>
-int by_columns(GroupArgs p, hipStream_t st) {
-  const double share = (RR == 1 ? 0.1 : RR == 2 ? 0.3 : 1.0) * (is_i8(XT) ? 0.5 : 1.0), products = ZEROS || XT == kBF16 ? 0.5 : 0.25;
+struct Columns {
+  int matrix_tiles, width;
+};
+Columns deal_columns(int64_t N, int RR, bool i8, bool bf16, bool zeros) {
+  const double share = (RR == 1 ? 0.1 : RR == 2 ? 0.3 : 1.0) * (i8 ? 0.5 : 1.0), products = zeros || (bf16 && !i8) ? 0.5 : 0.25;
   const int64_t cus = num_cus();
   auto width = [&](int ft) {
-    const int64_t most = 16 * ft, rounds = ((p.N + most - 1) / most + cus - 1) / cus;
-    return static_cast<int>((p.N + rounds * cus - 1) / (rounds * cus));
+    const int64_t most = 16 * ft, rounds = ((N + most - 1) / most + cus - 1) / cus;
+    return static_cast<int>((N + rounds * cus - 1) / (rounds * cus));
   };
   auto cost = [&](int ft) {
     const int w = width(ft);
-    const int64_t rounds = ((p.N + w - 1) / w + cus - 1) / cus;
+    const int64_t rounds = ((N + w - 1) / w + cus - 1) / cus;
     return static_cast<double>(rounds) * ((1.0 - products) * w / 16.0 + products * ft + share);
   };
   const double c1 = cost(1), c2 = cost(2), c4 = RR == 4 ? cost(4) : 1e30;
-  if (c4 < c2 && c4 < c1) {
-    p.width = width(4);
-    if constexpr (RR == 4) return launch_decode<XT, RR, 4, 4, 2, SMALL, ZEROS>(p, st);
-  }
-  p.width = width(c2 < c1 ? 2 : 1);
-  if (c2 < c1) return launch_decode<XT, RR, 2, 8, 2, SMALL, ZEROS>(p, st);
+  const int ft = c4 < c2 && c4 < c1 ? 4 : c2 < c1 ? 2 : 1;
+  return Columns{ft, width(ft)};
+}
+
+template <int XT, int RR, bool SMALL, bool ZEROS>
+int by_columns(GroupArgs p, hipStream_t st) {
+  const Columns c = deal_columns(p.N, RR, is_i8(XT), is_bf16(XT), ZEROS);
+  p.width = c.width;
+  if constexpr (RR == 4)
+    if (c.matrix_tiles == 4) return launch_decode<XT, RR, 4, 4, 2, SMALL, ZEROS>(p, st);
+  if (c.matrix_tiles == 2) return launch_decode<XT, RR, 2, 8, 2, SMALL, ZEROS>(p, st);
   return launch_decode<XT, RR, 1, 8, 2, SMALL, ZEROS>(p, st);
 }
 
@@ -909,6 +917,10 @@ Choice choose(int64_t M, int64_t N, int64_t K, int acts, bool may_split) {
 }
 int acts_of(int x_bits, int dtype) { return x_bits == 8 ? 2 : dtype == QUIK_BF16 ? 1 : 0; }
 int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
+Choice choose_within(int64_t M, int64_t N, int64_t K, int acts, int64_t workspace_bytes) {
+  const Choice c = choose(M, N, K, acts, true);
+  return workspace_bytes < partial_bytes(M, N, c.splits) ? choose(M, N, K, acts, false) : c;
+}
 
 template <int XT, int PARTS, bool ZEROS>
 int by_rows(const GroupArgs &p, int64_t workspace_bytes, hipStream_t st) {
@@ -916,9 +928,7 @@ int by_rows(const GroupArgs &p, int64_t workspace_bytes, hipStream_t st) {
   if (p.M <= 8) return by_columns<XT, 2, (PARTS > 1), ZEROS>(p, st);
   if (p.M <= 16) return by_columns<XT, 4, (PARTS > 1), ZEROS>(p, st);
   GroupArgs q = p;
-  constexpr int acts = is_i8(XT) ? 2 : XT == kBF16 ? 1 : 0;
-  Choice c = choose(p.M, p.N, p.K, acts, true);
-  if (c.splits > 1 && (!p.partial || workspace_bytes < partial_bytes(p.M, p.N, c.splits))) c = choose(p.M, p.N, p.K, acts, false);
+  const Choice c = choose_within(p.M, p.N, p.K, is_i8(XT) ? 2 : XT == kBF16 ? 1 : 0, p.partial ? workspace_bytes : 0);
   q.splits = c.splits;
   if (c.plan == 0) return launch_tile<XT, 2, 2, 1, 4, 2, 2, PARTS, ZEROS>(q, st);
   if (c.plan == 1) return launch_tile<XT, 4, 2, 1, 4, 2, 2, PARTS, ZEROS>(q, st);
@@ -942,6 +952,16 @@ using namespace quik;
 extern "C" int64_t quik_int4_group_matmul_workspace_bytes(int x_bits, int dtype, int64_t M, int64_t N, int64_t K) {
   if (M <= 16 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > 1 << 20) return 0;
   return partial_bytes(M, N, choose(M, N, K, acts_of(x_bits, dtype), true).splits);
+}
+
+extern "C" int quik_int4_group_matmul_tile(int x_bits, int dtype, int zeros, int64_t M, int64_t N, int64_t K, int64_t workspace_bytes) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > 1 << 20) return 0;
+  if (M > 16) {
+    const TilePlan &t = kPlans[choose_within(M, N, K, acts_of(x_bits, dtype), workspace_bytes).plan];
+    return t.rows << 16 | t.cols;
+  }
+  const int rr = M <= 4 ? 1 : M <= 8 ? 2 : 4;
+  return 4 * rr << 16 | deal_columns(N, rr, x_bits == 8, dtype == QUIK_BF16, zeros != 0).width;
 }
 
 extern "C" int quik_int4_group_matmul(const void *x, int x_bits, const uint8_t *w, const void *scales, const void *zeros,
