@@ -12,11 +12,14 @@
 // matrix-core sum of its own (fp32; exact int32 for int8), scaled and added to the others in fp32: no product of a scale and a code is rounded
 // to 16 bits.  sum x of a block comes from the same instruction with a matrix of ones.
 //
-// Up to 16 rows the stream of codes bounds it (group4_decode_kernel: 1 x 8192 -> 28672 fp16 29 us, 4.2 TB/s; bf16 with zeros 31; 16 x 13824 ->
-// 5120 int8 8.8; a copy on this card 5.2 TB/s).  Above, the issue of instructions does (group4_tile_kernel: 2048 x 4096 -> 11008 int8 140 us,
-// 1320 TOP/s, fp16 204 us, 905 TFLOP/s): per result and group a conversion (int8) and an fma beside the matrix instructions, and the
-// widening, which a matrix instruction hides two to three of (measured: 16 cycles alone, 19 with two vector instructions beside it, 39 with
-// eight).  Widening less often is why the wide tiles are 128 rows per wave.
+// Times are per launch, launches one after the other, three weight matrices in turn, groups of 128 without zeros and K not split where nothing
+// else is said.  Up to 16 rows the stream of codes bounds it (group4_decode_kernel: 1 x 8192 -> 28672 fp16 26.5 us, 4.6 TB/s; bf16 with zeros
+// 30.9; 16 x 13824 -> 5120 int8 8.6; a copy on this card 5.2 TB/s).  Above, neither the vector nor the matrix unit is full (group4_tile_kernel:
+// 2048 x 4096 -> 11008 int8 140 us, 1320 TOP/s, fp16 205, 900 TFLOP/s, bf16 217): of a SIMD's cycles vector instructions take 43 % (int8; fp16 29,
+// bf16 35), matrix instructions 25 (37, 35), and the rest is waiting: two waves per SIMD, kept in step by a barrier per 128 columns.  Per
+// result and group there are a conversion (int8) and an fma beside the matrix instructions, and the widening, which a matrix instruction hides
+// two to three of (measured: 16 cycles alone, 19 with two vector instructions beside it, 39 with eight).  Widening less often is why the
+// wide tiles are 128 rows per wave.
 #include "common.h"
 
 #include <type_traits>
@@ -393,7 +396,8 @@ int launch_decode(const GroupArgs &p, hipStream_t st) {
   static_assert(smem <= kLdsBytes, "");
   auto kern = group4_decode_kernel<XT, RR, FT, W, D, SMALL, ZEROS>;
   if (int rc = prepare(kern, smem)) return rc;
-  // as many workgroups as run at a time, two of eight waves per CU at most (1 x 8192 -> 28672 fp16, 16 columns: 27.2 us, three 29.0)
+  // as many workgroups as run at a time, two of eight waves per CU at most (1 x 8192 -> 28672 fp16: one 26.8 us, two 26.4, three 26.5; in one
+  // matrix tile each two 29.8, three 30.8)
   const int per_cu = kLdsBytes / smem < 16 / W ? kLdsBytes / smem : 16 / W;
   const int64_t tiles = (p.N + p.width - 1) / p.width, slots = static_cast<int64_t>(num_cus()) * per_cu;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles < slots ? tiles : slots)), dim3(64 * W), smem, st, p);
@@ -415,11 +419,12 @@ struct TileShape {
   static constexpr int kReduce = WK > 1 ? WM * WN * WK * RM * RN * 1024 : 0;
   static constexpr bool kSums = ZEROS || XT == kBF16;
   // Sums of the activations: of eight row tiles the waves side by side make one each and take the others' a step later (us at 2048 x 4096 ->
-  // 11008, each wave all of them and this: bf16 267, 256, fp16 with zeros 292, 258); of fewer each wave makes all that it needs (64 x 4096
-  // -> 11008 bf16 with zeros, so and shared: 22.7, 26.3).
+  // 11008, each wave all of them and this: bf16 327, 218, fp16 with zeros 552, 248, int8 with zeros 186, 183); of
+  // fewer each wave makes all that it needs (so and shared: 300 x 4544 -> 4541 fp16, groups of 64 with zeros 41.1, 44.1; 64 x 4096 -> 11008
+  // bf16 with zeros, K split 21.9, 22.1).
   static constexpr bool kShared = kSums && RM >= 8, kOwnSums = kSums && !kShared;
   // Groups of 32 and the like: what the sums are multiplied by is a matrix product of its own, of 16 columns and 16 rows over the block's four
-  // units of 32 columns, in fp32 (300 x 4544 -> 4541 int8, groups of 32 with zeros: 65 us, so 56; groups of 64 lose 1 - 7 %).
+  // units of 32 columns, in fp32 (300 x 4544 -> 4541, groups of 32 with zeros: int8 56 us, so 46, fp16 49.6, 45.0; groups of 64 lost 1 - 7 %).
   static constexpr bool kUnits = kOwnSums && PARTS == 4;
   static constexpr int kAtSums = D * kStage, kRings = kAtSums + (kShared ? 2 * WK * PARTS * kBM * 4 : 0);  // of two steps
   static constexpr int kLds = kRings > kReduce ? kRings : kReduce;
@@ -440,8 +445,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   constexpr bool sbf = is_bf16(XT);
   const int blocks = static_cast<int>((p.K + 127) >> 7), all_steps = (blocks + WK - 1) / WK;
   // Workgroups go to the eight dies in turn: each die gets a run of tiles, in bands of four row tiles, column by column, so that those
-  // that run on a die at a time share both their rows and their weights in its L2 (2048 x 8192 -> 8192 fp16, 128x256 tiles: 312 us row
-  // tiles first, 306 in bands).  A tile whose K is split is `splits` workgroups, one after the other.
+  // that run on a die at a time share both their rows and their weights in its L2 (2048 x 8192 -> 8192 fp16, 128x256 tiles: 278 us row
+  // tiles first, 274 in bands).  A tile whose K is split is `splits` workgroups, one after the other.
   constexpr int kBand = 4;
   const int m_tiles = static_cast<int>((p.M + S::kBM - 1) / S::kBM), n_tiles = static_cast<int>((p.N + S::kBN - 1) / S::kBN);
   const int all = static_cast<int>(gridDim.x), die = blockIdx.x & 7, run = all >> 3, rest = all & 7;
@@ -458,8 +463,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
   const int last_w = static_cast<int>(p.K / 32) - 1, last_x = static_cast<int>(p.K * kSize / 16) - 1;
   // Where a row's 16-byte pieces lie in LDS: at the row's number exclusive-or the piece's; in wide tiles with the piece's two fields (lane row,
   // matrix step) changed over where a lane reads neighbouring pieces in its steps.  A 16-byte read goes by lanes 0 .. 3, 12 .. 15, 20 .. 27 and
-  // so on, which are at different banks then (else half as many cycles again per read: 2048 x 4096 -> 11008 int8 151 us, so 140, bf16
-  // 236, 229).  Copies in that order cost more than the banks in small tiles (64 x 8192 -> 8192 fp16 35.1 us, 36.5).
+  // so on, which are at different banks then (else half as many cycles again per read: 2048 x 4096 -> 11008 int8 144.5 us, so 140.6, fp16 206.9,
+  // 204.8, bf16 221.7, 216.8).  Copies in that order cost more than the banks in small tiles (64 x 8192 -> 8192 fp16 33.5 us, 34.1).
   constexpr bool kSwap = !kTurn && RM >= 8;
   auto place_of = [](int piece) { return !kSwap ? piece : is_i8(XT) ? (piece & 1) * 4 + (piece >> 1) : (piece & 3) * 4 + (piece >> 2); };
   auto piece_at = [](int place) { return !kSwap ? place : is_i8(XT) ? (place & 3) * 2 + (place >> 2) : (place & 3) * 4 + (place >> 2); };
@@ -594,8 +599,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void group4_tile_kernel(GroupArg
     }
   };
   // The copies of the step D - 1 on: in front of the products, or dealt to the places between them, where all of them first hold a wave longer
-  // than they are late then (us, first and dealt: 300 x 4544 -> 4541 fp16, groups of 64 with zeros 49.0, 43.8; 2048 x 4096 -> 11008 fp16 212, 204, bf16
-  // 230, 218, int8 142, 140; 64 x 8192 -> 8192 fp16 34.2, 44.4).
+  // than they are late then (us, first and dealt: 300 x 4544 -> 4541 fp16, groups of 64 with zeros 46.6, 41.4, int8, groups of 32 with zeros 52.4,
+  // 46.1; 2048 x 4096 -> 11008 fp16 206.7, 204.6, bf16 222.4, 217.2, but int8 138.7, 140.9; 64 x 8192 -> 8192 fp16 33.6, 41.9, K split 19.5, 20.8).
   constexpr bool kDealt = PARTS > 1 || RM >= 8;
   constexpr int kSlots = (is_i8(XT) && !kTurn ? 2 : 4) * RN;
   auto multiply = [&](int step) {
@@ -849,8 +854,9 @@ int launch_tile(const GroupArgs &p, hipStream_t st) {
 // Columns per workgroup for up to 16 rows: with FT matrix tiles side by side, the rounds that all CUs need, and the columns of a round dealt
 // to them evenly.  A round's time goes as the columns that are read, as the matrix tiles that are computed (a quarter of it; half where sums of
 // the activations come in), and as the activations' share (of 16 columns: 0.1 for one to four rows, 0.3 up to eight, 1 up to sixteen of 16
-// bits, half of it for int8).  us with the rule's FT and the next best, in turn on one card: 1 x 4096 -> 4096 5.3 (1), 6.1 (2); 1 x 8192 -> 28672 28.8
-// (2), 31.3 (1), bf16 with zeros 31.0 (1), 33.7 (2); 1 x 4096 -> 22016 int8 10.1 (2), 11.7 (1); 1 x 5120 -> 13824 10.6 (2), 12.6 (1).
+// bits, half of it for int8).  us with the rule's matrix tiles and the next best, in turn on one card: 1 x 4096 -> 4096 4.4 (1), 5.1 (2); 1 x 8192
+// -> 28672 26.6 (2), 30.0 (1), bf16 with zeros 30.9 (1), 32.1 (2); 1 x 4096 -> 22016 int8 8.7 (2), 10.2 (1); 1 x 5120 -> 13824 9.2 (2), 10.9 (1);
+// 16 x 13824 -> 5120 int8 8.6 (2), 11.5 (1); 16 x 5120 -> 13824 11.5 (4), 11.3 (2), 15.3 (1).
 struct Columns {
   int matrix_tiles, width;
 };
@@ -893,9 +899,9 @@ struct Choice {
   int plan, splits;
 };
 // The cheapest tiles and K split: rounds of the busiest CU, 4 us around them, and for a split the second launch (3 us) and its sums, written
-// and read.  us, as the rule has it and measured: 64 x 13824 -> 5120 int8, 64 rows, K in 6: 18.2, 19.7 (not split: 53); 64 x 8192 -> 8192
-// fp16, K in 4: 21.2, 21.7 (47); 128 x 13824 -> 5120 int8, K in 3: 26.3, 26.9 (53); 2048 x 4096 -> 11008 int8, 128 rows: 137, 140 (64
-// rows: 153).
+// and read.  us, as the rule has it and measured: 64 x 13824 -> 5120 int8, 64 rows, K in 6: 18.2, 17.7 (not split: 51.7); 64 x 8192 -> 8192
+// fp16, K in 4: 21.2, 19.6 (44); 128 x 13824 -> 5120 int8, K in 3: 26.3, 25.1 (51); 2048 x 4096 -> 11008 int8, 128 rows: 137, 140 (64
+// rows: 146.5).
 Choice choose(int64_t M, int64_t N, int64_t K, int acts, bool may_split) {
   Choice best{1, 1};
   double least = 1e30;
