@@ -625,7 +625,7 @@ PyObject *py_rms_norm_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) 
   const c10::DeviceIndex dev = current_gpu();
   const at::Tensor *x = matrix(args[0], dev), *w = plain(args[1], dev), *r = nullptr;
   if (!x || !w || (args[3] != Py_None && !(r = matrix(args[3], dev)))) Py_RETURN_NONE;
-  at::ScalarType scales;
+  at::ScalarType scales = at::kFloat;
   const int dt = dtype_of(*x), st = scale_type_of(args[4], scales);
   const double eps = PyFloat_AsDouble(args[2]);
   if (PyErr_Occurred()) {
@@ -653,7 +653,7 @@ PyObject *py_silu_mul_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) 
   const c10::DeviceIndex dev = current_gpu();
   const at::Tensor *g = matrix(args[0], dev), *u = matrix(args[1], dev);
   if (!g || !u) Py_RETURN_NONE;
-  at::ScalarType scales;
+  at::ScalarType scales = at::kFloat;
   const int dt = dtype_of(*g), st = scale_type_of(args[2], scales);
   if (dt < 0 || st < 0 || u->scalar_type() != g->scalar_type() || u->sizes() != g->sizes()) Py_RETURN_NONE;
   const int64_t rows = g->size(0), cols = g->size(1);
