@@ -429,6 +429,70 @@ int64_t quik_int4_group_matmul_workspace_bytes(int x_bits, int dtype, int64_t M,
  * columns that are dealt to it, in one, two or four (only with 16 rows) matrix tiles of 16. */
 int quik_int4_group_matmul_tile(int x_bits, int dtype, int zeros, int64_t M, int64_t N, int64_t K, int64_t workspace_bytes);
 
+/* ---- rows, products and caches in blocks of 32 -------------------------------------------------------
+ * No counterpart in the reference.  32 neighbouring columns share a power of two: codes of 4 bits (e2m1, two per byte, the even column in the
+ * low half) or 8 bits (e4m3) and one byte per block, e, for 2^(e - 127).  e is the exponent of the block's largest magnitude less
+ * that of the format's largest number (2; 8), at least 0; a code is the nearest number of the format (of two the even code; at most 6; 448).  A
+ * block that holds a NaN or an infinity has codes 0 and e = 255, and gives NaNs in whatever reads it.
+ *   bits 4: q [rows, cols / 2] uint8, cols even; bits 8: q [rows, cols]; scale [rows, ceil(cols / 32)] uint8 (a last block may be shorter)
+ * Pitches are distances of rows in elements (>= cols; not used with one row); outputs are contiguous.  Any cols (up to 2^30) and any alignment
+ * of whole elements; 16-byte aligned rows of a multiple of 8 columns take wide accesses. */
+int quik_mx_quantize(const void *x, int64_t x_pitch, int dtype, int64_t rows, int64_t cols, int bits, void *q, uint8_t *scale, void *stream);
+/* value = gate / (1 + exp(-gate)) * up, as quik_silu_mul_quantize computes it */
+int quik_mx_silu_mul_quantize(const void *gate, int64_t gate_pitch, const void *up, int64_t up_pitch, int dtype, int64_t rows, int64_t cols, int bits,
+                              void *q, uint8_t *scale, void *stream);
+/* h = dtype(x + residual) (written to `sum`; residual NULL: h = x and sum is not written); the codes are those of h * gain, and the factor of the
+ * row, 1 / sqrt(mean(h^2) + eps), is scale_row [rows]: value ~ q * 2^(e - 127) * scale_row.  At an eps of 0 a row of zeros has the factor 0;
+ * a row whose sum of squares passes fp32's range has a NaN, and one whose factor does (all of it below 2^-127, eps 0) an infinity.
+ * sum may be x or residual itself where that one's rows are contiguous (pitch cols); it may not overlap them otherwise. */
+int quik_mx_rms_norm_quantize(const void *x, int64_t x_pitch, const void *residual, int64_t residual_pitch, const void *gain, float eps, int dtype,
+                              int64_t rows, int64_t cols, int bits, void *sum, void *q, uint8_t *scale, float *scale_row, void *stream);
+/* out [rows, heads, cols] of dtype = q * 2^(e - 127) (* scale_row[row]) of the rows of q [source_rows, heads, cols] that index [rows] names (NULL: all of
+ * them, rows == source_rows); a row that is not there (below 0, source_rows and more) is zeros.  Blocks are of a head's columns. */
+int quik_mx_dequantize(const void *q, int bits, const uint8_t *scale, const int64_t *index, const float *scale_row, int dtype, int64_t rows,
+                       int64_t source_rows, int64_t heads, int64_t cols, void *out, void *stream);
+
+/* Heads of one product's columns on their way to attention, one launch: queries and keys are normed per head (where there is a gain: x / sqrt(mean(x^2) +
+ * eps) * gain), turned by their token's position (columns i and i + half with cos and sin [positions, half] of that position, i < half; columns from
+ * 2 half on stay), queries rounded to dtype, keys and values put into the cache rows of their token's slot in blocks of 32 columns of a head.
+ * q [tokens, q_heads, size], k, v [tokens, kv_heads, size], tokens *_pitch elements apart; q_out contiguous, not q itself; size even, up to 512.
+ * A token whose slot is below 0 or at `slots` or beyond writes nothing to the cache; slots of tokens are different from each other (of a slot named
+ * twice the row is of neither for certain).  A position below 0 or at `positions` or beyond gives NaNs. */
+typedef struct quik_mx_heads {
+  int32_t struct_bytes; /* sizeof(quik_mx_heads) */
+  int32_t dtype, k_bits, v_bits;
+  int64_t tokens, q_heads, kv_heads, size, half, positions, slots;
+  const void *q, *k, *v;
+  int64_t q_pitch, k_pitch, v_pitch;
+  const float *cos, *sin;
+  const int64_t *position, *slot;
+  const void *q_gain, *k_gain; /* [size] of dtype, or NULL: no norm */
+  void *q_out;
+  void *k_codes;    /* [slots, kv_heads, size / 2] or [slots, kv_heads, size] */
+  uint8_t *k_scale; /* [slots, kv_heads, ceil(size / 32)] */
+  void *v_codes;
+  uint8_t *v_scale;
+  float eps;
+  int32_t reserved;
+} quik_mx_heads;
+int quik_mx_rotate_to_cache(const quik_mx_heads *heads, void *stream);
+
+/* Product of rows in blocks of 32 with 4-bit weights in blocks of 32, on the scaled matrix instructions:
+ *   out[m,n] = dtype( scale_row[m] * sum_k x[m,k] * w[n,k] + bias[n] )
+ *   x  x_bits 4: [M, K/2] uint8, 8: [M, K]; x_scale [M, K/32];  w [N, K/2] uint8; w_scale [N, K/32];  scale_row [M] fp32 or NULL (1);  bias [N] or NULL
+ * K % 32 == 0, K <= 2^20; x and w 16-byte aligned.  Sums in fp32, one rounding. */
+int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row, const void *bias,
+                   int dtype, int64_t M, int64_t N, int64_t K, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+/* Calls whose tiles leave CUs idle split K: workspace (16-byte aligned, not to be shared by calls that may overlap, free again behind the call on the
+ * stream) then holds the sums of each part, which a second launch adds in order.  Bytes that such a call makes use of, 0: none.  With NULL or
+ * fewer bytes K is not split: slower, the same result within its rounding. */
+int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t N, int64_t K);
+/* The first half of a gated feed-forward block in one launch: gate = x w[:inner]^T and up = x w[inner:]^T (times scale_row, rounded to dtype, which is all
+ * that dtype is for), value = gate / (1 + exp(-gate)) * up, codes of q_bits: the bits that quik_mx_matmul and quik_mx_silu_mul_quantize give one after
+ * the other where K is not split.  w [2 inner, K/2], inner % 32 == 0. */
+int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row, int dtype,
+                         int64_t M, int64_t inner, int64_t K, int q_bits, void *q, uint8_t *q_scale, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ The package mirrors the reference's Python surface for this path:
 All compute runs in libquik_hip.so (hand-written HIP for gfx950) through a C ABI declared in
 include/quik_hip.h; there is no CPU or PyTorch fallback.
 """
-from . import asymmetric, matmul, symmetric  # noqa: F401
+from . import asymmetric, matmul, microscaled, symmetric  # noqa: F401
 from .version import __version__  # noqa: F401
 
-__all__ = ["asymmetric", "matmul", "symmetric", "__version__"]
+__all__ = ["asymmetric", "matmul", "microscaled", "symmetric", "__version__"]

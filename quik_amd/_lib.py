@@ -74,6 +74,14 @@ SIGNATURES = {
     "quik_int4_group_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
     "quik_int4_group_matmul_workspace_bytes": (_i64, [_int, _int, _i64, _i64, _i64]),
     "quik_int4_group_matmul_tile": (_int, [_int, _int, _int, _i64, _i64, _i64, _i64]),
+    "quik_mx_quantize": (_int, [_vp, _i64, _int, _i64, _i64, _int, _vp, _vp, _vp]),
+    "quik_mx_silu_mul_quantize": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _int, _vp, _vp, _vp]),
+    "quik_mx_rms_norm_quantize": (_int, [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _int, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp]),
+    "quik_mx_dequantize": (_int, [_vp, _int, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "quik_mx_rotate_to_cache": (_int, [_vp, _vp]),
+    "quik_mx_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "quik_mx_matmul_workspace_bytes": (_i64, [_int, _i64, _i64, _i64]),
+    "quik_mx_gated_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
 }
 
 TILED_4 = 0x344C5451    # QUIK_TILED_4: operand buffers, tiled weights of 4 bits
@@ -86,6 +94,15 @@ class QuikLayer(ctypes.Structure):
                 ("out_features", _i64), ("sym_divisor", ctypes.c_float), ("colmap_streams", ctypes.c_int32),
                 ("tiled_min_rows", ctypes.c_int32), ("tiled_format", ctypes.c_int32), ("colmap", _vp), ("int_weight", _vp),
                 ("weights_scales", _vp), ("reduced_w", _vp), ("fp_weight", _vp), ("bias", _vp), ("tiled_weight", _vp)]
+
+
+class QuikMxHeads(ctypes.Structure):
+    """struct quik_mx_heads of include/quik_hip.h."""
+    _fields_ = [("struct_bytes", ctypes.c_int32), ("dtype", ctypes.c_int32), ("k_bits", ctypes.c_int32), ("v_bits", ctypes.c_int32)] + \
+               [(name, _i64) for name in ("tokens", "q_heads", "kv_heads", "size", "half", "positions", "slots")] + \
+               [(name, _vp) for name in ("q", "k", "v")] + [(name, _i64) for name in ("q_pitch", "k_pitch", "v_pitch")] + \
+               [(name, _vp) for name in ("cos", "sin", "position", "slot", "q_gain", "k_gain", "q_out", "k_codes", "k_scale", "v_codes",
+                                         "v_scale")] + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
 _lib = None

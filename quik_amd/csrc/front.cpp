@@ -702,6 +702,231 @@ PyObject *py_int4_group_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) 
   });
 }
 
+// ---------------------------------------------------------------------------------------------- rows in blocks of 32
+constexpr int64_t kMxBlock = 32;
+
+// the bits of codes: of a number that says them, or of a tensor that holds them; 0: others
+int mx_bits(PyObject *o) {
+  if (!PyLong_Check(o)) return 0;
+  const long v = PyLong_AsLong(o);
+  if (PyErr_Occurred()) PyErr_Clear();
+  return v == 4 || v == 8 ? static_cast<int>(v) : 0;
+}
+int mx_bits(const at::Tensor &t) { return t.scalar_type() == at::kByte ? 4 : t.scalar_type() == at::kFloat8_e4m3fn ? 8 : 0; }
+at::Tensor mx_codes(int64_t rows, int64_t cols, int bits, c10::DeviceIndex dev) {
+  return bits == 4 ? new_empty({rows, cols / 2}, at::kByte, dev) : new_empty({rows, cols}, at::kFloat8_e4m3fn, dev);
+}
+at::Tensor mx_scales(int64_t rows, int64_t cols, c10::DeviceIndex dev) { return new_empty({rows, (cols + kMxBlock - 1) / kMxBlock}, at::kByte, dev); }
+uint8_t *bytes_of(const at::Tensor &t) { return static_cast<uint8_t *>(out_ptr(t)); }
+// the 16-bit type that a dtype object names; -1: another one
+int float_type_of(PyObject *o, at::ScalarType &type) {
+  if (!THPDtype_Check(o)) return -1;
+  type = reinterpret_cast<THPDtype *>(o)->scalar_type;
+  return type == at::kHalf ? QUIK_F16 : type == at::kBFloat16 ? QUIK_BF16 : -1;
+}
+bool optional(PyObject *o, c10::DeviceIndex dev, const at::Tensor *&t) { return o == Py_None || (t = plain(o, dev)); }
+
+// mx_quantize(src, bits) -> (q, scale) or None
+PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 2) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *x = matrix(args[0], dev);
+  const int bits = mx_bits(args[1]), dt = x ? dtype_of(*x) : -1;
+  if (dt < 0 || !bits || (bits == 4 && x->size(1) % 2 != 0)) Py_RETURN_NONE;
+  const int64_t rows = x->size(0), cols = x->size(1);
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = mx_codes(rows, cols, bits, dev), scale = mx_scales(rows, cols, dev);
+    const int rc = quik_mx_quantize(data_of(*x), x->stride(0), dt, rows, cols, bits, out_ptr(q), bytes_of(scale), stream_of(dev));
+    if (rc != QUIK_OK) return fail("quantize", rc);
+    return tuple_of({q, scale});
+  });
+}
+
+// mx_silu_mul_quantize(gate, up, bits) -> (q, scale) or None
+PyObject *py_mx_silu_mul_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 3) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *g = matrix(args[0], dev), *u = matrix(args[1], dev);
+  const int bits = mx_bits(args[2]), dt = g ? dtype_of(*g) : -1;
+  if (dt < 0 || !u || !bits || u->scalar_type() != g->scalar_type() || u->sizes() != g->sizes() || (bits == 4 && g->size(1) % 2 != 0)) Py_RETURN_NONE;
+  const int64_t rows = g->size(0), cols = g->size(1);
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = mx_codes(rows, cols, bits, dev), scale = mx_scales(rows, cols, dev);
+    const int rc = quik_mx_silu_mul_quantize(data_of(*g), g->stride(0), data_of(*u), u->stride(0), dt, rows, cols, bits, out_ptr(q), bytes_of(scale),
+                                             stream_of(dev));
+    if (rc != QUIK_OK) return fail("silu_mul_quantize", rc);
+    return tuple_of({q, scale});
+  });
+}
+
+// mx_rms_norm_quantize(x, weight, eps, residual, bits) -> (q, scale, scale_row, sum or None) or None
+PyObject *py_mx_rms_norm_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *x = matrix(args[0], dev), *w = plain(args[1], dev), *r = nullptr;
+  if (!x || !w || (args[3] != Py_None && !(r = matrix(args[3], dev)))) Py_RETURN_NONE;
+  const int dt = dtype_of(*x), bits = mx_bits(args[4]);
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const int64_t rows = x->size(0), cols = x->size(1);
+  if (dt < 0 || !bits || (bits == 4 && cols % 2 != 0) || !(eps >= 0) || w->dim() != 1 || w->size(0) != cols || w->scalar_type() != x->scalar_type() ||
+      (r && (r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = mx_codes(rows, cols, bits, dev), scale = mx_scales(rows, cols, dev), factor = new_empty({rows, 1}, at::kFloat, dev), sum;
+    if (r) sum = new_empty({rows, cols}, x->scalar_type(), dev);
+    const int rc = quik_mx_rms_norm_quantize(data_of(*x), x->stride(0), r ? data_of(*r) : nullptr, r ? r->stride(0) : 0, data_of(*w),
+                                             static_cast<float>(eps), dt, rows, cols, bits, r ? out_ptr(sum) : nullptr, out_ptr(q), bytes_of(scale),
+                                             static_cast<float *>(out_ptr(factor)), stream_of(dev));
+    if (rc != QUIK_OK) return fail("rms_norm_quantize", rc);
+    return tuple_of({q, scale, factor, sum});
+  });
+}
+
+// mx_dequantize(q, scale, dtype, rows, scale_row) -> out or None
+PyObject *py_mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *q = plain(args[0], dev), *s = plain(args[1], dev), *index = nullptr, *factor = nullptr;
+  at::ScalarType type = at::kHalf;
+  const int dt = float_type_of(args[2], type);
+  if (!q || !s || dt < 0 || !optional(args[3], dev, index) || !optional(args[4], dev, factor)) Py_RETURN_NONE;
+  const int bits = mx_bits(*q);
+  const int64_t dim = q->dim();
+  if (!bits || dim < 2 || dim > 4 || q->numel() == 0 || s->scalar_type() != at::kByte || s->dim() != dim ||
+      (index && (index->scalar_type() != at::kLong || index->dim() != 1 || index->numel() == 0)))
+    Py_RETURN_NONE;
+  const int64_t source = q->size(0), cols = q->size(dim - 1) * (bits == 4 ? 2 : 1), count = index ? index->numel() : source;
+  int64_t heads = 1, shape[4] = {count};
+  for (int64_t i = 0; i < dim - 1; ++i) {
+    if (s->size(i) != q->size(i)) Py_RETURN_NONE;
+    if (i) heads *= shape[i] = q->size(i);
+  }
+  shape[dim - 1] = cols;
+  if (s->size(dim - 1) != (cols + kMxBlock - 1) / kMxBlock || (factor && (factor->scalar_type() != at::kFloat || factor->numel() != count))) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor out = new_empty(at::IntArrayRef(shape, static_cast<size_t>(dim)), type, dev);
+    const int rc = quik_mx_dequantize(data_of(*q), bits, bytes_of(*s), index ? static_cast<const int64_t *>(data_of(*index)) : nullptr,
+                                      factor ? static_cast<const float *>(data_of(*factor)) : nullptr, dt, count, source, heads, cols, out_ptr(out),
+                                      stream_of(dev));
+    if (rc != QUIK_OK) return fail("dequantize", rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// what both products take: (x, x_scale, weight, weight_scale, dtype, scale_row)
+struct MxProduct {
+  const at::Tensor *x = nullptr, *xs = nullptr, *w = nullptr, *ws = nullptr, *row = nullptr;
+  at::ScalarType type = at::kHalf;
+  int dt = -1, bits = 0;
+  int64_t M = 0, N = 0, K = 0;
+  bool take(PyObject *const *args, c10::DeviceIndex dev) {
+    if (!(x = plain(args[0], dev)) || !(xs = plain(args[1], dev)) || !(w = plain(args[2], dev)) || !(ws = plain(args[3], dev)) ||
+        (dt = float_type_of(args[4], type)) < 0 || !optional(args[5], dev, row) || !(bits = mx_bits(*x)))
+      return false;
+    if (w->scalar_type() != at::kByte || xs->scalar_type() != at::kByte || ws->scalar_type() != at::kByte || x->dim() != 2 || w->dim() != 2 ||
+        xs->dim() != 2 || ws->dim() != 2 || x->numel() == 0 || w->numel() == 0)
+      return false;
+    M = x->size(0), N = w->size(0), K = 2 * w->size(1);
+    return x->size(1) * (8 / bits) == K && K % kMxBlock == 0 && xs->size(0) == M && ws->size(0) == N && xs->size(1) == K / kMxBlock &&
+           ws->size(1) == K / kMxBlock && (!row || (row->scalar_type() == at::kFloat && row->numel() == M));
+  }
+  const float *row_data() const { return row ? static_cast<const float *>(data_of(*row)) : nullptr; }
+};
+
+// mx_matmul(x, x_scale, weight, weight_scale, dtype, scale_row, bias) -> out or None
+PyObject *py_mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  MxProduct p;
+  const at::Tensor *b = nullptr;
+  if (!p.take(args, dev) || !optional(args[6], dev, b) || (b && (b->scalar_type() != p.type || b->numel() != p.N))) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor out = new_empty({p.M, p.N}, p.type, dev);
+    const int64_t need = quik_mx_matmul_workspace_bytes(p.bits, p.M, p.N, p.K);
+    c10::DataPtr ws;
+    if (need) ws = c10::hip::HIPCachingAllocator::get()->allocate(static_cast<size_t>(need));
+    const int rc = quik_mx_matmul(data_of(*p.x), p.bits, bytes_of(*p.xs), bytes_of(*p.w), bytes_of(*p.ws), p.row_data(), b ? data_of(*b) : nullptr, p.dt,
+                                  p.M, p.N, p.K, out_ptr(out), ws.get(), need, stream_of(dev));
+    if (rc != QUIK_OK) return fail("matmul", rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// mx_gated_matmul(x, x_scale, weight, weight_scale, dtype, scale_row, bits) -> (q, scale) or None
+PyObject *py_mx_gated_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  MxProduct p;
+  const int bits = mx_bits(args[6]);
+  if (!bits || !p.take(args, dev) || p.N % (2 * kMxBlock) != 0) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor q = mx_codes(p.M, p.N / 2, bits, dev), scale = mx_scales(p.M, p.N / 2, dev);
+    const int rc = quik_mx_gated_matmul(data_of(*p.x), p.bits, bytes_of(*p.xs), bytes_of(*p.w), bytes_of(*p.ws), p.row_data(), p.dt, p.M, p.N / 2, p.K,
+                                        bits, out_ptr(q), bytes_of(scale), stream_of(dev));
+    if (rc != QUIK_OK) return fail("gated_matmul", rc);
+    return tuple_of({q, scale});
+  });
+}
+
+// [tokens, heads, size] whose heads follow each other and whose tokens do not overlap, or null
+const at::Tensor *heads_of(PyObject *o, c10::DeviceIndex dev) {
+  const at::Tensor *t = strided(o, dev);
+  return t && t->dim() == 3 && t->numel() != 0 && (t->stride(2) == 1 || t->size(2) == 1) && (t->stride(1) == t->size(2) || t->size(1) == 1) &&
+                 (t->stride(0) >= t->size(1) * t->size(2) || t->size(0) == 1)
+             ? t
+             : nullptr;
+}
+
+// mx_rotate_to_cache(q, k, v, cos, sin, positions, slots, k_cache, k_scale, v_cache, v_scale, q_weight, k_weight, eps) -> out or None
+PyObject *py_mx_rotate_to_cache(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 14) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = current_gpu();
+  const at::Tensor *q = heads_of(args[0], dev), *k = heads_of(args[1], dev), *v = heads_of(args[2], dev), *t[8], *qw = nullptr, *kw = nullptr;
+  if (!q || !k || !v || !optional(args[11], dev, qw) || !optional(args[12], dev, kw)) Py_RETURN_NONE;
+  for (int i = 0; i < 8; ++i)
+    if (!(t[i] = plain(args[3 + i], dev)) || t[i]->numel() == 0) Py_RETURN_NONE;
+  const at::Tensor &cos = *t[0], &sin = *t[1], &positions = *t[2], &slots = *t[3], &kc = *t[4], &ks = *t[5], &vc = *t[6], &vs = *t[7];
+  const double eps = PyFloat_AsDouble(args[13]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const int64_t tokens = q->size(0), size = q->size(2), kv = k->size(1);
+  const int dt = dtype_of(*q), kb = mx_bits(kc), vb = mx_bits(vc);
+  auto typed = [](const at::Tensor &x, at::ScalarType type) { return x.scalar_type() == type; };
+  auto cache = [&](const at::Tensor &c, const at::Tensor &s, int bits) {
+    return bits && c.dim() == 3 && s.dim() == 3 && typed(s, at::kByte) && c.size(0) == kc.size(0) && s.size(0) == kc.size(0) && c.size(1) == kv &&
+           s.size(1) == kv && c.size(2) == (bits == 4 ? size / 2 : size) && s.size(2) == (size + kMxBlock - 1) / kMxBlock;
+  };
+  auto gain = [&](const at::Tensor *w) { return !w || (typed(*w, q->scalar_type()) && w->dim() == 1 && w->size(0) == size); };
+  if (dt < 0 || !typed(*k, q->scalar_type()) || !typed(*v, q->scalar_type()) || k->size(0) != tokens || k->size(2) != size || v->sizes() != k->sizes() ||
+      size % 2 != 0 || size > 512 || !typed(cos, at::kFloat) || !typed(sin, at::kFloat) || cos.dim() != 2 || sin.sizes() != cos.sizes() ||
+      2 * cos.size(1) > size || !typed(positions, at::kLong) || !typed(slots, at::kLong) || positions.dim() != 1 || slots.dim() != 1 ||
+      positions.size(0) != tokens || slots.size(0) != tokens || !cache(kc, ks, kb) || !cache(vc, vs, vb) || !gain(qw) || !gain(kw) || !(eps >= 0))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject * {
+    at::Tensor out = new_empty({tokens, q->size(1), size}, q->scalar_type(), dev);
+    quik_mx_heads h{};
+    h.struct_bytes = static_cast<int32_t>(sizeof h);
+    h.dtype = dt, h.k_bits = kb, h.v_bits = vb;
+    h.tokens = tokens, h.q_heads = q->size(1), h.kv_heads = kv, h.size = size, h.half = cos.size(1), h.positions = cos.size(0), h.slots = kc.size(0);
+    h.q = data_of(*q), h.k = data_of(*k), h.v = data_of(*v);
+    h.q_pitch = q->stride(0), h.k_pitch = k->stride(0), h.v_pitch = v->stride(0);
+    h.cos = static_cast<const float *>(data_of(cos)), h.sin = static_cast<const float *>(data_of(sin));
+    h.position = static_cast<const int64_t *>(data_of(positions)), h.slot = static_cast<const int64_t *>(data_of(slots));
+    h.q_gain = qw ? data_of(*qw) : nullptr, h.k_gain = kw ? data_of(*kw) : nullptr;
+    h.q_out = out_ptr(out), h.k_codes = out_ptr(kc), h.k_scale = bytes_of(ks), h.v_codes = out_ptr(vc), h.v_scale = bytes_of(vs);
+    h.eps = static_cast<float>(eps);
+    const int rc = quik_mx_rotate_to_cache(&h, stream_of(dev));
+    if (rc != QUIK_OK) return fail("rotate_to_cache", rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_forward)), METH_FASTCALL, nullptr},
     {"group_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_group_forward)), METH_FASTCALL, nullptr},
@@ -714,6 +939,13 @@ PyMethodDef kMethods[] = {
     {"rms_norm_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rms_norm_quantize)), METH_FASTCALL, nullptr},
     {"silu_mul_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_silu_mul_quantize)), METH_FASTCALL, nullptr},
     {"int4_group_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_int4_group_matmul)), METH_FASTCALL, nullptr},
+    {"mx_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_quantize)), METH_FASTCALL, nullptr},
+    {"mx_silu_mul_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_silu_mul_quantize)), METH_FASTCALL, nullptr},
+    {"mx_rms_norm_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_rms_norm_quantize)), METH_FASTCALL, nullptr},
+    {"mx_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_dequantize)), METH_FASTCALL, nullptr},
+    {"mx_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_matmul)), METH_FASTCALL, nullptr},
+    {"mx_gated_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_gated_matmul)), METH_FASTCALL, nullptr},
+    {"mx_rotate_to_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_mx_rotate_to_cache)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_front", "Host front end of quik_amd's hot calls.", -1, kMethods,

@@ -1,0 +1,741 @@
+// Products of rows in blocks of 32 with 4-bit weights in blocks of 32 (mx_format.h):
+//   y[m, n] = row[m] * sum_b 2^(ex[m, b] - 127) 2^(ew[n, b] - 127) sum_{k in b} x[m, k] w[n, k] + bias[n]
+// and the first half of a gated feed-forward block on them, with its result in such blocks.
+//
+// The scaled matrix instructions take a block of 32 codes per lane and its exponent byte, for either operand: 4-bit codes are 16 bytes, as they
+// lie in a row, and nothing is widened, scaled or summed apart from them.  8-bit codes lie in two pieces of 16 bytes, columns 16 g .. of the
+// first and of the second half of the instruction's columns (g: the lane's group), while the byte of group g is that of columns 32 g ..
+// Sums of products of 4-bit codes are exact up to fp32's alignment (off by 2^-24 of the magnitudes' sum per instruction); 8-bit ones are aligned to their largest product
+// first (2^-13 of the sum measured over codes of the whole range).
+// Columns behind the end of K: codes of x are made 0 in registers, the weights and bytes there are the row's last ones.
+#include "mx_format.h"
+#include "rows_math.h"
+
+#include <type_traits>
+
+namespace quik {
+namespace {
+
+struct MxArgs {
+  const uint8_t *x, *xs, *w, *ws;
+  const float *row;
+  const void *bias;
+  void *out;      // 16-bit [M, N], or (gated) codes
+  uint8_t *out_scale;  // gated
+  int64_t M, N, K;     // N: columns of the result (gated: of either half)
+  int32_t bf16, q_bits;
+  int32_t width;   // result columns per tile of the kernel of few rows
+  float *partial;  // K split: sums [splits][M][N rounded up to 4]
+  int32_t splits;
+};
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// one byte per lane: it lands in the low byte of the four at LDS address m0 + 4 i (the others are not to be read)
+__device__ __forceinline__ void dma_load_u8(const void *sbase, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" : : "s"(lds_addr), "v"(voff), "s"(sbase) : "memory", "m0");
+}
+
+// An operand of 4-bit codes is 16 bytes; of 8-bit ones 32.
+template <int BITS>
+struct Operand {
+  u32x4 v[BITS / 4];
+};
+__device__ __forceinline__ i32x8 as_operand(const Operand<4> &o) {
+  i32x8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = static_cast<int>(o.v[0][i]);
+  r[4] = r[5] = r[6] = r[7] = 0;  // (not read)
+  return r;
+}
+__device__ __forceinline__ i32x8 as_operand(const Operand<8> &o) {
+  i32x8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = static_cast<int>(o.v[0][i]);
+    r[4 + i] = static_cast<int>(o.v[1][i]);
+  }
+  return r;
+}
+template <int BITS>
+constexpr int kFormat = BITS == 4 ? 4 : 0;
+template <int XB>
+__device__ __forceinline__ f32x4 mfma16(const Operand<4> &w, const Operand<XB> &x, f32x4 c, uint32_t sw, uint32_t sx) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(w), as_operand(x), c, 4, kFormat<XB>, 0, static_cast<int>(sw), 0, static_cast<int>(sx));
+}
+template <int XB, int BYTE>
+__device__ __forceinline__ f32x16 mfma32(const Operand<4> &w, const Operand<XB> &x, f32x16 c, uint32_t sw, uint32_t sx) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(as_operand(w), as_operand(x), c, 4, kFormat<XB>, BYTE, static_cast<int>(sw), BYTE, static_cast<int>(sx));
+}
+
+__device__ __forceinline__ float from16(uint16_t v, bool bf16) { return bf16 ? to_f32<true>(v) : to_f32<false>(v); }
+__device__ __forceinline__ uint16_t to16(float v, bool bf16) { return bf16 ? from_f32<true>(v) : from_f32<false>(v); }
+__device__ __forceinline__ float bias_of(const MxArgs &p, int64_t n) { return from16(static_cast<const uint16_t *>(p.bias)[n], p.bf16); }
+// the activation of a gated block, of products rounded to the 16-bit type
+__device__ __forceinline__ float activate(float gate, float up, bool bf16) {
+  gate = from16(to16(gate, bf16), bf16);
+  up = from16(to16(up, bf16), bf16);
+  return __float_as_uint(gate) > kFarBits ? gated_far(gate, up) : gated(gate, up);
+}
+
+// Where a row's 16-byte pieces lie in LDS: at the piece's number exclusive-or this, so that 16 rows' reads of one piece go to different banks.
+template <int PIECES>
+__device__ __forceinline__ int turn_of(int row) {
+  static_assert(PIECES == 4 || PIECES == 8 || PIECES == 16 || PIECES == 32, "");
+  return PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+// Up to 16 token rows (TR of them in LDS), on 16x16x128 instructions: the weights are the rows of the result tile, the tokens its columns.  A workgroup
+// takes tiles of p.width <= 16 * FT result columns, which deals all of them evenly to the CUs; its W waves take blocks of STEPS * 128 columns of K in
+// turn and add their sums through LDS at a tile's end.  Operands and bytes come by direct copies, D - 1 blocks ahead and on into the next tile,
+// into a ring of the wave's own (no barrier but at a tile's end).  Gated: matrix tiles 0 .. FT / 2 - 1 are gates, the others the same columns of up.
+template <int XB, int TR, int FT, int W, int D, int STEPS, bool TAIL>
+struct RingShape {
+  static constexpr int kPw = 4 * STEPS, kPx = kPw * (XB / 4), kPlanes = TAIL ? 4 : 1;
+  static constexpr int kCW = FT * STEPS, kCX = TR * kPx / 64, kCSW = (16 * FT * STEPS + 63) / 64, kCSX = (TR * STEPS + 63) / 64;
+  static constexpr int kCopies = kCW + kCX + kPlanes * (kCSW + kCSX);
+  static constexpr int kAtX = kCW * 1024, kAtSW = kAtX + kCX * 1024, kAtSX = kAtSW + kPlanes * kCSW * 256, kStage = kAtSX + kPlanes * kCSX * 256;
+  static constexpr int kRed = W * FT * 1024, kLds = kRed + W * D * kStage;
+  static_assert(TR * kPx % 64 == 0 && kCopies * (D - 1) < 64, "");
+};
+
+template <int XB, int TR, int FT, int W, int D, int STEPS, bool TAIL, bool GATED>
+__global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
+  using S = RingShape<XB, TR, FT, W, D, STEPS, TAIL>;
+  static_assert(!GATED || FT == 4, "");  // (a block of 32 results)
+  extern __shared__ float red[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  const int nb = static_cast<int>(p.K / kMxBlock), steps = (nb + 3) / 4, blocks = (steps + STEPS - 1) / STEPS;
+  const int tiles = static_cast<int>((p.N + p.width - 1) / p.width);
+  uint8_t *ring = reinterpret_cast<uint8_t *>(red) + S::kRed + wave * (D * S::kStage);
+  const uint32_t ring_at = lds_address(ring);
+  const int64_t pitch_w = p.K / 2, pitch_x = p.K * XB / 8;
+
+  uint32_t from_x[S::kCX], from_sx[S::kCSX];
+#pragma unroll
+  for (int i = 0; i < S::kCX; ++i) {
+    const int64_t row = i * (64 / S::kPx) + lane / S::kPx;
+    from_x[i] = static_cast<uint32_t>((row < p.M ? row : p.M - 1) * pitch_x);
+  }
+#pragma unroll
+  for (int i = 0; i < S::kCSX; ++i) {
+    int64_t row = (i * 64 + lane) / STEPS;
+    row = row < p.M ? row : p.M - 1;
+    from_sx[i] = static_cast<uint32_t>(row * nb);
+  }
+  uint32_t from_w[S::kCW], from_sw[S::kCSW];
+  const uint8_t *wbase, *wbase_up, *sbase;
+  auto aim = [&](int tile) {  // at a tile's columns (past its end: the last one)
+    const int64_t n0 = static_cast<int64_t>(tile) * p.width, left = (p.N - n0 < p.width ? p.N - n0 : p.width) - 1;
+    wbase = p.w + n0 * pitch_w;
+    wbase_up = GATED ? wbase + p.N * pitch_w : wbase;
+    sbase = p.ws + n0 * nb;
+    constexpr int kRows = GATED ? 8 * FT : 16 * FT;  // of either half
+#pragma unroll
+    for (int i = 0; i < S::kCW; ++i) {
+      const int64_t row = (i * (64 / S::kPw) + lane / S::kPw) % kRows;
+      from_w[i] = static_cast<uint32_t>((row < left ? row : left) * pitch_w);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kCSW; ++i) {
+      const int at = (i * 64 + lane) / STEPS;
+      const int64_t row = at % kRows;
+      from_sw[i] = static_cast<uint32_t>(((row < left ? row : left) + (GATED && at >= kRows ? p.N : 0)) * nb);
+    }
+  };
+  auto copy = [&](int stage, int blk) {
+    const uint32_t to = ring_at + stage * S::kStage;
+    const bool whole = (blk + 1) * STEPS <= steps && (!TAIL || (blk + 1) * STEPS * 4 <= nb);
+    // (pieces past the end of a row come from its last one)
+    const int w0 = blk * S::kPw, last_w = nb - 1, x0 = blk * S::kPx, last_x = nb * (XB / 4) - 1;
+#pragma unroll
+    for (int i = 0; i < S::kCW; ++i) {
+      const int row = i * (64 / S::kPw) + lane / S::kPw, piece = w0 + ((lane % S::kPw) ^ turn_of<S::kPw>(row));
+      const uint8_t *base = GATED && i * (64 / S::kPw) >= 8 * FT ? wbase_up : wbase;
+      dma_load16(base, from_w[i] + static_cast<uint32_t>(whole || piece < last_w ? piece : last_w) * 16, to + i * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kCX; ++i) {
+      const int row = i * (64 / S::kPx) + lane / S::kPx, piece = x0 + ((lane % S::kPx) ^ turn_of<S::kPx>(row));
+      dma_load16(p.x, from_x[i] + static_cast<uint32_t>(whole || piece < last_x ? piece : last_x) * 16, to + S::kAtX + i * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kCSW + S::kCSX; ++i) {
+      const bool is_x = i >= S::kCSW;
+      const int j = is_x ? i - S::kCSW : i, step = blk * STEPS + (j * 64 + lane) % STEPS;
+      const uint32_t row = is_x ? from_sx[is_x ? j : 0] : from_sw[is_x ? 0 : j];
+      const uint32_t at = to + (is_x ? S::kAtSX : S::kAtSW) + j * 256;
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int plane = 0; plane < 4; ++plane) {
+          const int b = 4 * step + plane;
+          dma_load_u8(is_x ? p.xs : sbase, row + static_cast<uint32_t>(b < nb ? b : nb - 1), at + plane * (is_x ? S::kCSX : S::kCSW) * 256);
+        }
+      } else {
+        dma_load_u32(is_x ? p.xs : sbase, row + 4u * static_cast<uint32_t>(step < steps ? step : steps - 1), at);
+      }
+    }
+  };
+  int ahead_tile = blockIdx.x, ahead_blk = wave;
+  auto copy_next = [&](int stage) {
+    copy(stage, ahead_blk);
+    ahead_blk += W;
+    if (ahead_blk >= blocks) {
+      ahead_blk = wave;
+      if (ahead_tile + static_cast<int>(gridDim.x) < tiles) {  // (past the last tile: its first blocks once more, not used)
+        ahead_tile += gridDim.x;
+        aim(ahead_tile);
+      }
+    }
+  };
+  if (wave < blocks) {
+    aim(ahead_tile);
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d) copy_next(d);
+  }
+  const int token = TR >= 16 ? col : col % TR;
+  int stage = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    f32x4 acc[FT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f) acc[f] = f32x4{0, 0, 0, 0};
+    for (int blk = wave; blk < blocks; blk += W) {
+      copy_next(stage == 0 ? D - 1 : stage - 1);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 1)));
+      asm volatile("" ::: "memory");
+      const uint8_t *from = ring + stage * S::kStage;
+      // a row's bytes of all steps; whole planes: of this lane's group
+      uint32_t sw[FT][STEPS], sx[STEPS];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int plane = TAIL ? kg : 0;
+        sx[s] = *reinterpret_cast<const uint32_t *>(from + S::kAtSX + plane * S::kCSX * 256 + (token * STEPS + s) * 4);
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+          sw[f][s] = *reinterpret_cast<const uint32_t *>(from + S::kAtSW + plane * S::kCSW * 256 + ((16 * f + col) * STEPS + s) * 4);
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        if (blk * STEPS + s >= steps) break;
+        Operand<XB> x;
+#pragma unroll
+        for (int h = 0; h < XB / 4; ++h) {
+          const int piece = XB == 4 ? 4 * s + kg : 8 * s + 4 * h + kg;
+          x.v[h] = *reinterpret_cast<const u32x4 *>(from + S::kAtX + (token * S::kPx + (piece ^ turn_of<S::kPx>(token))) * 16);
+          if constexpr (TAIL) {
+            const int b = 4 * (blk * STEPS + s) + (XB == 4 ? kg : 2 * h + (kg >> 1));
+            if (b >= nb) x.v[h] = u32x4{0, 0, 0, 0};
+          }
+        }
+        const uint32_t by_x = TAIL ? sx[s] : sx[s] >> (8 * kg);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+          Operand<4> w;
+          w.v[0] = *reinterpret_cast<const u32x4 *>(from + ((16 * f + col) * S::kPw + ((4 * s + kg) ^ turn_of<S::kPw>(col))) * 16);
+          acc[f] = mfma16<XB>(w, x, acc[f], TAIL ? sw[f][s] : sw[f][s] >> (8 * kg), by_x);
+        }
+      }
+      stage = stage == D - 1 ? 0 : stage + 1;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wait only; this stage is copied to next: its reads are done)
+    }
+    // the waves' sums: value r of lane l is column 16 f + 4 (l / 16) + r of token l % 16
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[((wave * FT + f) * 4 + r) * 64 + lane] = acc[f][r];
+    __syncthreads();
+    const int64_t n0 = static_cast<int64_t>(tile) * p.width;
+    auto sum = [&](int m, int n) {
+      const int at = ((n >> 4) * 4 + (n & 3)) * 64 + ((n >> 2) & 3) * 16 + m;
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v += red[i * FT * 256 + at];
+      return p.row ? v * p.row[m] : v;
+    };
+    if constexpr (GATED) {
+      for (int e = threadIdx.x; e < p.M * 32; e += 64 * W) {
+        const int m = e >> 5, n = e & 31;  // (inner is a multiple of 32: the block is whole)
+        const float v = activate(sum(m, n), sum(m, 32 + n), p.bf16);
+        uint32_t top = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) top = umax(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+        const int64_t block = m * (p.N / kMxBlock) + n0 / kMxBlock;
+        const uint32_t byte = p.q_bits == 4 ? block_byte<4>(top) : block_byte<8>(top);
+        const float other = __shfl_xor(v, 1);
+        if (n == 0) p.out_scale[block] = static_cast<uint8_t>(byte);
+        const float pair[8] = {v, other, 0, 0, 0, 0, 0, 0};
+        if (p.q_bits == 8) static_cast<uint8_t *>(p.out)[block * 32 + n] = static_cast<uint8_t>(encode8(pair, byte).x);
+        else if (n % 2 == 0) static_cast<uint8_t *>(p.out)[block * 16 + n / 2] = static_cast<uint8_t>(encode4(pair, byte));
+      }
+    } else {
+      for (int e = threadIdx.x; e < p.M * 16 * FT; e += 64 * W) {
+        const int m = e / (16 * FT), n = e % (16 * FT);
+        if (n >= p.width || n0 + n >= p.N) continue;
+        float v = sum(m, n);
+        if (p.bias) v += bias_of(p, n0 + n);
+        static_cast<uint16_t *>(p.out)[m * p.N + n0 + n] = to16(v, p.bf16);
+      }
+    }
+    __syncthreads();  // (the sums are read: the next tile's may be written)
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no copy is under way when the workgroup's LDS goes to another)
+}
+
+// More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on steps of 128 columns.  All operands
+// come to LDS by direct copies, D - 1 steps ahead, one barrier per step, in its middle: it says that the next step's operands are there, whose
+// first half a wave reads while it multiplies this one's second.  Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
+template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL>
+struct TileShape {
+  static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kPx = XB, kPlanes = TAIL ? 4 : 1;
+  static constexpr int kCX = kBM * kPx / 64, kCW = kBN * 4 / 64, kCSX = (kBM + 63) / 64, kCSW = (kBN + 63) / 64;
+  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kMyS = (kCSX + kCSW + kW - 1) / kW;
+  static constexpr int kCopies = kMyX + kMyW + kMyS * kPlanes;
+  static constexpr int kAtW = kCX * 1024, kAtS = kAtW + kCW * 1024, kStage = kAtS + kPlanes * (kCSX + kCSW) * 256;
+  static constexpr int kLds = D * kStage;
+  static_assert(D >= 3 && kCopies * (D - 2) < 64 && kBM * kPx % 64 == 0, "");
+};
+
+template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL, bool GATED>
+__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
+  using S = TileShape<XB, RM, RN, WM, WN, D, TAIL>;
+  static_assert(!GATED || RN % 2 == 0, "");
+  constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;  // result columns per tile
+  extern __shared__ float red[];
+  uint8_t *lds = reinterpret_cast<uint8_t *>(red);
+  const uint32_t lds_at = lds_address(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, kg = lane >> 5;
+  const int wn = wave % WN, wm = wave / WN;
+  const int nb = static_cast<int>(p.K / kMxBlock), all_steps = (nb + 3) / 4;
+  // Workgroups go to the eight dies in turn: each die gets a run of tiles, in bands of four row tiles, column by column, so that those
+  // that run on a die at a time share both their rows and their weights in its L2.  A tile whose K is split is `splits` workgroups, one after
+  // the other.
+  constexpr int kBand = 4;
+  const int m_tiles = static_cast<int>((p.M + S::kBM - 1) / S::kBM), n_tiles = static_cast<int>((p.N + kCols - 1) / kCols);
+  const int all = static_cast<int>(gridDim.x), die = blockIdx.x & 7, run = all >> 3, rest = all & 7;
+  const int unit = die * run + (die < rest ? die : rest) + static_cast<int>(blockIdx.x >> 3), tile = unit / p.splits, split = unit % p.splits;
+  const int band = tile / (kBand * n_tiles), in_band = tile - band * kBand * n_tiles;
+  const int high = m_tiles - band * kBand < kBand ? m_tiles - band * kBand : kBand;
+  const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * S::kBM, n0 = static_cast<int64_t>(in_band / high) * kCols;
+  const int first = static_cast<int>(static_cast<int64_t>(all_steps) * split / p.splits);
+  const int steps = static_cast<int>(static_cast<int64_t>(all_steps) * (split + 1) / p.splits);
+
+  const int64_t pitch_w = p.K / 2, pitch_x = p.K * XB / 8, left_m = p.M - 1 - m0, left_n = p.N - 1 - n0;
+  const uint8_t *xbase = p.x + m0 * pitch_x, *wbase = p.w + n0 * pitch_w, *xsbase = p.xs + m0 * nb, *wsbase = p.ws + n0 * nb;
+  // weight row R of the tile: wave R / (32 RN)'s, of its tiles the first half gates, the second up
+  auto column_of = [](int R) { return GATED ? R / (32 * RN) * (16 * RN) + R % (16 * RN) : R; };
+  auto is_up = [](int R) { return GATED && R % (32 * RN) >= 16 * RN; };
+  // this wave's copies: the row's offset and the piece of the step that this lane takes
+  uint32_t x_row[S::kMyX], w_row[S::kMyW], s_row[S::kMyS];
+  int x_piece[S::kMyX], w_piece[S::kMyW];
+#pragma unroll
+  for (int i = 0; i < S::kMyX; ++i) {
+    const int row = (wave + i * S::kW) % S::kCX * (64 / S::kPx) + lane / S::kPx;
+    x_piece[i] = (lane % S::kPx) ^ turn_of<S::kPx>(row);
+    x_row[i] = static_cast<uint32_t>((row < left_m ? row : left_m) * pitch_x);
+  }
+#pragma unroll
+  for (int i = 0; i < S::kMyW; ++i) {
+    const int row = (wave + i * S::kW) % S::kCW * 16 + (lane >> 2), n = column_of(row);
+    w_piece[i] = (lane & 3) ^ turn_of<4>(row);
+    w_row[i] = static_cast<uint32_t>((n < left_n ? n : left_n) * pitch_w);
+  }
+#pragma unroll
+  for (int i = 0; i < S::kMyS; ++i) {
+    const int c = (wave + i * S::kW) % (S::kCSX + S::kCSW);
+    if (c < S::kCSX) {
+      const int row = c * 64 + lane;
+      s_row[i] = static_cast<uint32_t>((row < left_m ? row : left_m) * nb);
+    } else {
+      int row = (c - S::kCSX) * 64 + lane;
+      row = row < S::kBN ? row : S::kBN - 1;
+      const int n = column_of(row);
+      s_row[i] = static_cast<uint32_t>(((n < left_n ? n : left_n) + (is_up(row) ? p.N : 0)) * nb);
+    }
+  }
+  auto copy = [&](int step) {
+    const uint32_t to = lds_at + step % D * S::kStage;
+    const bool whole = !TAIL || (step + 1) * 4 <= nb;
+    const uint8_t *xfrom = xbase + step * (S::kPx * 16), *wfrom = wbase + step * 64;
+    const int last_x = nb * (XB / 4) - 1 - step * S::kPx, last_w = nb - 1 - step * 4;  // (pieces past the end of a row come from its last one)
+#pragma unroll
+    for (int i = 0; i < S::kMyX; ++i) {
+      const int piece = whole || x_piece[i] < last_x ? x_piece[i] : last_x;
+      dma_load16(xfrom, x_row[i] + static_cast<uint32_t>(piece) * 16, to + (wave + i * S::kW) % S::kCX * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kMyW; ++i) {
+      const int c = (wave + i * S::kW) % S::kCW, piece = whole || w_piece[i] < last_w ? w_piece[i] : last_w;
+      dma_load16(is_up(c * 16) ? wfrom + p.N * pitch_w : wfrom, w_row[i] + static_cast<uint32_t>(piece) * 16, to + S::kAtW + c * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kMyS; ++i) {
+      const int c = (wave + i * S::kW) % (S::kCSX + S::kCSW);
+      const uint8_t *base = c < S::kCSX ? xsbase : wsbase;
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int plane = 0; plane < 4; ++plane) {
+          const int b = 4 * step + plane;
+          dma_load_u8(base + (b < nb ? b : nb - 1), s_row[i], to + S::kAtS + (plane * (S::kCSX + S::kCSW) + c) * 256);
+        }
+      } else {
+        dma_load_u32(base + 4 * step, s_row[i], to + S::kAtS + c * 256);
+      }
+    }
+  };
+  f32x16 acc[RM][RN];
+#pragma unroll
+  for (int t = 0; t < RM; ++t)
+#pragma unroll
+    for (int f = 0; f < RN; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][f][r] = 0.0f;
+
+  struct Half {
+    Operand<XB> x[RM];
+    Operand<4> w[RN];
+    uint32_t sx[RM], sw[RN];
+  };
+  // half s of a step: 64 columns.  Bytes: of this lane's group, without planes also those of the second half, in byte 2
+  auto read = [&](int step, int s, Half &h) {
+    const uint8_t *from = lds + step % D * S::kStage;
+#pragma unroll
+    for (int t = 0; t < RM; ++t) {
+      const int row = (wm * RM + t) * 32 + col;
+#pragma unroll
+      for (int i = 0; i < XB / 4; ++i) {
+        const int piece = XB == 4 ? 2 * s + kg : 4 * s + 2 * i + kg;
+        h.x[t].v[i] = *reinterpret_cast<const u32x4 *>(from + (row * S::kPx + (piece ^ turn_of<S::kPx>(row))) * 16);
+        if constexpr (TAIL) {
+          if (4 * step + 2 * s + (XB == 4 ? kg : i) >= nb) h.x[t].v[i] = u32x4{0, 0, 0, 0};
+        }
+      }
+      const int plane = TAIL ? 2 * s + kg : 0;
+      if (TAIL || s == 0) h.sx[t] = *reinterpret_cast<const uint32_t *>(from + S::kAtS + (plane * (S::kCSX + S::kCSW) * 64 + row) * 4) >> (TAIL ? 0 : 8 * kg);
+    }
+#pragma unroll
+    for (int f = 0; f < RN; ++f) {
+      const int row = (wn * RN + f) * 32 + col;
+      h.w[f].v[0] = *reinterpret_cast<const u32x4 *>(from + S::kAtW + (row * 4 + ((2 * s + kg) ^ turn_of<4>(row))) * 16);
+      const int plane = TAIL ? 2 * s + kg : 0;
+      if (TAIL || s == 0)
+        h.sw[f] = *reinterpret_cast<const uint32_t *>(from + S::kAtS + ((plane * (S::kCSX + S::kCSW) + S::kCSX) * 64 + row) * 4) >> (TAIL ? 0 : 8 * kg);
+    }
+  };
+  auto multiply = [&](const Half &h, const uint32_t (&sx)[RM], const uint32_t (&sw)[RN], auto second) {
+    constexpr int kByte = decltype(second)::value && !TAIL ? 2 : 0;
+#pragma unroll
+    for (int f = 0; f < RN; ++f)
+#pragma unroll
+      for (int t = 0; t < RM; ++t) acc[t][f] = mfma32<XB, kByte>(h.w[f], h.x[t], acc[t][f], sw[f], sx[t]);
+  };
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d)
+    if (first + d < steps) copy(first + d);
+  if (first + D - 2 < steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 2)));
+  else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  asm volatile("s_barrier" ::: "memory");
+  Half a, b;
+  read(first, 0, a);
+  for (int step = first; step < steps; ++step) {
+    uint32_t sx[RM], sw[RN];
+#pragma unroll
+    for (int t = 0; t < RM; ++t) sx[t] = a.sx[t];
+#pragma unroll
+    for (int f = 0; f < RN; ++f) sw[f] = a.sw[f];
+    read(step, 1, b);
+    multiply(a, sx, sw, std::false_type{});
+    if (step + 1 < steps) {
+      // the next step's operands: of this wave's copies, those of the steps behind it may be under way
+      if (step + D - 2 < steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 3)));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier: every wave's reads of the step before are done)
+      if (step + D - 1 < steps) copy(step + D - 1);
+      read(step + 1, 0, a);
+    }
+    if constexpr (TAIL) multiply(b, b.sx, b.sw, std::true_type{});
+    else multiply(b, sx, sw, std::true_type{});
+  }
+  // value r of a lane: column 8 (r / 4) + 4 kg + r % 4 of token col
+  typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(2)));  // four columns of a row in one store, at any of them
+#pragma unroll
+  for (int t = 0; t < RM; ++t) {
+    const int64_t m = m0 + (wm * RM + t) * 32 + col;
+    const float scale = p.row && m < p.M ? p.row[m] : 1.0f;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int f = 0; f < RN / 2; ++f) {
+        const int64_t n = n0 + wn * (16 * RN) + 32 * f;
+        float v[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float g = acc[t][f][r], u = acc[t][f + RN / 2][r];
+          v[r] = activate(p.row ? g * scale : g, p.row ? u * scale : u, p.bf16);
+          top = umax(top, __float_as_uint(v[r]) & 0x7FFFFFFFu);
+        }
+        top = umax(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+        const uint32_t byte = p.q_bits == 4 ? block_byte<4>(top) : block_byte<8>(top);
+        const int64_t block = m * (p.N / kMxBlock) + n / kMxBlock;
+        const bool there = m < p.M && n < p.N;  // (inner is a multiple of 32)
+        if (there && kg == 0) p.out_scale[block] = static_cast<uint8_t>(byte);
+        if (p.q_bits == 4) {  // two bytes of every four are this lane's, the others the lane's 32 on
+          uint32_t mine[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float e[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
+            mine[i] = encode4(e, byte);
+          }
+          const uint32_t o0 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[0]), 32)), o1 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[1]), 32));
+          const uint32_t lo = kg ? o1 : mine[0], hi = kg ? mine[1] : o0;  // group 0 stores columns 0 .. 15, group 1 the others
+          const uint2 w = make_uint2((lo & 0xFFFFu) | hi << 16, lo >> 16 | (hi & 0xFFFF0000u));
+          if (there) *reinterpret_cast<mx_loose2 *>(static_cast<uint8_t *>(p.out) + block * 16 + 8 * kg) = mx_loose2{w.x, w.y};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float e[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
+            const uint2 w = encode8(e, byte);
+            uint8_t *to = static_cast<uint8_t *>(p.out) + block * 32 + 16 * i + 4 * kg;
+            if (there) {
+              *reinterpret_cast<mx_loose1 *>(to) = w.x;
+              *reinterpret_cast<mx_loose1 *>(to + 8) = w.y;
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < RN; ++f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
+          if (m >= p.M || n >= p.N) continue;
+          f32x4 v = {acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
+          if (p.splits > 1) {
+            *reinterpret_cast<f32x4 *>(p.partial + (split * p.M + m) * ((p.N + 3) & ~int64_t{3}) + n) = v;
+            continue;
+          }
+          uint32_t h[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (p.row) v[r] *= scale;
+            if (p.bias) v[r] += bias_of(p, n + r < p.N ? n + r : p.N - 1);
+            h[r] = to16(v[r], p.bf16);
+          }
+          uint16_t *to = static_cast<uint16_t *>(p.out) + m * p.N + n;
+          if (n + 3 < p.N) {
+            *reinterpret_cast<loose2 *>(to) = loose2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n + r < p.N) to[r] = static_cast<uint16_t>(h[r]);
+          }
+        }
+    }
+  }
+}
+
+// the sums of a split K in the order of the splits, then what the tiles do with a sum
+__global__ __launch_bounds__(256) void mx_join_kernel(MxArgs p) {
+  const int64_t pitch = (p.N + 3) & ~int64_t{3}, quads = pitch / 4, at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= p.M * quads) return;
+  const int64_t m = at / quads, n = at % quads * 4;
+  const float *from = p.partial + m * pitch + n;
+  f32x4 v = *reinterpret_cast<const f32x4 *>(from);
+  for (int i = 1; i < p.splits; ++i) v += *reinterpret_cast<const f32x4 *>(from + i * p.M * pitch);
+  const float row = p.row ? p.row[m] : 1.0f;
+  for (int r = 0; r < 4 && n + r < p.N; ++r) {
+    float y = p.row ? v[r] * row : v[r];
+    if (p.bias) y += bias_of(p, n + r);
+    static_cast<uint16_t *>(p.out)[m * p.N + n + r] = to16(y, p.bf16);
+  }
+}
+
+template <int XB, int TR, int FT, int W, int D, int STEPS, bool TAIL, bool GATED>
+int launch_ring(const MxArgs &p, hipStream_t st) {
+  using S = RingShape<XB, TR, FT, W, D, STEPS, TAIL>;
+  static_assert(S::kLds <= kLdsBytes, "");
+  auto kern = mx_ring_kernel<XB, TR, FT, W, D, STEPS, TAIL, GATED>;
+  if (int rc = prepare(kern, S::kLds)) return rc;
+  const int per_cu = kLdsBytes / S::kLds < 16 / W ? kLdsBytes / S::kLds : 16 / W;
+  const int64_t tiles = (p.N + p.width - 1) / p.width, slots = static_cast<int64_t>(num_cus()) * per_cu;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles < slots ? tiles : slots)), dim3(64 * W), S::kLds, st, p);
+  return check_launch();
+}
+
+// (2^31 threads per launch: rows beyond are further launches, which follow each other and share the memory of the parts' sums)
+template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL, bool GATED>
+int launch_tile(const MxArgs &p, hipStream_t st) {
+  using S = TileShape<XB, RM, RN, WM, WN, D, TAIL>;
+  static_assert(S::kLds <= kLdsBytes, "");
+  auto kern = mx_tile_kernel<XB, RM, RN, WM, WN, D, TAIL, GATED>;
+  if (int rc = prepare(kern, S::kLds)) return rc;
+  constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;
+  const int64_t across = (p.N + kCols - 1) / kCols * p.splits, most = INT32_MAX / (S::kW * 64) / across * S::kBM;
+  if (most == 0) return QUIK_ERR_RANGE;
+  for (int64_t m = 0; m < p.M; m += most) {
+    MxArgs q = p;
+    q.M = p.M - m < most ? p.M - m : most;
+    q.x = p.x + m * p.K * XB / 8;
+    q.xs = p.xs + m * (p.K / kMxBlock);
+    if (p.row) q.row = p.row + m;
+    q.out = static_cast<uint8_t *>(p.out) + (GATED ? m * p.N * p.q_bits / 8 : m * p.N * 2);
+    if (GATED) q.out_scale = p.out_scale + m * (p.N / kMxBlock);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((q.M + S::kBM - 1) / S::kBM * across)), dim3(64 * S::kW), S::kLds, st, q);
+    if (int rc = check_launch()) return rc;
+    if (p.splits > 1) {
+      hipLaunchKernelGGL(mx_join_kernel, dim3(static_cast<unsigned>((q.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, q);
+      if (int rc = check_launch()) return rc;
+    }
+  }
+  return QUIK_OK;
+}
+
+// Result columns per workgroup for up to 16 rows: the rounds that all CUs need with FT matrix tiles side by side, and the columns of a round
+// dealt to them evenly.
+int deal_columns(int64_t N, int ft) {
+  const int64_t cus = num_cus(), most = 16 * ft, rounds = ((N + most - 1) / most + cus - 1) / cus;
+  return static_cast<int>((N + rounds * cus - 1) / (rounds * cus));
+}
+
+template <int XB, bool TAIL>
+int few_rows(MxArgs p, hipStream_t st) {
+  const int ft = p.N > 16 * num_cus() ? 2 : 1;
+  p.width = deal_columns(p.N, ft);
+  if (p.M <= 8) {
+    if (ft == 2) return launch_ring<XB, 8, 2, 8, 2, 2, TAIL, false>(p, st);
+    return launch_ring<XB, 8, 1, 8, 2, 2, TAIL, false>(p, st);
+  }
+  if (ft == 2) return launch_ring<XB, 16, 2, 4, 2, 2, TAIL, false>(p, st);
+  return launch_ring<XB, 16, 1, 4, 2, 2, TAIL, false>(p, st);
+}
+template <int XB, bool TAIL>
+int few_rows_gated(MxArgs p, hipStream_t st) {
+  p.width = 32;
+  if (p.M <= 8) return launch_ring<XB, 8, 4, 4, 2, 2, TAIL, true>(p, st);
+  return launch_ring<XB, 16, 4, 4, 2, 2, TAIL, true>(p, st);
+}
+
+// Tiles of more than 16 rows, for 4- and for 8-bit rows: rows, columns, the time of a step of 128 columns on a CU in us, and what a tile takes
+// besides.
+struct TilePlan {
+  int rows, cols;
+  double step, round;
+};
+constexpr TilePlan kPlans[2][4] = {{{32, 128, 0.12, 0.5}, {64, 128, 0.14, 0.5}, {128, 128, 0.2, 1.0}, {256, 256, 0.55, 3.0}},
+                                   {{32, 128, 0.14, 0.5}, {64, 128, 0.2, 0.5}, {128, 128, 0.3, 1.0}, {128, 256, 0.5, 2.0}}};
+struct Choice {
+  int plan, splits;
+};
+Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
+  Choice best{1, 1};
+  double least = 1e30;
+  const int64_t cus = num_cus(), steps = (K + 127) / 128;
+  for (int i = 0; i < 4; ++i) {
+    const TilePlan &t = kPlans[x_bits == 8][i];
+    const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
+    for (int s = 1; s <= (may_split ? 16 : 1) && 8 * s <= steps + 7; ++s) {
+      const int64_t rounds = (tiles * s + cus - 1) / cus, deep = (steps + s - 1) / s;
+      const double us = static_cast<double>(rounds) * (static_cast<double>(deep) * t.step + t.round) + 3.0 +
+                        (s > 1 ? 3.0 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8e-6 / 5.0 : 0.0);
+      if (us < least) {
+        least = us;
+        best = Choice{i, s};
+      }
+    }
+  }
+  return best;
+}
+int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
+
+template <int XB, bool TAIL>
+int many_rows(const MxArgs &p, int64_t workspace_bytes, hipStream_t st) {
+  MxArgs q = p;
+  Choice c = choose(p.M, p.N, p.K, XB, true);
+  if (!p.partial || workspace_bytes < partial_bytes(p.M, p.N, c.splits)) c = choose(p.M, p.N, p.K, XB, false);
+  q.splits = c.splits;
+  if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, 6, TAIL, false>(q, st);
+  if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, 6, TAIL, false>(q, st);
+  if (c.plan == 2) return launch_tile<XB, 2, 2, 2, 2, 4, TAIL, false>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 4, 2, 2, 4, TAIL, false>(q, st);
+}
+template <int XB, bool TAIL>
+int many_rows_gated(const MxArgs &p, hipStream_t st) {
+  MxArgs q = p;
+  q.splits = 1;
+  const int plan = choose(p.M, 2 * p.N, p.K, XB, false).plan;
+  if (plan == 0) return launch_tile<XB, 1, 2, 1, 2, 6, TAIL, true>(q, st);
+  if (plan == 1) return launch_tile<XB, 1, 2, 2, 2, 6, TAIL, true>(q, st);
+  if (plan == 2) return launch_tile<XB, 2, 2, 2, 2, 4, TAIL, true>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 4, 2, 2, 4, TAIL, true>(q, st);
+}
+
+bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// what both products check
+int check_product(const void *x, int x_bits, const uint8_t *xs, const uint8_t *w, const uint8_t *ws, const float *row, int dtype, int64_t M, int64_t N,
+                  int64_t K, const void *out) {
+  if (x_bits != 4 && x_bits != 8) return QUIK_ERR_BITS;
+  if (dtype != QUIK_F16 && dtype != QUIK_BF16) return QUIK_ERR_DTYPE;
+  if (M < 0 || N < 0 || K <= 0) return QUIK_ERR_SHAPE;
+  if (K % kMxBlock) return QUIK_ERR_ALIGN;
+  if (M > INT32_MAX || N > INT32_MAX / 2 || K > 1 << 20) return QUIK_ERR_RANGE;  // (offsets of a tile's rows in 32 bits)
+  if (M == 0 || N == 0) return QUIK_OK;
+  if (!x || !xs || !w || !ws || !out) return QUIK_ERR_NULL;
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(row, 4)) return QUIK_ERR_ALIGN;
+  return QUIK_OK;
+}
+// exponent bytes by fours, or one by one where rows of them do not start at multiples of four or end inside a step
+bool by_fours(const uint8_t *xs, const uint8_t *ws, int64_t K) { return K % 128 == 0 && aligned(xs, 4) && aligned(ws, 4); }
+}  // namespace
+}  // namespace quik
+
+using namespace quik;
+
+extern "C" int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t N, int64_t K) {
+  if (M <= 16 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX / 2 || K > 1 << 20) return 0;
+  return partial_bytes(M, N, choose(M, N, K, x_bits, true).splits);
+}
+
+extern "C" int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row,
+                              const void *bias, int dtype, int64_t M, int64_t N, int64_t K, void *out, void *workspace, int64_t workspace_bytes,
+                              void *stream) {
+  if (int rc = check_product(x, x_bits, x_scale, w, w_scale, scale_row, dtype, M, N, K, out)) return rc;
+  if (M == 0 || N == 0) return QUIK_OK;
+  if (!aligned(bias, 2) || !aligned(out, 2) || !aligned(workspace, 16)) return QUIK_ERR_ALIGN;
+  const MxArgs p{static_cast<const uint8_t *>(x), x_scale, w, w_scale, scale_row, bias, out, nullptr, M, N, K, dtype == QUIK_BF16, 0, 0,
+                 static_cast<float *>(workspace), 1};
+  hipStream_t st = as_stream(stream);
+  const bool fours = by_fours(x_scale, w_scale, K);
+  if (M <= 16) {
+    if (x_bits == 4) return fours ? few_rows<4, false>(p, st) : few_rows<4, true>(p, st);
+    return fours ? few_rows<8, false>(p, st) : few_rows<8, true>(p, st);
+  }
+  if (x_bits == 4) return fours ? many_rows<4, false>(p, workspace_bytes, st) : many_rows<4, true>(p, workspace_bytes, st);
+  return fours ? many_rows<8, false>(p, workspace_bytes, st) : many_rows<8, true>(p, workspace_bytes, st);
+}
+
+extern "C" int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row,
+                                    int dtype, int64_t M, int64_t inner, int64_t K, int q_bits, void *q, uint8_t *q_scale, void *stream) {
+  if (q_bits != 4 && q_bits != 8) return QUIK_ERR_BITS;
+  if (int rc = check_product(x, x_bits, x_scale, w, w_scale, scale_row, dtype, M, inner, K, q)) return rc;
+  if (inner % kMxBlock) return QUIK_ERR_ALIGN;
+  if (inner * (K / kMxBlock) > INT32_MAX) return QUIK_ERR_RANGE;  // (up's exponent bytes lie as far behind the gates')
+  if (M == 0 || inner == 0) return QUIK_OK;
+  if (!q_scale) return QUIK_ERR_NULL;
+  const MxArgs p{static_cast<const uint8_t *>(x), x_scale, w, w_scale, scale_row, nullptr, q, q_scale, M, inner, K, dtype == QUIK_BF16, q_bits, 0, nullptr, 1};
+  hipStream_t st = as_stream(stream);
+  const bool fours = by_fours(x_scale, w_scale, K);
+  if (M <= 16) {
+    if (x_bits == 4) return fours ? few_rows_gated<4, false>(p, st) : few_rows_gated<4, true>(p, st);
+    return fours ? few_rows_gated<8, false>(p, st) : few_rows_gated<8, true>(p, st);
+  }
+  if (x_bits == 4) return fours ? many_rows_gated<4, false>(p, st) : many_rows_gated<4, true>(p, st);
+  return fours ? many_rows_gated<8, false>(p, st) : many_rows_gated<8, true>(p, st);
+}
