@@ -33,7 +33,14 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mx_bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 
+// a pointer that is the same for the wave, in scalar registers
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))), hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)));
+  return reinterpret_cast<const uint8_t *>(hi << 32 | lo);
+}
 // one byte per lane: it lands in the low byte of the four at LDS address m0 + 4 i (the others are not to be read)
 __device__ __forceinline__ void dma_load_u8(const void *sbase, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" : : "s"(lds_addr), "v"(voff), "s"(sbase) : "memory", "m0");
@@ -284,23 +291,31 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no copy is under way when the workgroup's LDS goes to another)
 }
 
-// More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on steps of 128 columns.  All operands
-// come to LDS by direct copies, D - 1 steps ahead, one barrier per step, in its middle: it says that the next step's operands are there, whose
-// first half a wave reads while it multiplies this one's second.  Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
-template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL>
+// More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on stages of 256 columns: whole lines
+// of 128 bytes of the weights' rows (half lines cost as many requests again: 8192 x 8192 -> 8192 on stages of 128 columns 434 us).  Codes come to LDS by
+// direct copies into two stages.  A stage is four products of 64 columns; while a wave multiplies it reads the next one's operands, and
+// behind the barrier in front of the last one (which says that every wave has read all of the stage, and that the next stage is there) the
+// stage after the next is copied over this one.
+// Exponent bytes lie apart in rows of 32 bytes for 1024 columns, also twice, and go through registers: rows of them may start at any byte.  Four bytes
+// of a row side by side, those of this lane's group, are one operand for a stage.  Bytes behind the end of K are 0 on both sides: whatever codes stand there,
+// a product of 2^-254 does not change a sum.
+// Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
+template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
-  static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kPx = XB, kPlanes = TAIL ? 4 : 1;
-  static constexpr int kCX = kBM * kPx / 64, kCW = kBN * 4 / 64, kCSX = (kBM + 63) / 64, kCSW = (kBN + 63) / 64;
-  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kMyS = (kCSX + kCSW + kW - 1) / kW;
-  static constexpr int kCopies = kMyX + kMyW + kMyS * kPlanes;
-  static constexpr int kAtW = kCX * 1024, kAtS = kAtW + kCW * 1024, kStage = kAtS + kPlanes * (kCSX + kCSW) * 256;
-  static constexpr int kLds = D * kStage;
-  static_assert(D >= 3 && kCopies * (D - 2) < 64 && kBM * kPx % 64 == 0, "");
+  static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kT = 64 * kW;
+  static constexpr int kPx = 2 * XB, kPw = 8;                          // 16-byte pieces of a row in a stage
+  static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;     // copies of 1 KB
+  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kCopies = kMyX + kMyW;
+  static constexpr int kAtW = kCX * 1024, kStage = kAtW + kCW * 1024, kScales = (kBM + kBN) * 32;
+  static constexpr int kAtS = 2 * kStage, kRings = kAtS + 2 * kScales;
+  static constexpr int kPitch = RN * 64 + 16, kOut = kW * 32 * kPitch;  // (a wave's 32 rows on their way out)
+  static constexpr int kLds = kRings > kOut ? kRings : kOut;
+  static constexpr int kRows = (kBM + kBN + kT - 1) / kT;              // rows of exponent bytes per thread
 };
 
-template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL, bool GATED>
+template <int XB, int RM, int RN, int WM, int WN, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
-  using S = TileShape<XB, RM, RN, WM, WN, D, TAIL>;
+  using S = TileShape<XB, RM, RN, WM, WN>;
   static_assert(!GATED || RN % 2 == 0, "");
   constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;  // result columns per tile
   extern __shared__ float red[];
@@ -308,7 +323,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   const uint32_t lds_at = lds_address(lds);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, kg = lane >> 5;
   const int wn = wave % WN, wm = wave / WN;
-  const int nb = static_cast<int>(p.K / kMxBlock), all_steps = (nb + 3) / 4;
+  const int nb = static_cast<int>(p.K / kMxBlock), all_stages = (nb + 7) / 8;
   // Workgroups go to the eight dies in turn: each die gets a run of tiles, in bands of four row tiles, column by column, so that those
   // that run on a die at a time share both their rows and their weights in its L2.  A tile whose K is split is `splits` workgroups, one after
   // the other.
@@ -319,72 +334,93 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   const int band = tile / (kBand * n_tiles), in_band = tile - band * kBand * n_tiles;
   const int high = m_tiles - band * kBand < kBand ? m_tiles - band * kBand : kBand;
   const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * S::kBM, n0 = static_cast<int64_t>(in_band / high) * kCols;
-  const int first = static_cast<int>(static_cast<int64_t>(all_steps) * split / p.splits);
-  const int steps = static_cast<int>(static_cast<int64_t>(all_steps) * (split + 1) / p.splits);
+  const int first = static_cast<int>(static_cast<int64_t>(all_stages) * split / p.splits);
+  const int stages = static_cast<int>(static_cast<int64_t>(all_stages) * (split + 1) / p.splits);
 
   const int64_t pitch_w = p.K / 2, pitch_x = p.K * XB / 8, left_m = p.M - 1 - m0, left_n = p.N - 1 - n0;
-  const uint8_t *xbase = p.x + m0 * pitch_x, *wbase = p.w + n0 * pitch_w, *xsbase = p.xs + m0 * nb, *wsbase = p.ws + n0 * nb;
+  const uint8_t *xbase = p.x + m0 * pitch_x, *wbase = p.w + n0 * pitch_w;
   // weight row R of the tile: wave R / (32 RN)'s, of its tiles the first half gates, the second up
   auto column_of = [](int R) { return GATED ? R / (32 * RN) * (16 * RN) + R % (16 * RN) : R; };
   auto is_up = [](int R) { return GATED && R % (32 * RN) >= 16 * RN; };
-  // this wave's copies: the row's offset and the piece of the step that this lane takes
-  uint32_t x_row[S::kMyX], w_row[S::kMyW], s_row[S::kMyS];
-  int x_piece[S::kMyX], w_piece[S::kMyW];
+  // this wave's copies: the row's offset and the piece of the stage that this lane takes
+  uint32_t x_off[S::kMyX], w_off[S::kMyW];
+  auto x_row = [&](int i) { return (wave + i * S::kW) % S::kCX * (64 / S::kPx) + lane / S::kPx; };
+  auto w_row = [&](int i) { return (wave + i * S::kW) % S::kCW * 8 + (lane >> 3); };
+  auto x_piece = [&](int i) { return (lane % S::kPx) ^ turn_of<S::kPx>(x_row(i)); };
+  auto w_piece = [&](int i) { return (lane & 7) ^ turn_of<8>(w_row(i)); };
 #pragma unroll
-  for (int i = 0; i < S::kMyX; ++i) {
-    const int row = (wave + i * S::kW) % S::kCX * (64 / S::kPx) + lane / S::kPx;
-    x_piece[i] = (lane % S::kPx) ^ turn_of<S::kPx>(row);
-    x_row[i] = static_cast<uint32_t>((row < left_m ? row : left_m) * pitch_x);
-  }
+  for (int i = 0; i < S::kMyX; ++i) x_off[i] = static_cast<uint32_t>((x_row(i) < left_m ? x_row(i) : left_m) * pitch_x + x_piece(i) * 16);
 #pragma unroll
   for (int i = 0; i < S::kMyW; ++i) {
-    const int row = (wave + i * S::kW) % S::kCW * 16 + (lane >> 2), n = column_of(row);
-    w_piece[i] = (lane & 3) ^ turn_of<4>(row);
-    w_row[i] = static_cast<uint32_t>((n < left_n ? n : left_n) * pitch_w);
+    const int n = column_of(w_row(i));
+    w_off[i] = static_cast<uint32_t>((n < left_n ? n : left_n) * pitch_w + w_piece(i) * 16);
   }
-#pragma unroll
-  for (int i = 0; i < S::kMyS; ++i) {
-    const int c = (wave + i * S::kW) % (S::kCSX + S::kCSW);
-    if (c < S::kCSX) {
-      const int row = c * 64 + lane;
-      s_row[i] = static_cast<uint32_t>((row < left_m ? row : left_m) * nb);
-    } else {
-      int row = (c - S::kCSX) * 64 + lane;
-      row = row < S::kBN ? row : S::kBN - 1;
-      const int n = column_of(row);
-      s_row[i] = static_cast<uint32_t>(((n < left_n ? n : left_n) + (is_up(row) ? p.N : 0)) * nb);
-    }
-  }
-  auto copy = [&](int step) {
-    const uint32_t to = lds_at + step % D * S::kStage;
-    const bool whole = !TAIL || (step + 1) * 4 <= nb;
-    const uint8_t *xfrom = xbase + step * (S::kPx * 16), *wfrom = wbase + step * 64;
-    const int last_x = nb * (XB / 4) - 1 - step * S::kPx, last_w = nb - 1 - step * 4;  // (pieces past the end of a row come from its last one)
+  // Copies `from` .. `until` - 1 of this wave's S::kCopies of a stage.
+  auto copy = [&](int stage, int from, int until) {
+    const uint32_t to = lds_at + ((stage - first) & 1) * S::kStage;
+    const bool whole = (stage + 1) * 8 <= nb;
+    const uint8_t *xfrom = xbase + stage * (S::kPx * 16), *wfrom = wbase + stage * 128;
+    const int last_x = nb * (XB / 4) - 1 - stage * S::kPx, last_w = nb - 1 - stage * 8;  // (pieces past the end of a row come from its last one)
 #pragma unroll
     for (int i = 0; i < S::kMyX; ++i) {
-      const int piece = whole || x_piece[i] < last_x ? x_piece[i] : last_x;
-      dma_load16(xfrom, x_row[i] + static_cast<uint32_t>(piece) * 16, to + (wave + i * S::kW) % S::kCX * 1024);
+      if (i < from || i >= until) continue;
+      const uint32_t past = whole || x_piece(i) < last_x ? 0 : static_cast<uint32_t>(x_piece(i) - last_x);
+      dma_load16(uniform(xfrom), x_off[i] - past * 16, to + (wave + i * S::kW) % S::kCX * 1024);
     }
 #pragma unroll
     for (int i = 0; i < S::kMyW; ++i) {
-      const int c = (wave + i * S::kW) % S::kCW, piece = whole || w_piece[i] < last_w ? w_piece[i] : last_w;
-      dma_load16(is_up(c * 16) ? wfrom + p.N * pitch_w : wfrom, w_row[i] + static_cast<uint32_t>(piece) * 16, to + S::kAtW + c * 1024);
+      if (S::kMyX + i < from || S::kMyX + i >= until) continue;
+      const int c = (wave + i * S::kW) % S::kCW;
+      const uint32_t past = whole || w_piece(i) < last_w ? 0 : static_cast<uint32_t>(w_piece(i) - last_w);
+      dma_load16(uniform(is_up(c * 8) ? wfrom + p.N * pitch_w : wfrom), w_off[i] - past * 16, to + S::kAtW + c * 1024);
     }
+  };
+  // exponent bytes: rows of x, then of w
+  const uint8_t *bytes_of[S::kRows];
 #pragma unroll
-    for (int i = 0; i < S::kMyS; ++i) {
-      const int c = (wave + i * S::kW) % (S::kCSX + S::kCSW);
-      const uint8_t *base = c < S::kCSX ? xsbase : wsbase;
-      if constexpr (TAIL) {
+  for (int i = 0; i < S::kRows; ++i) {
+    int row = threadIdx.x + i * S::kT;
+    row = row < S::kBM + S::kBN ? row : S::kBM + S::kBN - 1;
+    const int R = row - S::kBM, n = column_of(R < 0 ? 0 : R);
+    bytes_of[i] = row < S::kBM ? p.xs + (m0 + (row < left_m ? row : left_m)) * nb
+                               : p.ws + (n0 + (n < left_n ? n : left_n) + (is_up(R < 0 ? 0 : R) ? p.N : 0)) * nb;
+  }
+  uint32_t bytes[S::kRows][8];
+  auto load_bytes = [&](int batch) {  // (32 of a row from the batch's first on, 0 behind the end)
+    const int b0 = (first + 4 * batch) * 8;
 #pragma unroll
-        for (int plane = 0; plane < 4; ++plane) {
-          const int b = 4 * step + plane;
-          dma_load_u8(base + (b < nb ? b : nb - 1), s_row[i], to + S::kAtS + (plane * (S::kCSX + S::kCSW) + c) * 256);
+    for (int i = 0; i < S::kRows; ++i) {
+      if (b0 + 32 <= nb) {
+        const mx_bytes16 lo = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + b0), hi = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + b0 + 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          bytes[i][k] = lo[k];
+          bytes[i][4 + k] = hi[k];
         }
       } else {
-        dma_load_u32(base + 4 * step, s_row[i], to + S::kAtS + c * 256);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = b0 + 4 * k, from = at < nb - 4 ? at : nb - 4, shift = 8 * (at - from);
+          uint32_t w = 0;
+          if (nb >= 4) w = shift < 32 ? *reinterpret_cast<const mx_loose1 *>(bytes_of[i] + from) >> shift : 0;
+          else if (at == 0) w = bytes_of[i][0] | (nb > 1 ? bytes_of[i][1] << 8 : 0) | (nb > 2 ? bytes_of[i][2] << 16 : 0);
+          bytes[i][k] = w;
+        }
       }
     }
   };
+  // (eight bytes of a row, a stage's, at their number exclusive-or (row / 8) % 4: 32 rows' reads of one stage at different banks)
+  auto write_bytes = [&](int batch) {
+#pragma unroll
+    for (int i = 0; i < S::kRows; ++i) {
+      const int row = threadIdx.x + i * S::kT;
+      if (row >= S::kBM + S::kBN) continue;
+      uint8_t *to = lds + S::kAtS + (batch & 1) * S::kScales + row * 32;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint2 *>(to + (k ^ ((row >> 3) & 3)) * 8) = make_uint2(bytes[i][2 * k], bytes[i][2 * k + 1]);
+    }
+  };
+
   f32x16 acc[RM][RN];
 #pragma unroll
   for (int t = 0; t < RM; ++t)
@@ -393,73 +429,93 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[t][f][r] = 0.0f;
 
-  struct Half {
+  struct Quarter {  // operands of 64 columns
     Operand<XB> x[RM];
     Operand<4> w[RN];
-    uint32_t sx[RM], sw[RN];
   };
-  // half s of a step: 64 columns.  Bytes: of this lane's group, without planes also those of the second half, in byte 2
-  auto read = [&](int step, int s, Half &h) {
-    const uint8_t *from = lds + step % D * S::kStage;
-#pragma unroll
-    for (int t = 0; t < RM; ++t) {
-      const int row = (wm * RM + t) * 32 + col;
+  const int x_at = (wm * RM * 32 + col) * S::kPx * 16, w_at = S::kAtW + (wn * RN * 32 + col) * 128;
+  const int x_turn = turn_of<S::kPx>(col), w_turn = turn_of<8>(col);  // (of every tile's rows: they are 32 apart)
+  constexpr int kReads = RM + RN, kProducts = RM * RN, kSlots = kProducts < kReads ? kProducts : kReads;
+  auto read = [&](int stage, int s, Quarter &q, int n) {  // n: row tiles, then the weights'
+    const uint8_t *from = lds + ((stage - first) & 1) * S::kStage;
+    if (n < RM) {
 #pragma unroll
       for (int i = 0; i < XB / 4; ++i) {
         const int piece = XB == 4 ? 2 * s + kg : 4 * s + 2 * i + kg;
-        h.x[t].v[i] = *reinterpret_cast<const u32x4 *>(from + (row * S::kPx + (piece ^ turn_of<S::kPx>(row))) * 16);
-        if constexpr (TAIL) {
-          if (4 * step + 2 * s + (XB == 4 ? kg : i) >= nb) h.x[t].v[i] = u32x4{0, 0, 0, 0};
-        }
+        q.x[n].v[i] = *reinterpret_cast<const u32x4 *>(from + x_at + n * (32 * S::kPx * 16) + (piece ^ x_turn) * 16);
       }
-      const int plane = TAIL ? 2 * s + kg : 0;
-      if (TAIL || s == 0) h.sx[t] = *reinterpret_cast<const uint32_t *>(from + S::kAtS + (plane * (S::kCSX + S::kCSW) * 64 + row) * 4) >> (TAIL ? 0 : 8 * kg);
-    }
-#pragma unroll
-    for (int f = 0; f < RN; ++f) {
-      const int row = (wn * RN + f) * 32 + col;
-      h.w[f].v[0] = *reinterpret_cast<const u32x4 *>(from + S::kAtW + (row * 4 + ((2 * s + kg) ^ turn_of<4>(row))) * 16);
-      const int plane = TAIL ? 2 * s + kg : 0;
-      if (TAIL || s == 0)
-        h.sw[f] = *reinterpret_cast<const uint32_t *>(from + S::kAtS + ((plane * (S::kCSX + S::kCSW) + S::kCSX) * 64 + row) * 4) >> (TAIL ? 0 : 8 * kg);
+    } else {
+      q.w[n - RM].v[0] = *reinterpret_cast<const u32x4 *>(from + w_at + (n - RM) * 4096 + ((2 * s + kg) ^ w_turn) * 16);
     }
   };
-  auto multiply = [&](const Half &h, const uint32_t (&sx)[RM], const uint32_t (&sw)[RN], auto second) {
-    constexpr int kByte = decltype(second)::value && !TAIL ? 2 : 0;
-#pragma unroll
-    for (int f = 0; f < RN; ++f)
-#pragma unroll
-      for (int t = 0; t < RM; ++t) acc[t][f] = mfma32<XB, kByte>(h.w[f], h.x[t], acc[t][f], sw[f], sx[t]);
+  uint2 raw[kReads];  // a stage's exponent bytes of the rows of this lane's operands
+  const int byte_turn = (col >> 3) & 3;
+  auto read_bytes = [&](int stage, int n) {
+    const int i = stage - first, row = n < RM ? (wm * RM + n) * 32 + col : S::kBM + (wn * RN + n - RM) * 32 + col;
+    raw[n] = *reinterpret_cast<const uint2 *>(lds + S::kAtS + ((i >> 2) & 1) * S::kScales + row * 32 + ((i & 3) ^ byte_turn) * 8);
   };
+  const uint32_t pick = 0x06040200u + static_cast<uint32_t>(kg) * 0x01010101u;
+  // The products of a quarter, and between them what else the wave has to issue, in this order (left to itself the compiler puts all reads first).
+  auto multiply = [&](const Quarter &q, const uint32_t (&by)[kReads], auto quarter, auto between) {
 #pragma unroll
-  for (int d = 0; d < D - 1; ++d)
-    if (first + d < steps) copy(first + d);
-  if (first + D - 2 < steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 2)));
+    for (int i = 0; i < kProducts; ++i) {
+      const int f = i / RM, t = i % RM;
+      acc[t][f] = mfma32<XB, decltype(quarter)::value>(q.w[f], q.x[t], acc[t][f], by[RM + f], by[t]);
+      between(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto spread = [](int i, int n, int slots, auto call) {  // calls i of `slots` of n
+    if (i < slots) {
+#pragma unroll
+      for (int k = 0; k < 64; ++k)
+        if (k >= i * n / slots && k < (i + 1) * n / slots) call(k);
+    }
+  };
+  copy(first, 0, S::kCopies);
+  load_bytes(0);
+  write_bytes(0);
+  if (first + 1 < stages) copy(first + 1, 0, S::kCopies);
+  if (first + 1 < stages) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies));
   else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  asm volatile("s_barrier" ::: "memory");
-  Half a, b;
-  read(first, 0, a);
-  for (int step = first; step < steps; ++step) {
-    uint32_t sx[RM], sw[RN];
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier)
+  Quarter a, b;
 #pragma unroll
-    for (int t = 0; t < RM; ++t) sx[t] = a.sx[t];
-#pragma unroll
-    for (int f = 0; f < RN; ++f) sw[f] = a.sw[f];
-    read(step, 1, b);
-    multiply(a, sx, sw, std::false_type{});
-    if (step + 1 < steps) {
-      // the next step's operands: of this wave's copies, those of the steps behind it may be under way
-      if (step + D - 2 < steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 3)));
-      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier: every wave's reads of the step before are done)
-      if (step + D - 1 < steps) copy(step + D - 1);
-      read(step + 1, 0, a);
-    }
-    if constexpr (TAIL) multiply(b, b.sx, b.sw, std::true_type{});
-    else multiply(b, sx, sw, std::true_type{});
+  for (int n = 0; n < kReads; ++n) {
+    read_bytes(first, n);
+    read(first, 0, a, n);
   }
+  uint32_t by[kReads];
+  auto three_quarters = [&](int stage) {
+#pragma unroll
+    for (int n = 0; n < kReads; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
+    multiply(a, by, std::integral_constant<int, 0>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 1, b, n); }); });
+    multiply(b, by, std::integral_constant<int, 1>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 2, a, n); }); });
+    multiply(a, by, std::integral_constant<int, 2>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 3, b, n); }); });
+  };
+  for (int stage = first; stage + 1 < stages; ++stage) {
+    three_quarters(stage);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (this wave's copies of the next stage, requested three products ago)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier)
+    __builtin_amdgcn_sched_barrier(0);
+    const int at = stage - first;
+    if ((at & 3) == 1 && first + 4 * (at >> 2) + 4 < stages) write_bytes((at >> 2) + 1);
+    if ((at & 3) == 0 && stage + 4 < stages) load_bytes((at >> 2) + 1);
+    const bool more = stage + 2 < stages;
+    multiply(b, by, std::integral_constant<int, 3>{}, [&](int i) {
+      spread(i, kReads, kSlots, [&](int n) {
+        read_bytes(stage + 1, n);
+        read(stage + 1, 0, a, n);
+      });
+      if (more) copy(stage + 2, i * S::kCopies / kProducts, (i + 1) * S::kCopies / kProducts);
+    });
+  }
+  three_quarters(stages - 1);
+  multiply(b, by, std::integral_constant<int, 3>{}, [](int) {});
   // value r of a lane: column 8 (r / 4) + 4 kg + r % 4 of token col
-  typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(2)));  // four columns of a row in one store, at any of them
+  if constexpr (!GATED) {
+    if (p.splits == 1) __syncthreads();  // (the last stage is read: results go out through its place)
+  }
 #pragma unroll
   for (int t = 0; t < RM; ++t) {
     const int64_t m = m0 + (wm * RM + t) * 32 + col;
@@ -509,34 +565,53 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
           }
         }
       }
-    } else {
+    } else if (p.splits > 1) {
 #pragma unroll
       for (int f = 0; f < RN; ++f)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
-          if (m >= p.M || n >= p.N) continue;
-          f32x4 v = {acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
-          if (p.splits > 1) {
-            *reinterpret_cast<f32x4 *>(p.partial + (split * p.M + m) * ((p.N + 3) & ~int64_t{3}) + n) = v;
-            continue;
-          }
+          if (m < p.M && n < p.N)
+            *reinterpret_cast<f32x4 *>(p.partial + (split * p.M + m) * ((p.N + 3) & ~int64_t{3}) + n) =
+                f32x4{acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
+        }
+    } else {
+      // 32 rows of the wave's columns through LDS, so that a store takes whole pieces of rows (four columns per lane as they lie in the registers: 29 us of
+      // 256 tiles of 256 x 256)
+      uint8_t *out = lds + wave * (32 * S::kPitch);
+#pragma unroll
+      for (int f = 0; f < RN; ++f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
           uint32_t h[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if (p.row) v[r] *= scale;
-            if (p.bias) v[r] += bias_of(p, n + r < p.N ? n + r : p.N - 1);
-            h[r] = to16(v[r], p.bf16);
+            float v = acc[t][f][4 * j + r];
+            if (p.row) v *= scale;
+            if (p.bias) v += bias_of(p, n + r < p.N ? n + r : p.N - 1);
+            h[r] = to16(v, p.bf16);
           }
-          uint16_t *to = static_cast<uint16_t *>(p.out) + m * p.N + n;
-          if (n + 3 < p.N) {
-            *reinterpret_cast<loose2 *>(to) = loose2{h[0] | h[1] << 16, h[2] | h[3] << 16};
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n + r < p.N) to[r] = static_cast<uint16_t>(h[r]);
-          }
+          *reinterpret_cast<uint2 *>(out + col * S::kPitch + (f * 32 + 8 * j + 4 * kg) * 2) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
         }
+      asm volatile("" ::: "memory");  // (one wave's LDS accesses follow each other)
+#pragma unroll
+      for (int i = 0; i < 2 * RN; ++i) {
+        const int piece = i * 64 + lane, row = piece / (4 * RN), at = piece % (4 * RN) * 8;
+        const int64_t mm = m0 + (wm * RM + t) * 32 + row, n = n0 + wn * (RN * 32) + at;
+        const uint4 w = *reinterpret_cast<const uint4 *>(out + row * S::kPitch + at * 2);
+        if (mm >= p.M || n >= p.N) continue;
+        uint16_t *to = static_cast<uint16_t *>(p.out) + mm * p.N + n;
+        if (n + 7 < p.N) {
+          *reinterpret_cast<mx_loose4 *>(to) = mx_loose4{w.x, w.y, w.z, w.w};
+        } else {
+          const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int r = 0; r < 7; ++r)
+            if (n + r < p.N) to[r] = static_cast<uint16_t>(h[r / 2] >> (16 * (r & 1)));
+        }
+      }
+      asm volatile("" ::: "memory");
     }
   }
 }
@@ -570,11 +645,11 @@ int launch_ring(const MxArgs &p, hipStream_t st) {
 }
 
 // (2^31 threads per launch: rows beyond are further launches, which follow each other and share the memory of the parts' sums)
-template <int XB, int RM, int RN, int WM, int WN, int D, bool TAIL, bool GATED>
+template <int XB, int RM, int RN, int WM, int WN, bool GATED>
 int launch_tile(const MxArgs &p, hipStream_t st) {
-  using S = TileShape<XB, RM, RN, WM, WN, D, TAIL>;
+  using S = TileShape<XB, RM, RN, WM, WN>;
   static_assert(S::kLds <= kLdsBytes, "");
-  auto kern = mx_tile_kernel<XB, RM, RN, WM, WN, D, TAIL, GATED>;
+  auto kern = mx_tile_kernel<XB, RM, RN, WM, WN, GATED>;
   if (int rc = prepare(kern, S::kLds)) return rc;
   constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;
   const int64_t across = (p.N + kCols - 1) / kCols * p.splits, most = INT32_MAX / (S::kW * 64) / across * S::kBM;
@@ -654,26 +729,26 @@ Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
 }
 int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
 
-template <int XB, bool TAIL>
+template <int XB>
 int many_rows(const MxArgs &p, int64_t workspace_bytes, hipStream_t st) {
   MxArgs q = p;
   Choice c = choose(p.M, p.N, p.K, XB, true);
   if (!p.partial || workspace_bytes < partial_bytes(p.M, p.N, c.splits)) c = choose(p.M, p.N, p.K, XB, false);
   q.splits = c.splits;
-  if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, 6, TAIL, false>(q, st);
-  if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, 6, TAIL, false>(q, st);
-  if (c.plan == 2) return launch_tile<XB, 2, 2, 2, 2, 4, TAIL, false>(q, st);
-  return launch_tile<XB, (XB == 8 ? 2 : 4), 4, 2, 2, 4, TAIL, false>(q, st);
+  if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, false>(q, st);
+  if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, false>(q, st);
+  if (c.plan == 2) return launch_tile<XB, 2, 2, 2, 2, false>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, false>(q, st);
 }
-template <int XB, bool TAIL>
+template <int XB>
 int many_rows_gated(const MxArgs &p, hipStream_t st) {
   MxArgs q = p;
   q.splits = 1;
   const int plan = choose(p.M, 2 * p.N, p.K, XB, false).plan;
-  if (plan == 0) return launch_tile<XB, 1, 2, 1, 2, 6, TAIL, true>(q, st);
-  if (plan == 1) return launch_tile<XB, 1, 2, 2, 2, 6, TAIL, true>(q, st);
-  if (plan == 2) return launch_tile<XB, 2, 2, 2, 2, 4, TAIL, true>(q, st);
-  return launch_tile<XB, (XB == 8 ? 2 : 4), 4, 2, 2, 4, TAIL, true>(q, st);
+  if (plan == 0) return launch_tile<XB, 1, 2, 1, 2, true>(q, st);
+  if (plan == 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
+  if (plan == 2) return launch_tile<XB, 2, 2, 2, 2, true>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, true>(q, st);
 }
 
 bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -717,8 +792,7 @@ extern "C" int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale,
     if (x_bits == 4) return fours ? few_rows<4, false>(p, st) : few_rows<4, true>(p, st);
     return fours ? few_rows<8, false>(p, st) : few_rows<8, true>(p, st);
   }
-  if (x_bits == 4) return fours ? many_rows<4, false>(p, workspace_bytes, st) : many_rows<4, true>(p, workspace_bytes, st);
-  return fours ? many_rows<8, false>(p, workspace_bytes, st) : many_rows<8, true>(p, workspace_bytes, st);
+  return x_bits == 4 ? many_rows<4>(p, workspace_bytes, st) : many_rows<8>(p, workspace_bytes, st);
 }
 
 extern "C" int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row,
@@ -736,6 +810,5 @@ extern "C" int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_
     if (x_bits == 4) return fours ? few_rows_gated<4, false>(p, st) : few_rows_gated<4, true>(p, st);
     return fours ? few_rows_gated<8, false>(p, st) : few_rows_gated<8, true>(p, st);
   }
-  if (x_bits == 4) return fours ? many_rows_gated<4, false>(p, st) : many_rows_gated<4, true>(p, st);
-  return fours ? many_rows_gated<8, false>(p, st) : many_rows_gated<8, true>(p, st);
+  return x_bits == 4 ? many_rows_gated<4>(p, st) : many_rows_gated<8>(p, st);
 }
