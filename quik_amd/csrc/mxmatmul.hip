@@ -82,9 +82,10 @@ __device__ __forceinline__ float from16(uint16_t v, bool bf16) { return bf16 ? t
 __device__ __forceinline__ uint16_t to16(float v, bool bf16) { return bf16 ? from_f32<true>(v) : from_f32<false>(v); }
 __device__ __forceinline__ float bias_of(const MxArgs &p, int64_t n) { return from16(static_cast<const uint16_t *>(p.bias)[n], p.bf16); }
 // the activation of a gated block, of products rounded to the 16-bit type
-__device__ __forceinline__ float activate(float gate, float up, bool bf16) {
-  gate = from16(to16(gate, bf16), bf16);
-  up = from16(to16(up, bf16), bf16);
+template <bool BF16>
+__device__ __forceinline__ float activate(float gate, float up) {
+  gate = round_storage<BF16>(gate);
+  up = round_storage<BF16>(up);
   return __float_as_uint(gate) > kFarBits ? gated_far(gate, up) : gated(gate, up);
 }
 
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
     if constexpr (GATED) {
       for (int e = threadIdx.x; e < p.M * 32; e += 64 * W) {
         const int m = e >> 5, n = e & 31;  // (inner is a multiple of 32: the block is whole)
-        const float v = activate(sum(m, n), sum(m, 32 + n), p.bf16);
+        const float g = sum(m, n), u = sum(m, 32 + n), v = p.bf16 ? activate<true>(g, u) : activate<false>(g, u);
         uint32_t top = __float_as_uint(v) & 0x7FFFFFFFu;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) top = umax(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
@@ -292,22 +293,24 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 }
 
 // More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on stages of 256 columns: whole lines
-// of 128 bytes of the weights' rows (half lines cost as many requests again: 8192 x 8192 -> 8192 on stages of 128 columns 434 us).  Codes come to LDS by
-// direct copies into two stages.  A stage is four products of 64 columns; while a wave multiplies it reads the next one's operands, and
-// behind the barrier in front of the last one (which says that every wave has read all of the stage, and that the next stage is there) the
-// stage after the next is copied over this one.
-// Exponent bytes lie apart in rows of 32 bytes for 1024 columns, also twice, and go through registers: rows of them may start at any byte.  Four bytes
-// of a row side by side, those of this lane's group, are one operand for a stage.  Bytes behind the end of K are 0 on both sides: whatever codes stand there,
-// a product of 2^-254 does not change a sum.
+// of 128 bytes of the weights' rows (half lines cost as many requests again: 8192 x 8192 -> 8192 on stages of 128 columns 434 us).  LDS holds two
+// stages; a third is on its way to registers.  (Direct copies to LDS hold the wave that issues them until the CU has taken the ones before, some
+// 36 cycles per kilobyte, and its products with it; and they can start only when their place is free: 300 us.)
+// A stage is four products of 64 columns.  An operand is read again for the next one behind its last product of this one.  In the middle of the fourth
+// there is a barrier: every wave has read all of the stage, and the next one is there; behind it the stage after the next is written over
+// this one, and the one behind that is requested.
+// Exponent bytes lie apart, eight of a row per stage in a ring of four stages, and come two stages at a time, also through registers: rows of them may start
+// at any byte.  Four bytes of a stage, those of this lane's group, are one operand for it.  Bytes behind the end of K are 0 on both sides:
+// whatever codes stand there, a product of 2^-254 does not change a sum.
 // Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
 template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
   static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kT = 64 * kW;
-  static constexpr int kPx = 2 * XB, kPw = 8;                          // 16-byte pieces of a row in a stage
-  static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;     // copies of 1 KB
-  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kCopies = kMyX + kMyW;
-  static constexpr int kAtW = kCX * 1024, kStage = kAtW + kCW * 1024, kScales = (kBM + kBN) * 32;
-  static constexpr int kAtS = 2 * kStage, kRings = kAtS + 2 * kScales;
+  static constexpr int kPx = 2 * XB, kPw = 8;                         // 16-byte pieces of a row in a stage
+  static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;    // loads of 1 KB
+  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kLoads = kMyX + kMyW;
+  static constexpr int kAtW = kCX * 1024, kStage = kAtW + kCW * 1024;
+  static constexpr int kAtS = 2 * kStage, kRings = kAtS + (kBM + kBN) * 32;
   static constexpr int kPitch = RN * 64 + 16, kOut = kW * 32 * kPitch;  // (a wave's 32 rows on their way out)
   static constexpr int kLds = kRings > kOut ? kRings : kOut;
   static constexpr int kRows = (kBM + kBN + kT - 1) / kT;              // rows of exponent bytes per thread
@@ -342,82 +345,73 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   // weight row R of the tile: wave R / (32 RN)'s, of its tiles the first half gates, the second up
   auto column_of = [](int R) { return GATED ? R / (32 * RN) * (16 * RN) + R % (16 * RN) : R; };
   auto is_up = [](int R) { return GATED && R % (32 * RN) >= 16 * RN; };
-  // this wave's copies: the row's offset and the piece of the stage that this lane takes
+  // this wave's loads: the row's offset and the piece of the stage that this lane takes, and where it goes
   uint32_t x_off[S::kMyX], w_off[S::kMyW];
-  auto x_row = [&](int i) { return (wave + i * S::kW) % S::kCX * (64 / S::kPx) + lane / S::kPx; };
-  auto w_row = [&](int i) { return (wave + i * S::kW) % S::kCW * 8 + (lane >> 3); };
-  auto x_piece = [&](int i) { return (lane % S::kPx) ^ turn_of<S::kPx>(x_row(i)); };
-  auto w_piece = [&](int i) { return (lane & 7) ^ turn_of<8>(w_row(i)); };
+  auto nth = [&](int i, int all) { return all % S::kW == 0 ? wave + i * S::kW : (wave + i * S::kW) % all; };
+  auto x_row = [&](int i) { return nth(i, S::kCX) * (64 / S::kPx) + lane / S::kPx; };
+  auto w_row = [&](int i) { return nth(i, S::kCW) * 8 + (lane >> 3); };
+  const int x_piece = lane % S::kPx, w_piece = lane & 7;
 #pragma unroll
-  for (int i = 0; i < S::kMyX; ++i) x_off[i] = static_cast<uint32_t>((x_row(i) < left_m ? x_row(i) : left_m) * pitch_x + x_piece(i) * 16);
+  for (int i = 0; i < S::kMyX; ++i) x_off[i] = static_cast<uint32_t>((x_row(i) < left_m ? x_row(i) : left_m) * pitch_x);
 #pragma unroll
   for (int i = 0; i < S::kMyW; ++i) {
     const int n = column_of(w_row(i));
-    w_off[i] = static_cast<uint32_t>((n < left_n ? n : left_n) * pitch_w + w_piece(i) * 16);
+    w_off[i] = static_cast<uint32_t>((n < left_n ? n : left_n) * pitch_w);
   }
-  // Copies `from` .. `until` - 1 of this wave's S::kCopies of a stage.
-  auto copy = [&](int stage, int from, int until) {
-    const uint32_t to = lds_at + ((stage - first) & 1) * S::kStage;
-    const bool whole = (stage + 1) * 8 <= nb;
-    const uint8_t *xfrom = xbase + stage * (S::kPx * 16), *wfrom = wbase + stage * 128;
-    const int last_x = nb * (XB / 4) - 1 - stage * S::kPx, last_w = nb - 1 - stage * 8;  // (pieces past the end of a row come from its last one)
-#pragma unroll
-    for (int i = 0; i < S::kMyX; ++i) {
-      if (i < from || i >= until) continue;
-      const uint32_t past = whole || x_piece(i) < last_x ? 0 : static_cast<uint32_t>(x_piece(i) - last_x);
-      dma_load16(uniform(xfrom), x_off[i] - past * 16, to + (wave + i * S::kW) % S::kCX * 1024);
-    }
-#pragma unroll
-    for (int i = 0; i < S::kMyW; ++i) {
-      if (S::kMyX + i < from || S::kMyX + i >= until) continue;
-      const int c = (wave + i * S::kW) % S::kCW;
-      const uint32_t past = whole || w_piece(i) < last_w ? 0 : static_cast<uint32_t>(w_piece(i) - last_w);
-      dma_load16(uniform(is_up(c * 8) ? wfrom + p.N * pitch_w : wfrom), w_off[i] - past * 16, to + S::kAtW + c * 1024);
+  // (a load's rows are a multiple of 16 behind the first one's: the same turn)
+  static_assert(S::kW * (64 / S::kPx) % 16 == 0, "");
+  const int x_to = (x_row(0) * S::kPx + (x_piece ^ turn_of<S::kPx>(x_row(0)))) * 16, w_to = S::kAtW + (w_row(0) * 8 + (w_piece ^ turn_of<8>(w_row(0)))) * 16;
+  u32x4 staged[S::kLoads];
+  auto load = [&](int stage, int i) {  // (pieces past the end of a row come from its last one)
+    if (i < S::kMyX) {
+      const int last = nb * (XB / 4) - 1 - stage * S::kPx, piece = x_piece < last ? x_piece : last;
+      staged[i] = *reinterpret_cast<const u32x4 *>(xbase + stage * (S::kPx * 16) + (x_off[i] + static_cast<uint32_t>(piece) * 16));
+    } else {
+      const int last = nb - 1 - stage * 8, piece = w_piece < last ? w_piece : last;
+      const uint8_t *from = is_up(nth(i - S::kMyX, S::kCW) * 8) ? wbase + p.N * pitch_w : wbase;
+      staged[i] = *reinterpret_cast<const u32x4 *>(from + stage * 128 + (w_off[i - S::kMyX] + static_cast<uint32_t>(piece) * 16));
     }
   };
-  // exponent bytes: rows of x, then of w
+  auto write = [&](int stage, int i) {
+    uint8_t *to = lds + ((stage - first) & 1) * S::kStage;
+    if (i < S::kMyX) *reinterpret_cast<u32x4 *>(to + x_to + (nth(i, S::kCX) - wave) * 1024) = staged[i];
+    else *reinterpret_cast<u32x4 *>(to + w_to + (nth(i - S::kMyX, S::kCW) - wave) * 1024) = staged[i];
+  };
+  // exponent bytes: rows of x, then of w (a thread without a row of its own takes the last one too)
   const uint8_t *bytes_of[S::kRows];
+  auto byte_row = [&](int i) {
+    const int row = threadIdx.x + i * S::kT;
+    return row < S::kBM + S::kBN ? row : S::kBM + S::kBN - 1;
+  };
 #pragma unroll
   for (int i = 0; i < S::kRows; ++i) {
-    int row = threadIdx.x + i * S::kT;
-    row = row < S::kBM + S::kBN ? row : S::kBM + S::kBN - 1;
-    const int R = row - S::kBM, n = column_of(R < 0 ? 0 : R);
-    bytes_of[i] = row < S::kBM ? p.xs + (m0 + (row < left_m ? row : left_m)) * nb
-                               : p.ws + (n0 + (n < left_n ? n : left_n) + (is_up(R < 0 ? 0 : R) ? p.N : 0)) * nb;
+    const int row = byte_row(i), R = row < S::kBM ? 0 : row - S::kBM, n = column_of(R);
+    bytes_of[i] = row < S::kBM ? p.xs + (m0 + (row < left_m ? row : left_m)) * nb : p.ws + (n0 + (n < left_n ? n : left_n) + (is_up(R) ? p.N : 0)) * nb;
   }
-  uint32_t bytes[S::kRows][8];
-  auto load_bytes = [&](int batch) {  // (32 of a row from the batch's first on, 0 behind the end)
-    const int b0 = (first + 4 * batch) * 8;
+  u32x4 bytes[S::kRows];  // of two stages
+  // A pair of stages' bytes; of the last pair the row's last sixteen, of which the first `less` belong to stages before.
+  auto load_bytes = [&](int pair) {
+    const int at = (first + 2 * pair) * 8, from = at < nb - 16 ? at : nb - 16;
 #pragma unroll
-    for (int i = 0; i < S::kRows; ++i) {
-      if (b0 + 32 <= nb) {
-        const mx_bytes16 lo = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + b0), hi = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + b0 + 16);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          bytes[i][k] = lo[k];
-          bytes[i][4 + k] = hi[k];
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int at = b0 + 4 * k, from = at < nb - 4 ? at : nb - 4, shift = 8 * (at - from);
-          uint32_t w = 0;
-          if (nb >= 4) w = shift < 32 ? *reinterpret_cast<const mx_loose1 *>(bytes_of[i] + from) >> shift : 0;
-          else if (at == 0) w = bytes_of[i][0] | (nb > 1 ? bytes_of[i][1] << 8 : 0) | (nb > 2 ? bytes_of[i][2] << 16 : 0);
-          bytes[i][k] = w;
-        }
-      }
-    }
+    for (int i = 0; i < S::kRows; ++i) bytes[i] = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + (nb < 16 ? 0 : from));
+    return at - from;
   };
   // (eight bytes of a row, a stage's, at their number exclusive-or (row / 8) % 4: 32 rows' reads of one stage at different banks)
-  auto write_bytes = [&](int batch) {
+  auto write_bytes = [&](int pair, int less) {
 #pragma unroll
     for (int i = 0; i < S::kRows; ++i) {
-      const int row = threadIdx.x + i * S::kT;
-      if (row >= S::kBM + S::kBN) continue;
-      uint8_t *to = lds + S::kAtS + (batch & 1) * S::kScales + row * 32;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint2 *>(to + (k ^ ((row >> 3) & 3)) * 8) = make_uint2(bytes[i][2 * k], bytes[i][2 * k + 1]);
+      // (sixteen bytes less the first `less`, zeros behind; bit by bit: no branch)
+      const uint32_t by4 = less & 4 ? ~0u : 0, by8 = less & 8 ? ~0u : 0, some = less >= 16 ? 0 : ~0u;
+      auto choose_of = [](uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); };
+      u32x4 v = bytes[i];
+      v = u32x4{choose_of(by4, v[1], v[0]), choose_of(by4, v[2], v[1]), choose_of(by4, v[3], v[2]), v[3] & ~by4};
+      v = u32x4{choose_of(by8, v[2], v[0]), choose_of(by8, v[3], v[1]), v[2] & ~by8, v[3] & ~by8};
+      v = u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], less & 3) & some, __builtin_amdgcn_alignbyte(v[2], v[1], less & 3) & some,
+                __builtin_amdgcn_alignbyte(v[3], v[2], less & 3) & some, __builtin_amdgcn_alignbyte(0, v[3], less & 3) & some};
+      const int row = byte_row(i);
+      uint8_t *to = lds + S::kAtS + row * 32;
+      *reinterpret_cast<uint2 *>(to + ((2 * pair & 3) ^ ((row >> 3) & 3)) * 8) = make_uint2(v[0], v[1]);
+      *reinterpret_cast<uint2 *>(to + (((2 * pair + 1) & 3) ^ ((row >> 3) & 3)) * 8) = make_uint2(v[2], v[3]);
     }
   };
 
@@ -429,191 +423,266 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[t][f][r] = 0.0f;
 
-  struct Quarter {  // operands of 64 columns
-    Operand<XB> x[RM];
-    Operand<4> w[RN];
-  };
+  // operands of 64 columns
+  Operand<XB> x[RM];
+  Operand<4> w[RN];
+  uint2 raw[RM + RN];  // the next stage's exponent bytes of their rows
+  uint32_t by[RM + RN];
   const int x_at = (wm * RM * 32 + col) * S::kPx * 16, w_at = S::kAtW + (wn * RN * 32 + col) * 128;
   const int x_turn = turn_of<S::kPx>(col), w_turn = turn_of<8>(col);  // (of every tile's rows: they are 32 apart)
-  constexpr int kReads = RM + RN, kProducts = RM * RN, kSlots = kProducts < kReads ? kProducts : kReads;
-  auto read = [&](int stage, int s, Quarter &q, int n) {  // n: row tiles, then the weights'
-    const uint8_t *from = lds + ((stage - first) & 1) * S::kStage;
-    if (n < RM) {
+  auto read_x = [&](const uint8_t *from, int s, int t) {
 #pragma unroll
-      for (int i = 0; i < XB / 4; ++i) {
-        const int piece = XB == 4 ? 2 * s + kg : 4 * s + 2 * i + kg;
-        q.x[n].v[i] = *reinterpret_cast<const u32x4 *>(from + x_at + n * (32 * S::kPx * 16) + (piece ^ x_turn) * 16);
-      }
-    } else {
-      q.w[n - RM].v[0] = *reinterpret_cast<const u32x4 *>(from + w_at + (n - RM) * 4096 + ((2 * s + kg) ^ w_turn) * 16);
+    for (int i = 0; i < XB / 4; ++i) {
+      const int piece = XB == 4 ? 2 * s + kg : 4 * s + 2 * i + kg;
+      x[t].v[i] = *reinterpret_cast<const u32x4 *>(from + x_at + t * (32 * S::kPx * 16) + (piece ^ x_turn) * 16);
     }
   };
-  uint2 raw[kReads];  // a stage's exponent bytes of the rows of this lane's operands
-  const int byte_turn = (col >> 3) & 3;
+  auto read_w = [&](const uint8_t *from, int s, int f) {
+    w[f].v[0] = *reinterpret_cast<const u32x4 *>(from + w_at + f * 4096 + ((2 * s + kg) ^ w_turn) * 16);
+  };
+  const int bytes_at = S::kAtS + (wm * RM * 32 + col) * 32, bytes_at_w = S::kAtS + (S::kBM + wn * RN * 32 + col) * 32;
   auto read_bytes = [&](int stage, int n) {
-    const int i = stage - first, row = n < RM ? (wm * RM + n) * 32 + col : S::kBM + (wn * RN + n - RM) * 32 + col;
-    raw[n] = *reinterpret_cast<const uint2 *>(lds + S::kAtS + ((i >> 2) & 1) * S::kScales + row * 32 + ((i & 3) ^ byte_turn) * 8);
+    const int to = (((stage - first) & 3) ^ ((col >> 3) & 3)) * 8;
+    raw[n] = *reinterpret_cast<const uint2 *>(lds + (n < RM ? bytes_at + n * 1024 : bytes_at_w + (n - RM) * 1024) + to);
   };
   const uint32_t pick = 0x06040200u + static_cast<uint32_t>(kg) * 0x01010101u;
-  // The products of a quarter, and between them what else the wave has to issue, in this order (left to itself the compiler puts all reads first).
-  auto multiply = [&](const Quarter &q, const uint32_t (&by)[kReads], auto quarter, auto between) {
-#pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-      const int f = i / RM, t = i % RM;
-      acc[t][f] = mfma32<XB, decltype(quarter)::value>(q.w[f], q.x[t], acc[t][f], by[RM + f], by[t]);
-      between(i);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  // Product i of quarter s, then the reads for the next quarter (of `next`) that wait for it, in this order (left to itself the compiler puts all reads
+  // first, behind them all products).
+  auto product = [&](auto quarter, int i, const uint8_t *next, bool reads) {
+    constexpr int s = decltype(quarter)::value;
+    const int f = i / RM, t = i % RM;
+    acc[t][f] = mfma32<XB, s>(w[f], x[t], acc[t][f], by[RM + f], by[t]);
+    if (reads && t == RM - 1) read_w(next, (s + 1) % 4, f);
+    if (reads && f == RN - 1) read_x(next, (s + 1) % 4, t);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto spread = [](int i, int n, int slots, auto call) {  // calls i of `slots` of n
-    if (i < slots) {
+  auto quarter = [&](auto which, const uint8_t *next) {
 #pragma unroll
-      for (int k = 0; k < 64; ++k)
-        if (k >= i * n / slots && k < (i + 1) * n / slots) call(k);
-    }
+    for (int i = 0; i < RM * RN; ++i) product(which, i, next, true);
   };
-  copy(first, 0, S::kCopies);
-  load_bytes(0);
-  write_bytes(0);
-  if (first + 1 < stages) copy(first + 1, 0, S::kCopies);
-  if (first + 1 < stages) __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies));
-  else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier)
-  Quarter a, b;
+  constexpr std::integral_constant<int, 0> k0{};
+  constexpr std::integral_constant<int, 1> k1{};
+  constexpr std::integral_constant<int, 2> k2{};
+  constexpr std::integral_constant<int, 3> k3{};
+  // (past the last stage: that one once more, not used)
+  auto there = [&](int stage) { return stage < stages ? stage : stages - 1; };
+  int less = 0;
+  if (nb >= 16) {
+    less = load_bytes(0);
+  } else {  // rows of fewer bytes than a load: one pair, byte by byte; the loop's loads, whose bytes are not used, are of the first rows' (M > 16)
 #pragma unroll
-  for (int n = 0; n < kReads; ++n) {
-    read_bytes(first, n);
-    read(first, 0, a, n);
+    for (int i = 0; i < S::kRows; ++i) {
+      uint64_t v[2] = {0, 0};
+#pragma unroll 1
+      for (int e = 0; e < nb; ++e) {
+        const uint64_t byte = bytes_of[i][e];
+        if (e < 8) v[0] |= byte << (8 * e);
+        else v[1] |= byte << (8 * (e - 8));
+      }
+      bytes[i] = u32x4{static_cast<uint32_t>(v[0]), static_cast<uint32_t>(v[0] >> 32), static_cast<uint32_t>(v[1]), static_cast<uint32_t>(v[1] >> 32)};
+      bytes_of[i] = p.xs;
+    }
   }
-  uint32_t by[kReads];
-  auto three_quarters = [&](int stage) {
 #pragma unroll
-    for (int n = 0; n < kReads; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
-    multiply(a, by, std::integral_constant<int, 0>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 1, b, n); }); });
-    multiply(b, by, std::integral_constant<int, 1>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 2, a, n); }); });
-    multiply(a, by, std::integral_constant<int, 2>{}, [&](int i) { spread(i, kReads, kSlots, [&](int n) { read(stage, 3, b, n); }); });
-  };
-  for (int stage = first; stage + 1 < stages; ++stage) {
-    three_quarters(stage);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (this wave's copies of the next stage, requested three products ago)
+  for (int d = 0; d < 3; ++d) {
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) load(there(first + d), i);
+    if (d == 0) {
+      write_bytes(0, nb < 16 ? first * 8 : less);
+      less = load_bytes(1);
+    }
+    if (d < 2) {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) write(first + d, i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < RM + RN; ++n) read_bytes(first, n);
+#pragma unroll
+  for (int f = 0; f < RN; ++f) read_w(lds, 0, f);
+#pragma unroll
+  for (int t = 0; t < RM; ++t) read_x(lds, 0, t);
+  // Products of a stage's last quarter in front of the barrier: those of the first half of the weights' tiles.
+  constexpr int kBefore = RM * (RN / 2);
+  auto stage_of = [&](int stage, auto odd) {
+    constexpr int kOdd = decltype(odd)::value;
+    const uint8_t *from = lds + kOdd * S::kStage, *next = lds + (1 - kOdd) * S::kStage;
+#pragma unroll
+    for (int n = 0; n < RM + RN; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
+    quarter(k0, from);
+    quarter(k1, from);
+    quarter(k2, from);
+#pragma unroll
+    for (int i = 0; i < kBefore; ++i) product(k3, i, nullptr, false);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier)
     __builtin_amdgcn_sched_barrier(0);
-    const int at = stage - first;
-    if ((at & 3) == 1 && first + 4 * (at >> 2) + 4 < stages) write_bytes((at >> 2) + 1);
-    if ((at & 3) == 0 && stage + 4 < stages) load_bytes((at >> 2) + 1);
-    const bool more = stage + 2 < stages;
-    multiply(b, by, std::integral_constant<int, 3>{}, [&](int i) {
-      spread(i, kReads, kSlots, [&](int n) {
-        read_bytes(stage + 1, n);
-        read(stage + 1, 0, a, n);
-      });
-      if (more) copy(stage + 2, i * S::kCopies / kProducts, (i + 1) * S::kCopies / kProducts);
-    });
+#pragma unroll
+    for (int f = 0; f < RN / 2; ++f) read_w(next, 0, f);
+#pragma unroll
+    for (int n = 0; n < RM + RN; ++n) read_bytes(stage + 1, n);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kOdd == 0) write_bytes((stage - first) / 2 + 1, less);
+    // the rest of the products, and between them what is written and requested
+    constexpr int kRest = RM * RN - kBefore;
+#pragma unroll
+    for (int i = 0; i < kRest; ++i) {
+#pragma unroll
+      for (int k = i * S::kLoads / kRest; k < (i + 1) * S::kLoads / kRest; ++k) {
+        write(stage + 2, k);
+        load(there(stage + 3), k);
+      }
+      if (kOdd == 1 && i == kRest - 1) less = load_bytes((stage - first + 1) / 2 + 1);
+      product(k3, kBefore + i, next, true);
+    }
+  };
+  int stage = first;
+  for (; stage + 2 < stages; stage += 2) {
+    stage_of(stage, std::false_type{});
+    stage_of(stage + 1, std::true_type{});
   }
-  three_quarters(stages - 1);
-  multiply(b, by, std::integral_constant<int, 3>{}, [](int) {});
+  const uint8_t *at_last = lds;
+  if (stage + 1 < stages) {
+    stage_of(stage, std::false_type{});
+    at_last = lds + S::kStage;
+  }
+#pragma unroll
+  for (int n = 0; n < RM + RN; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
+  quarter(k0, at_last);
+  quarter(k1, at_last);
+  quarter(k2, at_last);
+#pragma unroll
+  for (int i = 0; i < RM * RN; ++i) product(k3, i, nullptr, false);
   // value r of a lane: column 8 (r / 4) + 4 kg + r % 4 of token col
   if constexpr (!GATED) {
     if (p.splits == 1) __syncthreads();  // (the last stage is read: results go out through its place)
   }
+  // (one code for either type: a choice per number costs a branch per number, 9 us of a 256 x 256 tile's results)
+  auto finish = [&](auto type) {
+    constexpr bool kBF16 = decltype(type)::value;
+    // added without a bias: -0, which leaves every number as it is
+    float bias[GATED ? 1 : RN][4][4];
+    if constexpr (!GATED) {
 #pragma unroll
-  for (int t = 0; t < RM; ++t) {
-    const int64_t m = m0 + (wm * RM + t) * 32 + col;
-    const float scale = p.row && m < p.M ? p.row[m] : 1.0f;
-    if constexpr (GATED) {
+      for (int f = 0; f < RN; ++f)
 #pragma unroll
-      for (int f = 0; f < RN / 2; ++f) {
-        const int64_t n = n0 + wn * (16 * RN) + 32 * f;
-        float v[16];
-        uint32_t top = 0;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float g = acc[t][f][r], u = acc[t][f + RN / 2][r];
-          v[r] = activate(p.row ? g * scale : g, p.row ? u * scale : u, p.bf16);
-          top = umax(top, __float_as_uint(v[r]) & 0x7FFFFFFFu);
-        }
-        top = umax(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        const uint32_t byte = p.q_bits == 4 ? block_byte<4>(top) : block_byte<8>(top);
-        const int64_t block = m * (p.N / kMxBlock) + n / kMxBlock;
-        const bool there = m < p.M && n < p.N;  // (inner is a multiple of 32)
-        if (there && kg == 0) p.out_scale[block] = static_cast<uint8_t>(byte);
-        if (p.q_bits == 4) {  // two bytes of every four are this lane's, the others the lane's 32 on
-          uint32_t mine[2];
+          for (int r = 0; r < 4; ++r) bias[f][j][r] = -0.0f;
+      if (p.bias) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float e[8];
+        for (int f = 0; f < RN; ++f)
 #pragma unroll
-            for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
-            mine[i] = encode4(e, byte);
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg + r;
+              bias[f][j][r] = to_f32<kBF16>(static_cast<const uint16_t *>(p.bias)[n < p.N ? n : p.N - 1]);
+            }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RM; ++t) {
+      const int64_t m = m0 + (wm * RM + t) * 32 + col;
+      const float scale = p.row && m < p.M ? p.row[m] : 1.0f;
+      if constexpr (GATED) {
+#pragma unroll
+        for (int f = 0; f < RN / 2; ++f) {
+          const int64_t n = n0 + wn * (16 * RN) + 32 * f;
+          float v[16];
+          uint32_t top = 0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            v[r] = activate<kBF16>(acc[t][f][r] * scale, acc[t][f + RN / 2][r] * scale);
+            top = umax(top, __float_as_uint(v[r]) & 0x7FFFFFFFu);
           }
-          const uint32_t o0 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[0]), 32)), o1 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[1]), 32));
-          const uint32_t lo = kg ? o1 : mine[0], hi = kg ? mine[1] : o0;  // group 0 stores columns 0 .. 15, group 1 the others
-          const uint2 w = make_uint2((lo & 0xFFFFu) | hi << 16, lo >> 16 | (hi & 0xFFFF0000u));
-          if (there) *reinterpret_cast<mx_loose2 *>(static_cast<uint8_t *>(p.out) + block * 16 + 8 * kg) = mx_loose2{w.x, w.y};
-        } else {
+          top = umax(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          const uint32_t byte = p.q_bits == 4 ? block_byte<4>(top) : block_byte<8>(top);
+          const int64_t block = m * (p.N / kMxBlock) + n / kMxBlock;
+          const bool there = m < p.M && n < p.N;  // (inner is a multiple of 32)
+          if (there && kg == 0) p.out_scale[block] = static_cast<uint8_t>(byte);
+          if (p.q_bits == 4) {  // two bytes of every four are this lane's, the others the lane's 32 on
+            uint32_t mine[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float e[8];
+            for (int i = 0; i < 2; ++i) {
+              float e[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
-            const uint2 w = encode8(e, byte);
-            uint8_t *to = static_cast<uint8_t *>(p.out) + block * 32 + 16 * i + 4 * kg;
-            if (there) {
-              *reinterpret_cast<mx_loose1 *>(to) = w.x;
-              *reinterpret_cast<mx_loose1 *>(to + 8) = w.y;
+              for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
+              mine[i] = encode4(e, byte);
+            }
+            const uint32_t o0 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[0]), 32)), o1 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[1]), 32));
+            const uint32_t lo = kg ? o1 : mine[0], hi = kg ? mine[1] : o0;  // group 0 stores columns 0 .. 15, group 1 the others
+            const uint2 both = make_uint2((lo & 0xFFFFu) | hi << 16, lo >> 16 | (hi & 0xFFFF0000u));
+            if (there) *reinterpret_cast<mx_loose2 *>(static_cast<uint8_t *>(p.out) + block * 16 + 8 * kg) = mx_loose2{both.x, both.y};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float e[8];
+#pragma unroll
+              for (int r = 0; r < 8; ++r) e[r] = v[8 * i + r];
+              const uint2 both = encode8(e, byte);
+              uint8_t *to = static_cast<uint8_t *>(p.out) + block * 32 + 16 * i + 4 * kg;
+              if (there) {
+                *reinterpret_cast<mx_loose1 *>(to) = both.x;
+                *reinterpret_cast<mx_loose1 *>(to + 8) = both.y;
+              }
             }
           }
         }
-      }
-    } else if (p.splits > 1) {
+      } else {
+        // 32 rows of the wave's columns through LDS, so that a store takes whole pieces of rows (four columns per lane as they lie in the registers: 29 us
+        // of 256 tiles of 256 x 256)
+        uint8_t *out = lds + wave * (32 * S::kPitch);
 #pragma unroll
-      for (int f = 0; f < RN; ++f)
+        for (int f = 0; f < RN; ++f)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
-          if (m < p.M && n < p.N)
-            *reinterpret_cast<f32x4 *>(p.partial + (split * p.M + m) * ((p.N + 3) & ~int64_t{3}) + n) =
-                f32x4{acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
-        }
-    } else {
-      // 32 rows of the wave's columns through LDS, so that a store takes whole pieces of rows (four columns per lane as they lie in the registers: 29 us of
-      // 256 tiles of 256 x 256)
-      uint8_t *out = lds + wave * (32 * S::kPitch);
+          for (int j = 0; j < 4; ++j) {
+            float v[4];
 #pragma unroll
-      for (int f = 0; f < RN; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
-          uint32_t h[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = acc[t][f][4 * j + r];
-            if (p.row) v *= scale;
-            if (p.bias) v += bias_of(p, n + r < p.N ? n + r : p.N - 1);
-            h[r] = to16(v, p.bf16);
+            for (int r = 0; r < 4; ++r) v[r] = acc[t][f][4 * j + r] * scale + bias[f][j][r];
+            *reinterpret_cast<uint2 *>(out + col * S::kPitch + (f * 32 + 8 * j + 4 * kg) * 2) =
+                make_uint2(pack2_from_f32<kBF16>(v[0], v[1]), pack2_from_f32<kBF16>(v[2], v[3]));
           }
-          *reinterpret_cast<uint2 *>(out + col * S::kPitch + (f * 32 + 8 * j + 4 * kg) * 2) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-        }
-      asm volatile("" ::: "memory");  // (one wave's LDS accesses follow each other)
+        asm volatile("" ::: "memory");  // (one wave's LDS accesses follow each other)
 #pragma unroll
-      for (int i = 0; i < 2 * RN; ++i) {
-        const int piece = i * 64 + lane, row = piece / (4 * RN), at = piece % (4 * RN) * 8;
-        const int64_t mm = m0 + (wm * RM + t) * 32 + row, n = n0 + wn * (RN * 32) + at;
-        const uint4 w = *reinterpret_cast<const uint4 *>(out + row * S::kPitch + at * 2);
-        if (mm >= p.M || n >= p.N) continue;
-        uint16_t *to = static_cast<uint16_t *>(p.out) + mm * p.N + n;
-        if (n + 7 < p.N) {
-          *reinterpret_cast<mx_loose4 *>(to) = mx_loose4{w.x, w.y, w.z, w.w};
-        } else {
-          const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+        for (int i = 0; i < 2 * RN; ++i) {
+          const int piece = i * 64 + lane, row = piece / (4 * RN), at = piece % (4 * RN) * 8;
+          const int64_t mm = m0 + (wm * RM + t) * 32 + row, n = n0 + wn * (RN * 32) + at;
+          const uint4 w = *reinterpret_cast<const uint4 *>(out + row * S::kPitch + at * 2);
+          if (mm >= p.M || n >= p.N) continue;
+          uint16_t *to = static_cast<uint16_t *>(p.out) + mm * p.N + n;
+          if (n + 7 < p.N) {
+            *reinterpret_cast<mx_loose4 *>(to) = mx_loose4{w.x, w.y, w.z, w.w};
+          } else {
+            const uint32_t h[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int r = 0; r < 7; ++r)
-            if (n + r < p.N) to[r] = static_cast<uint16_t>(h[r / 2] >> (16 * (r & 1)));
+            for (int r = 0; r < 7; ++r)
+              if (n + r < p.N) to[r] = static_cast<uint16_t>(h[r / 2] >> (16 * (r & 1)));
+          }
         }
+        asm volatile("" ::: "memory");
       }
-      asm volatile("" ::: "memory");
+    }
+  };
+  if constexpr (!GATED) {
+    if (p.splits > 1) {
+#pragma unroll
+      for (int t = 0; t < RM; ++t)
+#pragma unroll
+        for (int f = 0; f < RN; ++f)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int64_t m = m0 + (wm * RM + t) * 32 + col, n = n0 + (wn * RN + f) * 32 + 8 * j + 4 * kg;
+            if (m < p.M && n < p.N)
+              *reinterpret_cast<f32x4 *>(p.partial + (split * p.M + m) * ((p.N + 3) & ~int64_t{3}) + n) =
+                  f32x4{acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
+          }
+      return;
     }
   }
+  if (p.bf16) finish(std::true_type{});
+  else finish(std::false_type{});
 }
 
 // the sums of a split K in the order of the splits, then what the tiles do with a sum
@@ -745,8 +814,7 @@ int many_rows_gated(const MxArgs &p, hipStream_t st) {
   MxArgs q = p;
   q.splits = 1;
   const int plan = choose(p.M, 2 * p.N, p.K, XB, false).plan;
-  if (plan == 0) return launch_tile<XB, 1, 2, 1, 2, true>(q, st);
-  if (plan == 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
+  if (plan <= 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
   if (plan == 2) return launch_tile<XB, 2, 2, 2, 2, true>(q, st);
   return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, true>(q, st);
 }
