@@ -303,32 +303,28 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 // at any byte.  Four bytes of a stage, those of this lane's group, are one operand for it.  Bytes behind the end of K are 0 on both sides:
 // whatever codes stand there, a product of 2^-254 does not change a sum.
 // Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
-template <int XB, int RM, int RN, int WM, int WN, int WK>
+template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
-  // Stages that are on their way to registers: where the results leave room, two, whose loads have as long (us, one and two: 64 x 5120 -> 2 x 13824 gated
-  // 22.3, PRE2A; 300 x 4544 -> 4541 16.1, PRE2B).
-  static constexpr int kPre = RM * RN <= 4 ? 2 : 1;
   static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kT = 64 * kW;
   static constexpr int kPx = 2 * XB, kPw = 8;                         // 16-byte pieces of a row in a stage
   static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;    // loads of 1 KB
   static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kLoads = kMyX + kMyW;
   static constexpr int kAtW = kCX * 1024, kStage = kAtW + kCW * 1024;
-  static constexpr int kAtS = 2 * kStage, kRings = kAtS + (kBM + kBN) * 32;  // of a set of waves
+  static constexpr int kAtS = 2 * kStage, kRings = kAtS + (kBM + kBN) * 32;
   static constexpr int kPitch = RN * 64 + 16, kOut = kW * 32 * kPitch;  // (a wave's 32 rows on their way out)
-  static constexpr int kSums = (WK - 1) * kW * RM * RN * 4096, kOuts = kOut + kSums;
-  static constexpr int kLds = WK * kRings > kOuts ? WK * kRings : kOuts;
+  static constexpr int kLds = kRings > kOut ? kRings : kOut;
   static constexpr int kRows = (kBM + kBN + kT - 1) / kT;              // rows of exponent bytes per thread
 };
 
-template <int XB, int RM, int RN, int WM, int WN, int WK, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
-  using S = TileShape<XB, RM, RN, WM, WN, WK>;
+template <int XB, int RM, int RN, int WM, int WN, bool GATED>
+__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
+  using S = TileShape<XB, RM, RN, WM, WN>;
   static_assert(!GATED || RN % 2 == 0, "");
   constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;  // result columns per tile
   extern __shared__ float red[];
-  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, kg = lane >> 5;
-  const int set = WK == 1 ? 0 : all_waves / S::kW, wave = WK == 1 ? all_waves : all_waves % S::kW;
-  uint8_t *const whole_lds = reinterpret_cast<uint8_t *>(red), *lds = whole_lds + set * S::kRings;
+  uint8_t *lds = reinterpret_cast<uint8_t *>(red);
+  const uint32_t lds_at = lds_address(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, kg = lane >> 5;
   const int wn = wave % WN, wm = wave / WN;
   const int nb = static_cast<int>(p.K / kMxBlock), all_stages = (nb + 7) / 8;
   // Workgroups go to the eight dies in turn: each die gets a run of tiles, in bands of four row tiles, column by column, so that those
@@ -341,10 +337,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
   const int band = tile / (kBand * n_tiles), in_band = tile - band * kBand * n_tiles;
   const int high = m_tiles - band * kBand < kBand ? m_tiles - band * kBand : kBand;
   const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * S::kBM, n0 = static_cast<int64_t>(in_band / high) * kCols;
-  // Of the part's stages each set takes every WK-th: what a workgroup reads of a row at a time is WK lines side by side.  (A part has at least WK.)
-  const int part = static_cast<int>(static_cast<int64_t>(all_stages) * split / p.splits), part_end = static_cast<int>(static_cast<int64_t>(all_stages) * (split + 1) / p.splits);
-  const int stages = (part_end - part - set + WK - 1) / WK;  // of this set, which it counts from 0
-  auto global = [&](int stage) { return part + set + stage * WK; };
+  const int first = static_cast<int>(static_cast<int64_t>(all_stages) * split / p.splits);
+  const int stages = static_cast<int>(static_cast<int64_t>(all_stages) * (split + 1) / p.splits);
 
   const int64_t pitch_w = p.K / 2, pitch_x = p.K * XB / 8, left_m = p.M - 1 - m0, left_n = p.N - 1 - n0;
   const uint8_t *xbase = p.x + m0 * pitch_x, *wbase = p.w + n0 * pitch_w;
@@ -367,27 +361,26 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
   // (a load's rows are a multiple of 16 behind the first one's: the same turn)
   static_assert(S::kW * (64 / S::kPx) % 16 == 0, "");
   const int x_to = (x_row(0) * S::kPx + (x_piece ^ turn_of<S::kPx>(x_row(0)))) * 16, w_to = S::kAtW + (w_row(0) * 8 + (w_piece ^ turn_of<8>(w_row(0)))) * 16;
-  constexpr int kPre = S::kPre;
-  u32x4 staged_of[kPre][S::kLoads];
-  auto load = [&](u32x4 (&staged)[S::kLoads], int stage, int i) {  // (pieces past the end of a row come from its last one)
+  u32x4 staged[S::kLoads];
+  auto load = [&](int stage, int i) {  // (pieces past the end of a row come from its last one)
     if (i < S::kMyX) {
-      const int at = global(stage), last = nb * (XB / 4) - 1 - at * S::kPx, piece = x_piece < last ? x_piece : last;
-      staged[i] = *reinterpret_cast<const u32x4 *>(xbase + at * (S::kPx * 16) + (x_off[i] + static_cast<uint32_t>(piece) * 16));
+      const int last = nb * (XB / 4) - 1 - stage * S::kPx, piece = x_piece < last ? x_piece : last;
+      staged[i] = *reinterpret_cast<const u32x4 *>(xbase + stage * (S::kPx * 16) + (x_off[i] + static_cast<uint32_t>(piece) * 16));
     } else {
-      const int at = global(stage), last = nb - 1 - at * 8, piece = w_piece < last ? w_piece : last;
+      const int last = nb - 1 - stage * 8, piece = w_piece < last ? w_piece : last;
       const uint8_t *from = is_up(nth(i - S::kMyX, S::kCW) * 8) ? wbase + p.N * pitch_w : wbase;
-      staged[i] = *reinterpret_cast<const u32x4 *>(from + at * 128 + (w_off[i - S::kMyX] + static_cast<uint32_t>(piece) * 16));
+      staged[i] = *reinterpret_cast<const u32x4 *>(from + stage * 128 + (w_off[i - S::kMyX] + static_cast<uint32_t>(piece) * 16));
     }
   };
-  auto write = [&](const u32x4 (&staged)[S::kLoads], int stage, int i) {
-    uint8_t *to = lds + (stage & 1) * S::kStage;
+  auto write = [&](int stage, int i) {
+    uint8_t *to = lds + ((stage - first) & 1) * S::kStage;
     if (i < S::kMyX) *reinterpret_cast<u32x4 *>(to + x_to + (nth(i, S::kCX) - wave) * 1024) = staged[i];
     else *reinterpret_cast<u32x4 *>(to + w_to + (nth(i - S::kMyX, S::kCW) - wave) * 1024) = staged[i];
   };
   // exponent bytes: rows of x, then of w (a thread without a row of its own takes the last one too)
   const uint8_t *bytes_of[S::kRows];
   auto byte_row = [&](int i) {
-    const int row = static_cast<int>(threadIdx.x) - set * S::kT + i * S::kT;
+    const int row = threadIdx.x + i * S::kT;
     return row < S::kBM + S::kBN ? row : S::kBM + S::kBN - 1;
   };
 #pragma unroll
@@ -396,54 +389,25 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
     bytes_of[i] = row < S::kBM ? p.xs + (m0 + (row < left_m ? row : left_m)) * nb : p.ws + (n0 + (n < left_n ? n : left_n) + (is_up(R) ? p.N : 0)) * nb;
   }
   u32x4 bytes[S::kRows];  // of two stages
-  // A pair of stages' bytes.  One set: sixteen side by side, of the last pair the row's last sixteen, of which the first `less` belong to stages before;
-  // else eight and eight, of which likewise.
-  struct Less {
-    int one, two;
-  };
+  // A pair of stages' bytes; of the last pair the row's last sixteen, of which the first `less` belong to stages before.
   auto load_bytes = [&](int pair) {
-    const int at = global(2 * pair) * 8, next = global(2 * pair + 1) * 8;
-    if constexpr (WK == 1) {
-      const int from = at < nb - 16 ? at : nb - 16;
+    const int at = (first + 2 * pair) * 8, from = at < nb - 16 ? at : nb - 16;
 #pragma unroll
-      for (int i = 0; i < S::kRows; ++i) bytes[i] = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + (nb < 16 ? 0 : from));
-      return Less{at - from, 0};
-    } else {
-      const int from = at < nb - 8 ? at : nb - 8, from2 = next < nb - 8 ? next : nb - 8;
-#pragma unroll
-      for (int i = 0; i < S::kRows; ++i) {
-        const mx_loose2 a = *reinterpret_cast<const mx_loose2 *>(bytes_of[i] + from), b = *reinterpret_cast<const mx_loose2 *>(bytes_of[i] + from2);
-        bytes[i] = u32x4{a[0], a[1], b[0], b[1]};
-      }
-      return Less{at - from, next - from2};
-    }
-  };
-  auto choose_of = [](uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); };  // (bit by bit: no branch)
-  // eight bytes less the first `less`, zeros behind
-  auto without = [&](uint32_t &lo, uint32_t &hi, int less) {
-    const uint32_t by4 = less & 4 ? ~0u : 0, some = less >= 8 ? 0 : ~0u;
-    lo = choose_of(by4, hi, lo);
-    hi &= ~by4;
-    lo = __builtin_amdgcn_alignbyte(hi, lo, less & 3) & some;
-    hi = __builtin_amdgcn_alignbyte(0, hi, less & 3) & some;
+    for (int i = 0; i < S::kRows; ++i) bytes[i] = *reinterpret_cast<const mx_bytes16 *>(bytes_of[i] + (nb < 16 ? 0 : from));
+    return at - from;
   };
   // (eight bytes of a row, a stage's, at their number exclusive-or (row / 8) % 4: 32 rows' reads of one stage at different banks)
-  auto write_bytes = [&](int pair, Less less) {
+  auto write_bytes = [&](int pair, int less) {
 #pragma unroll
     for (int i = 0; i < S::kRows; ++i) {
+      // (sixteen bytes less the first `less`, zeros behind; bit by bit: no branch)
+      const uint32_t by4 = less & 4 ? ~0u : 0, by8 = less & 8 ? ~0u : 0, some = less >= 16 ? 0 : ~0u;
+      auto choose_of = [](uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); };
       u32x4 v = bytes[i];
-      if constexpr (WK == 1) {
-        const uint32_t by8 = less.one & 8 ? ~0u : 0, some = less.one >= 16 ? 0 : ~0u, by4 = less.one & 4 ? ~0u : 0;
-        v = u32x4{choose_of(by4, v[1], v[0]), choose_of(by4, v[2], v[1]), choose_of(by4, v[3], v[2]), v[3] & ~by4};
-        v = u32x4{choose_of(by8, v[2], v[0]), choose_of(by8, v[3], v[1]), v[2] & ~by8, v[3] & ~by8};
-        v = u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], less.one & 3) & some, __builtin_amdgcn_alignbyte(v[2], v[1], less.one & 3) & some,
-                  __builtin_amdgcn_alignbyte(v[3], v[2], less.one & 3) & some, __builtin_amdgcn_alignbyte(0, v[3], less.one & 3) & some};
-      } else {
-        uint32_t w[4] = {v[0], v[1], v[2], v[3]};
-        without(w[0], w[1], less.one);
-        without(w[2], w[3], less.two);
-        v = u32x4{w[0], w[1], w[2], w[3]};
-      }
+      v = u32x4{choose_of(by4, v[1], v[0]), choose_of(by4, v[2], v[1]), choose_of(by4, v[3], v[2]), v[3] & ~by4};
+      v = u32x4{choose_of(by8, v[2], v[0]), choose_of(by8, v[3], v[1]), v[2] & ~by8, v[3] & ~by8};
+      v = u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], less & 3) & some, __builtin_amdgcn_alignbyte(v[2], v[1], less & 3) & some,
+                __builtin_amdgcn_alignbyte(v[3], v[2], less & 3) & some, __builtin_amdgcn_alignbyte(0, v[3], less & 3) & some};
       const int row = byte_row(i);
       uint8_t *to = lds + S::kAtS + row * 32;
       *reinterpret_cast<uint2 *>(to + ((2 * pair & 3) ^ ((row >> 3) & 3)) * 8) = make_uint2(v[0], v[1]);
@@ -478,7 +442,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
   };
   const int bytes_at = S::kAtS + (wm * RM * 32 + col) * 32, bytes_at_w = S::kAtS + (S::kBM + wn * RN * 32 + col) * 32;
   auto read_bytes = [&](int stage, int n) {
-    const int to = ((stage & 3) ^ ((col >> 3) & 3)) * 8;
+    const int to = (((stage - first) & 3) ^ ((col >> 3) & 3)) * 8;
     raw[n] = *reinterpret_cast<const uint2 *>(lds + (n < RM ? bytes_at + n * 1024 : bytes_at_w + (n - RM) * 1024) + to);
   };
   const uint32_t pick = 0x06040200u + static_cast<uint32_t>(kg) * 0x01010101u;
@@ -502,8 +466,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
   constexpr std::integral_constant<int, 3> k3{};
   // (past the last stage: that one once more, not used)
   auto there = [&](int stage) { return stage < stages ? stage : stages - 1; };
-  Less less{0, 0};
-  if (WK > 1 || nb >= 16) {  // (several sets: more than 24 bytes)
+  int less = 0;
+  if (nb >= 16) {
     less = load_bytes(0);
   } else {  // rows of fewer bytes than a load: one pair, byte by byte; the loop's loads, whose bytes are not used, are of the first rows' (M > 16)
 #pragma unroll
@@ -520,23 +484,22 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
     }
   }
 #pragma unroll
-  for (int d = 0; d < kPre; ++d)
+  for (int d = 0; d < 3; ++d) {
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) load(staged_of[d], there(d), i);
-  write_bytes(0, WK == 1 && nb < 16 ? Less{part * 8, 0} : less);
-  less = load_bytes(1);
+    for (int i = 0; i < S::kLoads; ++i) load(there(first + d), i);
+    if (d == 0) {
+      write_bytes(0, nb < 16 ? first * 8 : less);
+      less = load_bytes(1);
+    }
+    if (d < 2) {
 #pragma unroll
-  for (int d = 0; d < 2; ++d) {
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      write(staged_of[d % kPre], d, i);
-      load(staged_of[d % kPre], there(d + kPre), i);
+      for (int i = 0; i < S::kLoads; ++i) write(first + d, i);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < RM + RN; ++n) read_bytes(0, n);
+  for (int n = 0; n < RM + RN; ++n) read_bytes(first, n);
 #pragma unroll
   for (int f = 0; f < RN; ++f) read_w(lds, 0, f);
 #pragma unroll
@@ -560,21 +523,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
 #pragma unroll
     for (int n = 0; n < RM + RN; ++n) read_bytes(stage + 1, n);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (kOdd == 0) write_bytes(stage / 2 + 1, less);
+    if constexpr (kOdd == 0) write_bytes((stage - first) / 2 + 1, less);
     // the rest of the products, and between them what is written and requested
     constexpr int kRest = RM * RN - kBefore;
 #pragma unroll
     for (int i = 0; i < kRest; ++i) {
 #pragma unroll
       for (int k = i * S::kLoads / kRest; k < (i + 1) * S::kLoads / kRest; ++k) {
-        write(staged_of[kOdd % kPre], stage + 2, k);
-        load(staged_of[kOdd % kPre], there(stage + 2 + kPre), k);
+        write(stage + 2, k);
+        load(there(stage + 3), k);
       }
-      if (kOdd == 1 && i == kRest - 1) less = load_bytes((stage + 1) / 2 + 1);
+      if (kOdd == 1 && i == kRest - 1) less = load_bytes((stage - first + 1) / 2 + 1);
       product(k3, kBefore + i, next, true);
     }
   };
-  int stage = 0;
+  int stage = first;
   for (; stage + 2 < stages; stage += 2) {
     stage_of(stage, std::false_type{});
     stage_of(stage + 1, std::true_type{});
@@ -591,37 +554,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void mx_tile_kernel(MxArgs p) {
   quarter(k2, at_last);
 #pragma unroll
   for (int i = 0; i < RM * RN; ++i) product(k3, i, nullptr, false);
-  if constexpr (WK > 1) {
-    if (stages < (part_end - part + WK - 1) / WK) asm volatile("s_barrier" ::: "memory");  // (a stage less than the first set: as many barriers)
-    __syncthreads();  // (the last stages are read)
-    f32x4 *sums = reinterpret_cast<f32x4 *>(whole_lds + S::kOut);
-    auto at = [&](int k, int t, int f, int j) { return sums + ((((k - 1) * S::kW + wave) * RM * RN + t * RN + f) * 4 + j) * 64 + lane; };
-    if (set > 0) {
-#pragma unroll
-      for (int t = 0; t < RM; ++t)
-#pragma unroll
-        for (int f = 0; f < RN; ++f)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) *at(set, t, f, j) = f32x4{acc[t][f][4 * j], acc[t][f][4 * j + 1], acc[t][f][4 * j + 2], acc[t][f][4 * j + 3]};
-    }
-    __syncthreads();
-    if (set > 0) return;
-#pragma unroll
-    for (int t = 0; t < RM; ++t)
-#pragma unroll
-      for (int f = 0; f < RN; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 1; k < WK; ++k) {
-            const f32x4 v = *at(k, t, f, j);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][f][4 * j + r] += v[r];
-          }
-  }
   // value r of a lane: column 8 (r / 4) + 4 kg + r % 4 of token col
   if constexpr (!GATED) {
-    if (WK == 1 && p.splits == 1) __syncthreads();  // (the last stage is read: results go out through its place)
+    if (p.splits == 1) __syncthreads();  // (the last stage is read: results go out through its place)
   }
   // (one code for either type: a choice per number costs a branch per number, 9 us of a 256 x 256 tile's results)
   auto finish = [&](auto type) {
@@ -779,14 +714,14 @@ int launch_ring(const MxArgs &p, hipStream_t st) {
 }
 
 // (2^31 threads per launch: rows beyond are further launches, which follow each other and share the memory of the parts' sums)
-template <int XB, int RM, int RN, int WM, int WN, int WK, bool GATED>
+template <int XB, int RM, int RN, int WM, int WN, bool GATED>
 int launch_tile(const MxArgs &p, hipStream_t st) {
-  using S = TileShape<XB, RM, RN, WM, WN, WK>;
+  using S = TileShape<XB, RM, RN, WM, WN>;
   static_assert(S::kLds <= kLdsBytes, "");
-  auto kern = mx_tile_kernel<XB, RM, RN, WM, WN, WK, GATED>;
+  auto kern = mx_tile_kernel<XB, RM, RN, WM, WN, GATED>;
   if (int rc = prepare(kern, S::kLds)) return rc;
   constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;
-  const int64_t across = (p.N + kCols - 1) / kCols * p.splits, most = INT32_MAX / (S::kT * WK) / across * S::kBM;
+  const int64_t across = (p.N + kCols - 1) / kCols * p.splits, most = INT32_MAX / (S::kW * 64) / across * S::kBM;
   if (most == 0) return QUIK_ERR_RANGE;
   for (int64_t m = 0; m < p.M; m += most) {
     MxArgs q = p;
@@ -796,7 +731,7 @@ int launch_tile(const MxArgs &p, hipStream_t st) {
     if (p.row) q.row = p.row + m;
     q.out = static_cast<uint8_t *>(p.out) + (GATED ? m * p.N * p.q_bits / 8 : m * p.N * 2);
     if (GATED) q.out_scale = p.out_scale + m * (p.N / kMxBlock);
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((q.M + S::kBM - 1) / S::kBM * across)), dim3(S::kT * WK), S::kLds, st, q);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((q.M + S::kBM - 1) / S::kBM * across)), dim3(64 * S::kW), S::kLds, st, q);
     if (int rc = check_launch()) return rc;
     if (p.splits > 1) {
       hipLaunchKernelGGL(mx_join_kernel, dim3(static_cast<unsigned>((q.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, q);
@@ -863,33 +798,25 @@ Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
 }
 int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
 
-// Small tiles: two sets of waves on either half of a part's stages, where there are two for each.
-bool two_sets(int64_t K, int splits) { return (K + 255) / 256 >= 4 * splits; }
-
 template <int XB>
 int many_rows(const MxArgs &p, int64_t workspace_bytes, hipStream_t st) {
   MxArgs q = p;
   Choice c = choose(p.M, p.N, p.K, XB, true);
   if (!p.partial || workspace_bytes < partial_bytes(p.M, p.N, c.splits)) c = choose(p.M, p.N, p.K, XB, false);
   q.splits = c.splits;
-  if (c.plan == 3) return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, 1, false>(q, st);
-  if (two_sets(p.K, c.splits)) {
-    if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, 2, false>(q, st);
-    if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, 2, false>(q, st);
-    return launch_tile<XB, 2, 2, 2, 2, (XB == 8 ? 1 : 2), false>(q, st);  // (8-bit rows: one set fills LDS)
-  }
-  if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, 1, false>(q, st);
-  if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, 1, false>(q, st);
-  return launch_tile<XB, 2, 2, 2, 2, 1, false>(q, st);
+  if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, false>(q, st);
+  if (c.plan == 1) return launch_tile<XB, 2, 1, 1, 4, false>(q, st);
+  if (c.plan == 2) return launch_tile<XB, 2, 2, 2, 2, false>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, false>(q, st);
 }
 template <int XB>
 int many_rows_gated(const MxArgs &p, hipStream_t st) {
   MxArgs q = p;
   q.splits = 1;
   const int plan = choose(p.M, 2 * p.N, p.K, XB, false).plan;
-  if (plan == 3) return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, 1, true>(q, st);
-  if (two_sets(p.K, 1)) return plan <= 1 ? launch_tile<XB, 1, 2, 2, 2, 2, true>(q, st) : launch_tile<XB, 2, 2, 2, 2, (XB == 8 ? 1 : 2), true>(q, st);
-  return plan <= 1 ? launch_tile<XB, 1, 2, 2, 2, 1, true>(q, st) : launch_tile<XB, 2, 2, 2, 2, 1, true>(q, st);
+  if (plan <= 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
+  if (plan == 2) return launch_tile<XB, 2, 2, 2, 2, true>(q, st);
+  return launch_tile<XB, (XB == 8 ? 2 : 4), 2, 2, 4, true>(q, st);
 }
 
 bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
