@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 
 // More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on stages of 256 columns: whole lines
 // of 128 bytes of the weights' rows (half lines cost as many requests again: 8192 x 8192 -> 8192 on stages of 128 columns 434 us).  LDS holds two
-// stages; a third is on its way to registers.  (Direct copies to LDS hold the wave that issues them until the CU has taken the ones before, some
+// stages; one or two more are on their way to registers.  (Direct copies to LDS hold the wave that issues them until the CU has taken the ones before, some
 // 36 cycles per kilobyte, and its products with it; and they can start only when their place is free: 300 us.)
 // A stage is four products of 64 columns.  An operand is read again for the next one behind its last product of this one.  In the middle of the fourth
 // there is a barrier: every wave has read all of the stage, and the next one is there; behind it the stage after the next is written over
@@ -305,6 +305,9 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 // Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
 template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
+  // Stages on their way to registers: two where the results leave room, with their loads dealt to three quarters of a stage (us, one on its way and
+  // this: 300 x 4544 -> 4544 16.2, 14.9, 64 x 5120 -> 27648 23.8, 22.4).
+  static constexpr int kPre = RM * RN <= 4 ? 2 : 1;
   static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kT = 64 * kW;
   static constexpr int kPx = 2 * XB, kPw = 8;                         // 16-byte pieces of a row in a stage
   static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;    // loads of 1 KB
@@ -361,8 +364,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   // (a load's rows are a multiple of 16 behind the first one's: the same turn)
   static_assert(S::kW * (64 / S::kPx) % 16 == 0, "");
   const int x_to = (x_row(0) * S::kPx + (x_piece ^ turn_of<S::kPx>(x_row(0)))) * 16, w_to = S::kAtW + (w_row(0) * 8 + (w_piece ^ turn_of<8>(w_row(0)))) * 16;
-  u32x4 staged[S::kLoads];
-  auto load = [&](int stage, int i) {  // (pieces past the end of a row come from its last one)
+  constexpr int kPre = S::kPre;
+  u32x4 staged_of[kPre][S::kLoads];
+  auto load = [&](u32x4 (&staged)[S::kLoads], int stage, int i) {  // (pieces past the end of a row come from its last one)
     if (i < S::kMyX) {
       const int last = nb * (XB / 4) - 1 - stage * S::kPx, piece = x_piece < last ? x_piece : last;
       staged[i] = *reinterpret_cast<const u32x4 *>(xbase + stage * (S::kPx * 16) + (x_off[i] + static_cast<uint32_t>(piece) * 16));
@@ -372,7 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
       staged[i] = *reinterpret_cast<const u32x4 *>(from + stage * 128 + (w_off[i - S::kMyX] + static_cast<uint32_t>(piece) * 16));
     }
   };
-  auto write = [&](int stage, int i) {
+  auto write = [&](const u32x4 (&staged)[S::kLoads], int stage, int i) {
     uint8_t *to = lds + ((stage - first) & 1) * S::kStage;
     if (i < S::kMyX) *reinterpret_cast<u32x4 *>(to + x_to + (nth(i, S::kCX) - wave) * 1024) = staged[i];
     else *reinterpret_cast<u32x4 *>(to + w_to + (nth(i - S::kMyX, S::kCW) - wave) * 1024) = staged[i];
@@ -456,9 +460,12 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
     if (reads && f == RN - 1) read_x(next, (s + 1) % 4, t);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto quarter = [&](auto which, const uint8_t *next) {
+  auto quarter = [&](auto which, const uint8_t *next, auto behind) {
 #pragma unroll
-    for (int i = 0; i < RM * RN; ++i) product(which, i, next, true);
+    for (int i = 0; i < RM * RN; ++i) {
+      product(which, i, next, true);
+      behind(decltype(which)::value * RM * RN + i);
+    }
   };
   constexpr std::integral_constant<int, 0> k0{};
   constexpr std::integral_constant<int, 1> k1{};
@@ -484,16 +491,15 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
     }
   }
 #pragma unroll
-  for (int d = 0; d < 3; ++d) {
+  for (int i = 0; i < S::kLoads; ++i) load(staged_of[0], first, i);
+  write_bytes(0, nb < 16 ? first * 8 : less);
+  less = load_bytes(1);
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) load(there(first + d), i);
-    if (d == 0) {
-      write_bytes(0, nb < 16 ? first * 8 : less);
-      less = load_bytes(1);
-    }
-    if (d < 2) {
+  for (int d = 0; d < 2; ++d) {
 #pragma unroll
-      for (int i = 0; i < S::kLoads; ++i) write(first + d, i);
+    for (int i = 0; i < S::kLoads; ++i) {
+      write(staged_of[0], first + d, i);
+      load(staged_of[0], there(first + d + 1), i);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -505,15 +511,25 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
 #pragma unroll
   for (int t = 0; t < RM; ++t) read_x(lds, 0, t);
   // Products of a stage's last quarter in front of the barrier: those of the first half of the weights' tiles.
-  constexpr int kBefore = RM * (RN / 2);
+  constexpr int kBefore = RM * (RN / 2), kHalf = S::kLoads / 2;
   auto stage_of = [&](int stage, auto odd) {
     constexpr int kOdd = decltype(odd)::value;
     const uint8_t *from = lds + kOdd * S::kStage, *next = lds + (1 - kOdd) * S::kStage;
 #pragma unroll
     for (int n = 0; n < RM + RN; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
-    quarter(k0, from);
-    quarter(k1, from);
-    quarter(k2, from);
+    // What is requested of the stage behind those under way, in the places of the stage's products: two on their way, in the first three quarters;
+    // one, half of it behind its place's writing and half in the first quarter.
+    constexpr int kSlots = kPre == 2 ? 3 * RM * RN : RM * RN, kFrom = kPre == 2 ? 0 : kHalf;
+    auto request = [&](int i) {
+      if (i >= kSlots) return;
+#pragma unroll
+      for (int k = kFrom + i * (S::kLoads - kFrom) / kSlots; k < kFrom + (i + 1) * (S::kLoads - kFrom) / kSlots; ++k)
+        load(staged_of[(kOdd + 1) % kPre], there(stage + 1 + kPre), k);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    quarter(k0, from, request);
+    quarter(k1, from, request);
+    quarter(k2, from, request);
 #pragma unroll
     for (int i = 0; i < kBefore; ++i) product(k3, i, nullptr, false);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (a wait and a barrier)
@@ -530,8 +546,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
     for (int i = 0; i < kRest; ++i) {
 #pragma unroll
       for (int k = i * S::kLoads / kRest; k < (i + 1) * S::kLoads / kRest; ++k) {
-        write(stage + 2, k);
-        load(there(stage + 3), k);
+        write(staged_of[kOdd % kPre], stage + 2, k);
+        if (kPre == 1 && k < kHalf) load(staged_of[0], there(stage + 3), k);
       }
       if (kOdd == 1 && i == kRest - 1) less = load_bytes((stage - first + 1) / 2 + 1);
       product(k3, kBefore + i, next, true);
@@ -549,9 +565,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   }
 #pragma unroll
   for (int n = 0; n < RM + RN; ++n) by[n] = __builtin_amdgcn_perm(raw[n].y, raw[n].x, pick);
-  quarter(k0, at_last);
-  quarter(k1, at_last);
-  quarter(k2, at_last);
+  quarter(k0, at_last, [](int) {});
+  quarter(k1, at_last, [](int) {});
+  quarter(k2, at_last, [](int) {});
 #pragma unroll
   for (int i = 0; i < RM * RN; ++i) product(k3, i, nullptr, false);
   // value r of a lane: column 8 (r / 4) + 4 kg + r % 4 of token col
@@ -766,28 +782,34 @@ int few_rows_gated(MxArgs p, hipStream_t st) {
   return launch_ring<XB, 16, 4, 4, 2, 2, TAIL, true>(p, st);
 }
 
-// Tiles of more than 16 rows, for 4- and for 8-bit rows: rows, columns, the time of a step of 128 columns on a CU in us, and what a tile takes
-// besides.
+// Tiles of more than 16 rows, for 4- and for 8-bit rows: rows, columns, workgroups that a CU takes at a time, the time of a stage of 256 columns with
+// one of them and with all, and what a workgroup takes besides, in us.
 struct TilePlan {
-  int rows, cols;
-  double step, round;
+  int rows, cols, slots;
+  double one, full, round;
 };
-constexpr TilePlan kPlans[2][4] = {{{32, 128, 0.12, 0.5}, {64, 128, 0.14, 0.5}, {128, 128, 0.2, 1.0}, {256, 256, 0.55, 3.0}},
-                                   {{32, 128, 0.14, 0.5}, {64, 128, 0.2, 0.5}, {128, 128, 0.3, 1.0}, {128, 256, 0.5, 2.0}}};
+constexpr TilePlan kPlans[2][4] = {{{32, 128, 3, 0.45, 1.2, 2.0}, {64, 128, 2, 0.58, 0.98, 2.0}, {128, 128, 2, 0.76, 1.5, 2.0}, {256, 256, 1, 1.75, 2.0, 5.0}},
+                                   {{32, 128, 2, 0.55, 1.2, 2.0}, {64, 128, 2, 0.67, 1.35, 2.0}, {128, 128, 1, 1.15, 1.2, 2.0}, {128, 256, 1, 1.8, 1.85, 4.0}}};
 struct Choice {
   int plan, splits;
 };
+// The cheapest tiles and K split: the rounds of workgroups, no less than the weights from memory, and for a split the second launch and its sums, written
+// and read.  us, as the rule has it and measured (the next best measured): 64 x 4096 -> 4096, 32 rows, 11.1, 10.8 (64 rows, K in 4: 12.1); 64 x 13824 -> 5120, 64
+// rows, K in 6, 17.3, 17.0 (32 rows 18.5); 300 x 4544 -> 4544, 64 rows, 14.9, 14.9 (128 rows 18.2); 777 x 5120 -> 5120, 128 rows, 34.5, 29.7 (64 rows 33.2);
+// 2048 x 4096 -> 4096, 128 rows, 28.5, 28.7 (256 rows 34.2); 2048 x 8192 -> 28672, 256 rows, 278, 277 (128 rows 333).
 Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
   Choice best{1, 1};
   double least = 1e30;
-  const int64_t cus = num_cus(), steps = (K + 127) / 128;
+  const int64_t cus = num_cus(), stages = (K + 255) / 256;
+  const double weights = static_cast<double>(N) * static_cast<double>(K) * 0.53125 / 4.6e6 + 1.0;
   for (int i = 0; i < 4; ++i) {
     const TilePlan &t = kPlans[x_bits == 8][i];
     const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
-    for (int s = 1; s <= (may_split ? 16 : 1) && 8 * s <= steps + 7; ++s) {
-      const int64_t rounds = (tiles * s + cus - 1) / cus, deep = (steps + s - 1) / s;
-      const double us = static_cast<double>(rounds) * (static_cast<double>(deep) * t.step + t.round) + 3.0 +
-                        (s > 1 ? 3.0 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8e-6 / 5.0 : 0.0);
+    for (int s = 1; s <= (may_split ? 16 : 1) && (s == 1 || 2 * s <= stages); ++s) {
+      const int64_t groups = tiles * s, rounds = groups / (cus * t.slots), rest = groups % (cus * t.slots), deep = (stages + s - 1) / s;
+      double us = static_cast<double>(rounds) * (static_cast<double>(deep) * t.full + t.round);
+      if (rest) us += static_cast<double>(deep) * (rest <= cus ? t.one : t.full) + t.round;
+      us = (us > weights ? us : weights) + 2.5 + (s > 1 ? 3.5 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8e-6 / 5.0 : 0.0);
       if (us < least) {
         least = us;
         best = Choice{i, s};
