@@ -30,16 +30,20 @@ __device__ __forceinline__ uint32_t encode4(const float (&v)[8], uint32_t byte) 
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], unit, 2);
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], unit, 3);
 }
+// (the conversion divides by the power of two; it does not stop at 448, but makes a NaN of numbers from 464 on)
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t byte) {
   if (byte == kMxNan) return make_uint2(0, 0);
-  const float inv = __uint_as_float((254u - byte) << 23);
+  typedef short s2 __attribute__((ext_vector_type(2)));
+  const float unit = block_unit(byte), most = 448.0f * unit;
   float t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.0f, 448.0f);
-  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[4], t[5], 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[6], t[7], hi, true);
-  return make_uint2(static_cast<uint32_t>(lo), static_cast<uint32_t>(hi));
+  for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
+  s2 lo = {0, 0}, hi = {0, 0};
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, t[0], t[1], unit, false);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, t[2], t[3], unit, true);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, t[4], t[5], unit, false);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, t[6], t[7], unit, true);
+  return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
 // Eight codes -> eight values (exact in fp32; NaNs where the byte is 255)

@@ -45,52 +45,75 @@ __device__ __forceinline__ void put(const float (&v)[8], int left, uint8_t *code
   store_block<BITS, WIDE>(v, left, codes + (vec * size + c * int64_t{8}) * BITS / 8, scale + vec * blocks + c / 4, c % 4 == 0);
 }
 
-// L lanes per head, the power of two from four per block up.
-template <bool BF16, int L, bool WIDE>
+// L lanes per head, the power of two from four per block up.  WHOLE: every column turns, in chunks of eight that turn with each other, at 16-byte
+// addresses; the other instance takes every size, element by element where a column's fellow is concerned.
+template <bool BF16, int L, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
   constexpr int kGroups = 256 / L;
-  const int64_t token = blockIdx.x / p.splits;
-  const int split = static_cast<int>(blockIdx.x % p.splits), c = threadIdx.x % L, blocks = (p.size + kMxBlock - 1) / kMxBlock;
+  const int64_t token = blockIdx.x / static_cast<uint32_t>(p.splits);
+  const int split = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.splits)), c = threadIdx.x % L, blocks = (p.size + kMxBlock - 1) / kMxBlock;
   const int rest = p.size - 8 * c, left = rest < 0 ? 0 : rest < 8 ? rest : 8, turned = 2 * p.half;
   const int64_t at = p.position[token], slot = p.slot[token];
   const bool known = at >= 0 && at < p.positions, kept = slot >= 0 && slot < p.slots;
   // this lane's columns: the factors of their own and of the number that they turn with, and where that one is
-  float own[8], other[8];
+  alignas(16) float own[8], other[8];
   int with[8];
+  if constexpr (WHOLE) {
+    const bool front = 8 * c < p.half;
+    const int j = left > 0 ? (front ? 8 * c : 8 * c - p.half) : 0;
+    const int64_t from = (known ? at : 0) * p.half + j;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = 8 * c + e;
-    own[e] = known ? 1.0f : __builtin_nanf(""), other[e] = 0.0f, with[e] = e < left ? i : 0;
-    if (known && i < turned && e < left) {
-      const int j = i < p.half ? i : i - p.half;
-      own[e] = p.cos[at * p.half + j];
-      other[e] = p.sin[at * p.half + j];
-      if (i < p.half) other[e] = -other[e];
-      with[e] = i < p.half ? i + p.half : j;
+    for (int e = 0; e < 8; e += 4) {
+      if (known) {
+        *reinterpret_cast<float4 *>(own + e) = *reinterpret_cast<const float4 *>(p.cos + from + e);
+        *reinterpret_cast<float4 *>(other + e) = *reinterpret_cast<const float4 *>(p.sin + from + e);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      other[e] = front ? -other[e] : other[e];
+      if (!known) own[e] = __builtin_nanf(""), other[e] = 0.0f;
+    }
+    with[0] = front ? j + p.half : j;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = 8 * c + e;
+      own[e] = known ? 1.0f : __builtin_nanf(""), other[e] = 0.0f, with[e] = e < left ? i : 0;
+      if (i < turned && e < left) {
+        const int j = i < p.half ? i : i - p.half;
+        if (known) {
+          own[e] = p.cos[at * p.half + j];
+          other[e] = p.sin[at * p.half + j];
+          if (i < p.half) other[e] = -other[e];
+        }
+        with[e] = i < p.half ? i + p.half : j;
+      }
     }
   }
-  // (whole chunks of eight turn with each other)
-  const bool chunks = WIDE && p.half % 8 == 0;
   const int all = p.q_heads + 2 * p.kv_heads;
+  const int64_t base_q = token * p.pitch_q, base_k = token * p.pitch_k, base_v = token * p.pitch_v;
   for (int item = split * kGroups + threadIdx.x / L; item < all; item += p.splits * kGroups) {
     const bool is_q = item < p.q_heads, is_v = item >= p.q_heads + p.kv_heads;
     const int head = is_q ? item : is_v ? item - p.q_heads - p.kv_heads : item - p.q_heads;
-    const uint16_t *from = (is_q ? p.q + token * p.pitch_q : is_v ? p.v + token * p.pitch_v : p.k + token * p.pitch_k) + head * static_cast<int64_t>(p.size);
+    const uint16_t *from = (is_q ? p.q + base_q : is_v ? p.v + base_v : p.k + base_k) + head * p.size;
     alignas(16) uint16_t x[8] = {}, y[8] = {};
-    if (left > 0) load_eight<WIDE>(from + 8 * c, left, x);
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = to_f32<BF16>(x[e]);
-    if (!is_v) {
-      const uint16_t *gain = is_q ? p.q_gain : p.k_gain;
-      if (left > 0) {
-        if (chunks) {
+    if (left > 0) {
+      load_eight<WHOLE>(from + 8 * c, left, x);
+      if (!is_v) {
+        if constexpr (WHOLE) {
           load_eight<true>(from + with[0], 8, y);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = from[with[e]];
         }
       }
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32<BF16>(x[e]);
+    if (!is_v) {
+      const uint16_t *gain = is_q ? p.q_gain : p.k_gain;
       float t[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] = to_f32<BF16>(y[e]);
@@ -112,8 +135,8 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
         if (!(square < __builtin_inff())) f = __builtin_nanf("");
         alignas(16) uint16_t g[8] = {}, h[8] = {};
         if (left > 0) {
-          load_eight<WIDE>(gain + 8 * c, left, g);
-          if (chunks) {
+          load_eight<WHOLE>(gain + 8 * c, left, g);
+          if constexpr (WHOLE) {
             load_eight<true>(gain + with[0], 8, h);
           } else {
 #pragma unroll
@@ -126,21 +149,28 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
           t[e] = t[e] * lift * f * to_f32<BF16>(h[e]);
         }
       }
-      if (turned == p.size || 8 * c < turned || !known) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < left ? 8 * c + e < turned || !known ? v[e] * own[e] + t[e] * other[e] : v[e] : 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        const float turn = v[e] * own[e] + t[e] * other[e];
+        v[e] = WHOLE || (e < left && (8 * c + e < turned || !known)) ? turn : v[e];  // (a column that stays is not added 0 * t: t may be an infinity)
+      }
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? v[e] : 0.0f;
       }
     }
     if (is_q) {
-      alignas(16) uint16_t h[8];
+      alignas(16) uint32_t h[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = from_f32<BF16>(v[e]);
-      if (left > 0) store_eight<WIDE>(p.q_out + (token * p.q_heads + head) * p.size + 8 * c, left, h);
+      for (int e = 0; e < 4; ++e) h[e] = pack2_from_f32<BF16>(v[2 * e], v[2 * e + 1]);
+      alignas(16) uint16_t out[8];
+      *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(h);
+      if (left > 0) store_eight<WHOLE>(p.q_out + (token * p.q_heads + head) * p.size + 8 * c, left, out);
     } else {
       uint8_t *codes = is_v ? p.v_codes : p.k_codes, *scale = is_v ? p.v_scale : p.k_scale;
       const int64_t vec = slot * p.kv_heads + head;
-      if ((is_v ? p.v_bits : p.k_bits) == 4) put<4, WIDE>(v, kept ? left : 0, codes, scale, vec, p.size, blocks, c);
-      else put<8, WIDE>(v, kept ? left : 0, codes, scale, vec, p.size, blocks, c);
+      if ((is_v ? p.v_bits : p.k_bits) == 4) put<4, WHOLE>(v, kept ? left : 0, codes, scale, vec, p.size, blocks, c);
+      else put<8, WHOLE>(v, kept ? left : 0, codes, scale, vec, p.size, blocks, c);
     }
   }
 }
@@ -204,7 +234,7 @@ extern "C" int quik_mx_rotate_to_cache(const quik_mx_heads *h, void *stream) {
   p.slots = h->slots, p.q_heads = static_cast<int>(h->q_heads), p.kv_heads = static_cast<int>(h->kv_heads), p.size = static_cast<int>(D);
   p.half = static_cast<int>(h->half), p.k_bits = h->k_bits, p.v_bits = h->v_bits;
   auto wide_rows = [&](const void *at, int64_t pitch) { return aligned(at, 16) && (h->tokens == 1 || pitch % 8 == 0); };
-  const bool wide = D % 8 == 0 && wide_rows(h->q, h->q_pitch) && wide_rows(h->k, h->k_pitch) && wide_rows(h->v, h->v_pitch) && aligned(h->q_out, 16) &&
+  const bool wide = D % 8 == 0 && 2 * h->half == D && h->half % 8 == 0 && wide_rows(h->q, h->q_pitch) && wide_rows(h->k, h->k_pitch) && wide_rows(h->v, h->v_pitch) && aligned(h->q_out, 16) && aligned(h->cos, 16) && aligned(h->sin, 16) &&
                     aligned(h->q_gain, 16) && aligned(h->k_gain, 16) && aligned(h->k_codes, 8) && aligned(h->v_codes, 8);
   return h->dtype == QUIK_BF16 ? by_size<true>(p, h->tokens, wide, as_stream(stream)) : by_size<false>(p, h->tokens, wide, as_stream(stream));
 }

@@ -213,6 +213,7 @@ template <bool BF16, bool ADD, int BITS>
 int launch_norm(MxRows p, bool wide, hipStream_t st) {
   const int64_t lanes = lanes_of(p.cols), all = p.rows, most = 1 << 20;
   p.by_lanes = divide_by(lanes);
+  // (two or four chunks per thread, requested together, gain nothing: 777 x 5120 8.2, 8.4, 8.9 us, 2048 x 8192 20.1, 20.3, 21.1, 300 x 28672 13.5, 15.6, 17.3)
   const int64_t threads = lanes < 1024 ? (lanes + 63) / 64 * 64 : 1024;
   for (int64_t first = 0; first < all; first += most) {
     p.rows = all - first < most ? all - first : most;
