@@ -476,7 +476,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   int less = 0;
   if (nb >= 16) {
     less = load_bytes(0);
-  } else {  // rows of fewer bytes than a load: one pair, byte by byte; the loop's loads, whose bytes are not used, are of the first rows' (M > 16)
+  } else {  // rows of fewer bytes than a load: one pair, byte by byte; the loop's loads, whose bytes are not used, are of x, a row of which has sixteen
 #pragma unroll
     for (int i = 0; i < S::kRows; ++i) {
       uint64_t v[2] = {0, 0};
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
         else v[1] |= byte << (8 * (e - 8));
       }
       bytes[i] = u32x4{static_cast<uint32_t>(v[0]), static_cast<uint32_t>(v[0] >> 32), static_cast<uint32_t>(v[1]), static_cast<uint32_t>(v[1] >> 32)};
-      bytes_of[i] = p.xs;
+      bytes_of[i] = p.x;
     }
   }
 #pragma unroll
@@ -764,15 +764,18 @@ int deal_columns(int64_t N, int ft) {
   return static_cast<int>((N + rounds * cus - 1) / (rounds * cus));
 }
 
+// Two matrix tiles side by side where one would leave a second round of workgroups; then four waves with two blocks under way, not eight with one
+// (us: 1 x 8192 -> 28672, 8 bit, 23.9, 25.5; 16 x 13824 -> 5120 10.2, 10.4; 8 x 8192 -> 8192 10.0, 9.9; gated the ring of two is the better one: 1 x 5120 ->
+// 27648 17.6, 20.5, and with one tile, 1 x 4096 -> 4096 4.2, 4.6).
 template <int XB, bool TAIL>
 int few_rows(MxArgs p, hipStream_t st) {
   const int ft = p.N > 16 * num_cus() ? 2 : 1;
   p.width = deal_columns(p.N, ft);
   if (p.M <= 8) {
-    if (ft == 2) return launch_ring<XB, 8, 2, 8, 2, 2, TAIL, false>(p, st);
+    if (ft == 2) return launch_ring<XB, 8, 2, 4, 3, 2, TAIL, false>(p, st);
     return launch_ring<XB, 8, 1, 8, 2, 2, TAIL, false>(p, st);
   }
-  if (ft == 2) return launch_ring<XB, 16, 2, 4, 2, 2, TAIL, false>(p, st);
+  if (ft == 2) return launch_ring<XB, 16, 2, 4, 3, 2, TAIL, false>(p, st);
   return launch_ring<XB, 16, 1, 4, 2, 2, TAIL, false>(p, st);
 }
 template <int XB, bool TAIL>
