@@ -480,7 +480,8 @@ int quik_mx_rotate_to_cache(const quik_mx_heads *heads, void *stream);
 /* Product of rows in blocks of 32 with 4-bit weights in blocks of 32, on the scaled matrix instructions:
  *   out[m,n] = dtype( scale_row[m] * sum_k x[m,k] * w[n,k] + bias[n] )
  *   x  x_bits 4: [M, K/2] uint8, 8: [M, K]; x_scale [M, K/32];  w [N, K/2] uint8; w_scale [N, K/32];  scale_row [M] fp32 or NULL (1);  bias [N] or NULL
- * K % 32 == 0, K <= 2^20; x and w 16-byte aligned.  Sums in fp32, one rounding. */
+ * K % 32 == 0, K <= 2^20; x and w 16-byte aligned.  Sums in fp32, one rounding; products of 8-bit rows are aligned to the largest of eight at a time
+ * first, and cut off 2^-13 below it. */
 int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row, const void *bias,
                    int dtype, int64_t M, int64_t N, int64_t K, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 /* Calls whose tiles leave CUs idle split K: workspace (16-byte aligned, not to be shared by calls that may overlap, free again behind the call on the
@@ -488,8 +489,8 @@ int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint
  * fewer bytes K is not split: slower, the same result within its rounding. */
 int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t N, int64_t K);
 /* The first half of a gated feed-forward block in one launch: gate = x w[:inner]^T and up = x w[inner:]^T (times scale_row, rounded to dtype, which is all
- * that dtype is for), value = gate / (1 + exp(-gate)) * up, codes of q_bits: the bits that quik_mx_matmul and quik_mx_silu_mul_quantize give one after
- * the other where K is not split.  w [2 inner, K/2], inner % 32 == 0. */
+ * that dtype is for), value = gate / (1 + exp(-gate)) * up, codes of q_bits: those of quik_mx_matmul and quik_mx_silu_mul_quantize one after the
+ * other, up to the order of the sums over K.  w [2 inner, K/2], inner % 32 == 0. */
 int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row, int dtype,
                          int64_t M, int64_t inner, int64_t K, int q_bits, void *q, uint8_t *q_scale, void *stream);
 

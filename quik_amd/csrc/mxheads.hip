@@ -7,6 +7,8 @@
 // Bound by memory: every number is read once and written once.  A head is 4 lanes per block, eight columns each; the columns that turn with a lane's are
 // loaded a second time (from the nearest cache) rather than exchanged.  A workgroup keeps its token's cosines and sines in registers and goes through
 // the heads; few tokens are dealt to several workgroups each.
+// 4096 tokens of 40 + 2 * 40 heads of 128 fp16, keys 8 bit, values 4: 45.4 us for 195 MB, 4.3 TB/s of a copy's 5.1 (by single columns 73.9 us); 64 tokens of
+// 64 + 2 * 8 heads bf16 5.5 us, which is a launch and its loads' way.
 #include "mx_format.h"
 #include "rows_math.h"
 
@@ -73,6 +75,7 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
     for (int e = 0; e < 8; ++e) {
       other[e] = front ? -other[e] : other[e];
       if (!known) own[e] = __builtin_nanf(""), other[e] = 0.0f;
+      if (left <= 0) own[e] = 0.0f, other[e] = 0.0f;  // (behind the head's end, in its last block: zeros whatever the angles are)
     }
     with[0] = front ? j + p.half : j;
   } else {
@@ -234,7 +237,8 @@ extern "C" int quik_mx_rotate_to_cache(const quik_mx_heads *h, void *stream) {
   p.slots = h->slots, p.q_heads = static_cast<int>(h->q_heads), p.kv_heads = static_cast<int>(h->kv_heads), p.size = static_cast<int>(D);
   p.half = static_cast<int>(h->half), p.k_bits = h->k_bits, p.v_bits = h->v_bits;
   auto wide_rows = [&](const void *at, int64_t pitch) { return aligned(at, 16) && (h->tokens == 1 || pitch % 8 == 0); };
-  const bool wide = D % 8 == 0 && 2 * h->half == D && h->half % 8 == 0 && wide_rows(h->q, h->q_pitch) && wide_rows(h->k, h->k_pitch) && wide_rows(h->v, h->v_pitch) && aligned(h->q_out, 16) && aligned(h->cos, 16) && aligned(h->sin, 16) &&
-                    aligned(h->q_gain, 16) && aligned(h->k_gain, 16) && aligned(h->k_codes, 8) && aligned(h->v_codes, 8);
+  const bool wide = 2 * h->half == D && h->half % 8 == 0 && wide_rows(h->q, h->q_pitch) && wide_rows(h->k, h->k_pitch) && wide_rows(h->v, h->v_pitch) &&
+                    aligned(h->q_out, 16) && aligned(h->cos, 16) && aligned(h->sin, 16) && aligned(h->q_gain, 16) && aligned(h->k_gain, 16) &&
+                    aligned(h->k_codes, 8) && aligned(h->v_codes, 8);
   return h->dtype == QUIK_BF16 ? by_size<true>(p, h->tokens, wide, as_stream(stream)) : by_size<false>(p, h->tokens, wide, as_stream(stream));
 }

@@ -121,7 +121,8 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor = None, bits: int = 4):
     """Root-mean-square norm in blocks of 32, in one launch: h = x + residual (rounded to x's type; residual None: h = x), value = h * weight *
     scale_row with scale_row = 1 / sqrt(mean(h^2) + eps).  Returns (q, scale, scale_row, h): the codes are those of h * weight, scale_row
-    [rows, 1] fp32 goes to matmul and gated_matmul; h is the next residual (None without one).
+    [rows, 1] fp32 goes to matmul and gated_matmul; h is the next residual (None without one).  A row with a NaN, or whose squares' sum passes fp32's
+    range, has the factor NaN.
 
     x, residual [rows, cols] fp16 or bf16 (rows may lie apart), weight [cols] of the same type."""
     op = "rms_norm_quantize"
@@ -196,7 +197,8 @@ def matmul(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_
 
     x, x_scale: 4- or 8-bit rows [M, K] as quantize, rms_norm_quantize, silu_mul_quantize and gated_matmul give them; weight [N, K/2] uint8 and
     weight_scale [N, K/32] 4-bit ones; scale_row [M] or [M, 1] fp32 (rms_norm_quantize); bias [N] of dtype.  K is a multiple of 32; x and weight start
-    at a multiple of 16 bytes.  Sums in fp32, one rounding; 8-bit rows' products are aligned to the largest of 64 or 128 of them first."""
+    at a multiple of 16 bytes.  Sums in fp32, one rounding; 8-bit rows' products are
+    aligned to the largest of eight at a time first, and cut off 2^-13 below it."""
     op = "matmul"
     out = L.front().mx_matmul(x, x_scale, weight, weight_scale, dtype, scale_row, bias)
     if out is not None:
@@ -216,7 +218,7 @@ def gated_matmul(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w
                  scale_row: torch.Tensor = None, bits: int = 4):
     """The first half of a gated feed-forward block in one launch: (q, scale) [M, inner] of silu(gate) * up, gate = x weight[:inner]^T, up = x
     weight[inner:]^T (times scale_row), both rounded to dtype.  weight [2 * inner, K/2] is gate's and up's one after the other, inner a multiple of
-    32; everything else as in matmul.  The codes are those that silu_mul_quantize makes of matmul's result where K is not split there."""
+    32; everything else as in matmul.  The codes are those that silu_mul_quantize makes of matmul's result, up to the order of the sums over K."""
     op = "gated_matmul"
     out = L.front().mx_gated_matmul(x, x_scale, weight, weight_scale, dtype, scale_row, bits)
     if out is not None:
@@ -277,6 +279,8 @@ def rotate_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torc
     _expect(op, "positions", positions, torch.int64, (tokens,))
     _expect(op, "slots", slots, torch.int64, (tokens,))
     bits = {}
+    if k_cache.dim() != 3:
+        raise RuntimeError(f"{op}: expected k_cache to have three dimensions, got {tuple(k_cache.shape)}")
     for name, cache, scale in (("k", k_cache, k_scale), ("v", v_cache, v_scale)):
         bits[name] = _bits_of(op, f"{name}_cache", cache)
         _expect(op, f"{name}_cache", cache, cache.dtype, (k_cache.size(0), kv_heads, size // 2 if bits[name] == 4 else size))
