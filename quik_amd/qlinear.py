@@ -25,12 +25,12 @@ from torch import Tensor
 from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import _lib as L
-from . import asymmetric, matmul, symmetric
+from . import asymmetric, matmul, microscaled, symmetric
 from ._lib import device_guard
 
 _front = None     # the native front end; set when the first plan is made (only plans lead into it)
 
-__all__ = ["MixedQLinear", "SharedQuantizedInput", "FusedMixedQLinearGroup", "Linear4bit", "Linear8bit", "GroupLinear4bit",
+__all__ = ["MixedQLinear", "SharedQuantizedInput", "FusedMixedQLinearGroup", "Linear4bit", "Linear8bit", "GroupLinear4bit", "MicroscaledLinear4bit",
            "pack_to_i4", "two_compl"]
 
 
@@ -862,3 +862,68 @@ class GroupLinear4bit(torch.nn.Module):
             rows = rows.clone()
         out = matmul.int4GroupMatmul(rows, self.int_weight, self.scales, self.group_size, zeros=self.zeros, scale_row=scale, bias=self.bias)
         return out.reshape(*x.shape[:-1], self.out_features)
+
+
+class MicroscaledLinear4bit(torch.nn.Module):
+    """4-bit floating-point weights in blocks of 32 input columns with a power of two each (quik.microscaled), and activations in such blocks of
+    `act_bits` (4 or 8).
+
+    weight [out, in/2] and weight_scale [out, in/32] are uint8.  forward(x) takes 16-bit activations of `dtype` and quantizes them; forward(q,
+    scale, scale_row) rows as microscaled.quantize, rms_norm_quantize and gated_matmul give them.  gated(...) takes the same where the
+    weight is the gates' rows and behind them up's, and returns the activated rows (q, scale) for the next product.  No counterpart in the reference."""
+
+    def __init__(self, in_features, out_features, act_bits=4, bias=False, dtype=torch.float16):
+        super().__init__()
+        if in_features <= 0 or in_features % microscaled.BLOCK:
+            raise ValueError(f"MicroscaledLinear4bit: in_features must be a multiple of {microscaled.BLOCK}, got {in_features}")
+        if act_bits not in (4, 8):
+            raise ValueError(f"MicroscaledLinear4bit: act_bits must be 4 or 8, got {act_bits}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.act_bits = act_bits
+        self.dtype = dtype
+        self.register_buffer('weight', torch.zeros((out_features, in_features // 2), dtype=torch.uint8))
+        self.register_buffer('weight_scale', torch.zeros((out_features, in_features // microscaled.BLOCK), dtype=torch.uint8))
+        self.register_buffer('bias', torch.zeros((out_features,), dtype=dtype) if bias else None)
+
+    @staticmethod
+    @torch.no_grad()
+    def from_float(module, act_bits=4):
+        """The nearest codes of a torch.nn.Linear on the GPU (an fp32 module's weight is rounded to fp16 first)."""
+        w = module.weight
+        dtype = w.dtype if w.dtype in (torch.float16, torch.bfloat16) else torch.float16
+        mod = MicroscaledLinear4bit(module.in_features, module.out_features, act_bits, module.bias is not None, dtype).to(w.device)
+        mod.weight, mod.weight_scale = microscaled.quantize(w.detach().to(dtype), 4)
+        if module.bias is not None:
+            mod.bias.copy_(module.bias)
+        return mod
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.dtype = fn(torch.empty(0, dtype=self.dtype)).dtype   # (.half(), .to(torch.bfloat16): the results' type goes with the bias)
+        return self
+
+    def _rows(self, x, scale, scale_row):
+        lead = x.shape[:-1]
+        if scale is None:
+            if scale_row is not None:
+                raise ValueError("MicroscaledLinear4bit: scale_row belongs to rows of codes, which come with their scale")
+            rows = x.reshape(-1, x.shape[-1])
+            if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+                rows = rows.contiguous()
+            x, scale = microscaled.quantize(rows, self.act_bits)
+        else:
+            x, scale = x.reshape(-1, x.shape[-1]), scale.reshape(-1, scale.shape[-1])
+        return lead, x, scale
+
+    def forward(self, x, scale=None, scale_row=None):
+        lead, q, scale = self._rows(x, scale, scale_row)
+        out = microscaled.matmul(q, scale, self.weight, self.weight_scale, self.dtype, scale_row, self.bias)
+        return out.reshape(*lead, self.out_features)
+
+    def gated(self, x, scale=None, scale_row=None, bits=None):
+        if self.bias is not None:
+            raise ValueError("MicroscaledLinear4bit: the gated product has no bias")
+        lead, q, scale = self._rows(x, scale, scale_row)
+        q, scale = microscaled.gated_matmul(q, scale, self.weight, self.weight_scale, self.dtype, scale_row, self.act_bits if bits is None else bits)
+        return q.reshape(*lead, q.shape[-1]), scale.reshape(*lead, scale.shape[-1])
