@@ -197,8 +197,7 @@ def matmul(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_
 
     x, x_scale: 4- or 8-bit rows [M, K] as quantize, rms_norm_quantize, silu_mul_quantize and gated_matmul give them; weight [N, K/2] uint8 and
     weight_scale [N, K/32] 4-bit ones; scale_row [M] or [M, 1] fp32 (rms_norm_quantize); bias [N] of dtype.  K is a multiple of 32; x and weight start
-    at a multiple of 16 bytes.  Sums in fp32, one rounding; 8-bit rows' products are
-    aligned to the largest of eight at a time first, and cut off 2^-13 below it."""
+    at a multiple of 16 bytes.  Sums in fp32, one rounding."""
     op = "matmul"
     out = L.front().mx_matmul(x, x_scale, weight, weight_scale, dtype, scale_row, bias)
     if out is not None:

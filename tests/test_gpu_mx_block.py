@@ -66,15 +66,14 @@ def inputs(rows, hidden, dtype, seed=1):
 @pytest.mark.parametrize("rows", [1, 7, 16, 40, 150])
 def test_block(rows, bits, dtype):
     """Each step against 64 bits, from what the steps before it left.  Sums are exact but for `near`, relative to the result's norm: a rounding to 16
-    bits (eps / 2), the norm's factor, and 8-bit products' alignment (7 * 2^-13 of the terms' magnitudes, whose sum is some sqrt(K) <= 38 of the
-    result's norm).  A value that is off by d goes to the neighbouring code with the probability d / step, so that behind a quantization the
+    bits (eps / 2) and the norm's factor.  A value that is off by d goes to the neighbouring code with the probability d / step, so that behind a quantization the
     squares of the differences are d * step of the values' own, step 2^-1 and 2^-3 (4 and 8 bits: a step over the smallest number that has it)."""
     block = Block(512, 8, 2, 64, 1376, bits, dtype)
     x, residual, positions, slots = inputs(rows, 512, dtype)
     out, last, keys, values, h, qkv, queries, a, gated = (t.double().cpu() for t in block.run(x, residual, positions, slots))
     heads, kv_heads, size = block.shape
     gains, cos, sin = [g.double().cpu() for g in block.gains], block.cos.double().cpu()[positions.cpu()], block.sin.double().cpu()[positions.cpu()]
-    near = torch.finfo(dtype).eps / 2 + 2.0 ** -18 + (38 * 7 * 2.0 ** -13 if bits == 8 else 0)
+    near = torch.finfo(dtype).eps / 2 + 2.0 ** -18
     apart = lambda got, want: ((got - want).norm() / want.norm()).item()
 
     def norm(t, gain):  # (the codes are those of t * gain, the row's factor is apart from them)

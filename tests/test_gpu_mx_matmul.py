@@ -21,11 +21,11 @@ def operands(seed, M, N, K, bits, spread=3):
 
 
 def allowed(x, w, y, bits, dtype):
-    """The rounding to the type; per instruction of 64 columns an alignment to 2^-24 of its largest term and a rounding of the sum so far, sixteen
-    parts of K joined, row factor and bias; 8 bits: eight products at a time are aligned to 2^-13 of their largest, cut, which the seven others lose."""
+    """The rounding to the type; per instruction of 64 columns (8 bits: two of them) an alignment to 2^-24 of its largest term and a rounding of
+    the sum so far, sixteen parts of K joined, row factor and bias."""
     total = x.abs() @ w.abs().t()
-    steps = -(-x.shape[1] // 64) + 20
-    return torch.finfo(dtype).eps / 2 * y.abs() + 2.0 ** -24 * (1 if dtype == torch.float16 else 0) + total * (steps * 2.0 ** -24 + (7 * 2.0 ** -13 if bits == 8 else 0))
+    steps = -(-x.shape[1] // 64) * (bits // 4) + 20
+    return torch.finfo(dtype).eps / 2 * y.abs() + 2.0 ** -24 * (1 if dtype == torch.float16 else 0) + total * (steps * 2.0 ** -24)
 
 
 SHAPES = [(1, 1, 32), (1, 5, 64), (1, 4096, 4096), (1, 1000, 11008), (2, 33, 96), (4, 64, 128), (5, 257, 160), (8, 8200, 512), (9, 100, 1056), (16, 300, 4544),
@@ -47,6 +47,28 @@ def test_product(M, N, K, bits):
     y = y * row.double() + bias.double()
     limit = allowed(x * row.double(), w, y, bits, dtype) + 2.0 ** -23 * y.abs()
     assert ((out.cpu().double() - y).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("M", [1, 8, 13, 40, 100, 300])
+def test_all_of_an_8_bit_code_counts(M):
+    """Numbers over all of e4m3's range next to each other: the largest cancel each other, and what remains of each sixteen is a sum of multiples of 2^-10
+    below 2^12 apart, which is a number of fp32."""
+    K, N = 256, 70
+    gen = torch.Generator().manual_seed(M)
+    v = torch.randint(0, 120, (M, K), generator=gen)
+    e = torch.full((M, K // 32), 127)
+    v[:, 0::16], v[:, 15::16] = 126, 254                      # 448 and -448
+    small = torch.randint(1, 16, (M, K // 4), generator=gen)  # multiples of 2^-9 up to 2^-5
+    v[:, 1::16] = small[:, :K // 16]
+    v[:, 2::16] = 128 + small[:, K // 16:K // 8]
+    for i in range(3, 15):
+        v[:, i::16] = torch.randint(0, 64, (M, K // 16), generator=gen)   # below 2
+    w = torch.randint(0, 16, (N, K), generator=gen)
+    w[:, 0::16] = w[:, 15::16] = 7                            # 6
+    we = torch.full((N, K // 32), 127)
+    y = P.numbers(v, e, 8) @ P.numbers(w, we, 4).t()
+    out = ms().matmul(P.pack(v, 8).to(DEV), e.to(torch.uint8).to(DEV), P.pack(w, 4).to(DEV), we.to(torch.uint8).to(DEV), torch.float16)
+    assert torch.equal(out.cpu(), y.to(torch.float16))
 
 
 @pytest.mark.parametrize("bits", [4, 8])
