@@ -29,46 +29,37 @@ struct MxRows {
 
 enum FlatOp { kPlain, kGated };
 
-// Lanes of all rows one after the other, V * 256 per workgroup.  (rows * lanes < 2^31 per launch)
-template <bool BF16, FlatOp OP, int BITS, bool WIDE, int V>
+// Lanes of all rows one after the other, one each: chunks of several per thread, requested together, take longer (us, four per thread and this: quantize
+// 2048 x 8192, 4 bits, 10.7, 9.3 (4.6 TB/s, a copy's are 5.1), 8192 x 4096 19.5, 17.2; two and this: silu_mul 2048 x 13824, 8 bits, 28.6, 26.3 (5.4 TB/s)).
+// (rows * lanes < 2^31 per launch)
+template <bool BF16, FlatOp OP, int BITS, bool WIDE>
 __global__ __launch_bounds__(256) void mx_flat_kernel(MxRows p) {
-  const uint32_t first = blockIdx.x * (256u * V) + threadIdx.x, all = static_cast<uint32_t>(p.rows) * p.by_lanes.d, blocks = p.by_lanes.d / 4;
-  alignas(16) uint16_t va[V][8], vb[V][8];
-  uint32_t row[V], c[V];
-  int left[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t at = first + 256u * j;
-    row[j] = p.by_lanes(at < all ? at : 0, c[j]);
-    const int64_t rest = p.cols - static_cast<int64_t>(c[j]) * 8;
-    left[j] = at >= all ? 0 : rest < 8 ? static_cast<int>(rest) : 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) va[j][e] = vb[j][e] = 0;
-    if (left[j] > 0) {
-      load_eight<WIDE>(p.a + row[j] * p.pitch_a + c[j] * int64_t{8}, left[j], va[j]);
-      if constexpr (OP == kGated) load_eight<WIDE>(p.b + row[j] * p.pitch_b + c[j] * int64_t{8}, left[j], vb[j]);
-    }
+  const uint32_t at = blockIdx.x * 256u + threadIdx.x, all = static_cast<uint32_t>(p.rows) * p.by_lanes.d, blocks = p.by_lanes.d / 4;
+  uint32_t c;
+  const uint32_t row = p.by_lanes(at < all ? at : 0, c);
+  const int64_t rest = p.cols - static_cast<int64_t>(c) * 8;
+  const int left = at >= all ? 0 : rest < 8 ? static_cast<int>(rest) : 8;
+  alignas(16) uint16_t va[8] = {}, vb[8] = {};
+  if (left > 0) {
+    load_eight<WIDE>(p.a + row * p.pitch_a + c * int64_t{8}, left, va);
+    if constexpr (OP == kGated) load_eight<WIDE>(p.b + row * p.pitch_b + c * int64_t{8}, left, vb);
   }
+  float v[8];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    float v[8];
+  for (int e = 0; e < 8; ++e) v[e] = OP == kGated ? gated(to_f32<BF16>(va[e]), to_f32<BF16>(vb[e])) : to_f32<BF16>(va[e]);
+  if constexpr (OP == kGated) {
+    uint32_t low = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = OP == kGated ? gated(to_f32<BF16>(va[j][e]), to_f32<BF16>(vb[j][e])) : to_f32<BF16>(va[j][e]);
-    if constexpr (OP == kGated) {
-      uint32_t low = 0;
+    for (int e = 0; e < 8; ++e) low = umax(low, __float_as_uint(to_f32<BF16>(va[e])));
+    if (low > kFarBits) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) low = umax(low, __float_as_uint(to_f32<BF16>(va[j][e])));
-      if (low > kFarBits) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float gate = to_f32<BF16>(va[j][e]);
-          if (__float_as_uint(gate) > kFarBits) v[e] = gated_far(gate, to_f32<BF16>(vb[j][e]));
-        }
+      for (int e = 0; e < 8; ++e) {
+        const float gate = to_f32<BF16>(va[e]);
+        if (__float_as_uint(gate) > kFarBits) v[e] = gated_far(gate, to_f32<BF16>(vb[e]));
       }
     }
-    store_block<BITS, WIDE>(v, left[j], p.q + (row[j] * p.cols + c[j] * int64_t{8}) * BITS / 8, p.scale + row[j] * static_cast<int64_t>(blocks) + c[j] / 4,
-                            c[j] % 4 == 0);
   }
+  store_block<BITS, WIDE>(v, left, p.q + (row * p.cols + c * int64_t{8}) * BITS / 8, p.scale + row * static_cast<int64_t>(blocks) + c / 4, c % 4 == 0);
 }
 
 template <bool BF16, bool ADD, int BITS, bool WIDE>
@@ -187,19 +178,13 @@ int64_t lanes_of(int64_t cols) { return (cols + kMxBlock - 1) / kMxBlock * 4; }
 
 template <bool BF16, FlatOp OP, int BITS>
 int launch_flat(MxRows p, bool wide, hipStream_t st) {
-  constexpr int V = OP == kGated ? 2 : 4;
   const int64_t lanes = lanes_of(p.cols), most = kLanes / lanes, all = p.rows;
   p.by_lanes = divide_by(lanes);
   for (int64_t first = 0; first < all; first += most) {
     p.rows = all - first < most ? all - first : most;
-    // (few lanes: one chunk per thread spreads them over more CUs)
-    const int64_t total = p.rows * lanes;
-    const bool few = total <= num_cus() * int64_t{256} * V;
-    const dim3 grid(static_cast<unsigned>((total + 256 * (few ? 1 : V) - 1) / (256 * (few ? 1 : V))));
-    if (wide && few) hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, true, 1>), grid, dim3(256), 0, st, p);
-    else if (wide) hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, true, V>), grid, dim3(256), 0, st, p);
-    else if (few) hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, false, 1>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, false, V>), grid, dim3(256), 0, st, p);
+    const dim3 grid(static_cast<unsigned>((p.rows * lanes + 255) / 256));
+    if (wide) hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((mx_flat_kernel<BF16, OP, BITS, false>), grid, dim3(256), 0, st, p);
     if (int rc = check_launch()) return rc;
     p.a += most * p.pitch_a;
     if (p.b) p.b += most * p.pitch_b;
@@ -243,7 +228,9 @@ int launch_read(MxRead p, bool wide, hipStream_t st) {
   for (int64_t first = 0; first < all; first += most) {
     p.count = all - first < most ? all - first : most;
     const int64_t total = p.count * p.heads * lanes;
-    const bool few = total <= num_cus() * int64_t{256} * V;
+    // Four chunks per thread for the largest calls: us, one and four, 32768 rows of 8 x 128, 8 bits, 19.1, 18.6 (101 MB, 5.4 TB/s of which codes still
+    // lie in the cache), 4096 of 40 x 128, 4 bits, 12.4, 12.0; below one spreads the lanes over more CUs, 2048 x 8192, 4 bits, 9.9, 10.4, 777 x 5120 4.7, 5.2.
+    const bool few = total <= num_cus() * int64_t{256} * 32;
     const dim3 grid(static_cast<unsigned>((total + 256 * (few ? 1 : V) - 1) / (256 * (few ? 1 : V))));
     if (wide && few) hipLaunchKernelGGL((mx_read_kernel<BF16, BITS, true, 1>), grid, dim3(256), 0, st, p);
     else if (wide) hipLaunchKernelGGL((mx_read_kernel<BF16, BITS, true, V>), grid, dim3(256), 0, st, p);
