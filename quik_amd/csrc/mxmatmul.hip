@@ -548,23 +548,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
       bytes_of[i] = p.x;
     }
   }
-  // the first two stages at once: a workgroup waits for memory one time before it begins
-  u32x4 second[S::kLoads];
 #pragma unroll
   for (int i = 0; i < S::kLoads; ++i) load(staged_of[0], first, i);
-#pragma unroll
-  for (int i = 0; i < S::kLoads; ++i) load(second, there(first + 1), i);
   write_bytes(0, nb < 16 ? first * 8 : less);
   less = load_bytes(1);
 #pragma unroll
-  for (int i = 0; i < S::kLoads; ++i) {
-    write(staged_of[0], first, i);
-    load(staged_of[0], there(first + 2), i);
-  }
-  __builtin_amdgcn_sched_barrier(0);
+  for (int d = 0; d < 2; ++d) {
 #pragma unroll
-  for (int i = 0; i < S::kLoads; ++i) write(second, first + 1, i);
-  __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < S::kLoads; ++i) {
+      write(staged_of[0], first + d, i);
+      load(staged_of[0], there(first + d + 1), i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < RM + RN; ++n) read_bytes(first, n);
