@@ -119,6 +119,9 @@ __device__ __forceinline__ int turn_of(int row) {
 // turn and add their sums through LDS at a tile's end.  Operands and bytes come by direct copies, D - 1 blocks ahead and on into the next tile,
 // into a ring of the wave's own (no barrier but at a tile's end).  Up to eight rows of 8-bit codes are sixteen columns: their codes from 2 up, and behind
 // them those below, whose sums are added in the end.  Gated: matrix tiles 0 .. FT / 2 - 1 are gates, the others the same columns of up.
+// Bound by the weights' stream: 1 x 8192 -> 28672 24.7 us, 5.1 TB/s (a copy's rate), with 8-bit rows 27.3, of which the codes' parting is 1.5; 1 x 13824 -> 5120 8.9 us,
+// 4.2 TB/s; 1 x 4096 -> 4096 4.2 us, a launch and three trips to memory one after the other.  Gated 4 x 8192 -> 57344 48.6 us, 5.1 TB/s, 1 x 4096 -> 22016 13.1:
+// 344 tiles of 32 columns for 256 CUs (smaller rings, two workgroups per CU, 13.8 .. 15.1).
 template <int XB, int TR, int FT, int W, int D, int STEPS, bool TAIL>
 struct RingShape {
   static constexpr int kPw = 4 * STEPS, kPx = kPw * (XB / 4), kPlanes = TAIL ? 4 : 1;
@@ -335,6 +338,10 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 // at any byte.  Four bytes of a stage, those of this lane's group, are one operand for it.  Bytes behind the end of K are 0 on both sides:
 // whatever codes stand there, a product of 2^-254 does not change a sum.
 // Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
+// 8-bit rows: the codes of the next 64 columns are taken apart behind the products of these, five vector instructions per four codes, in the places where
+// the matrix unit is busy.  So a wave has one row of matrix tiles and up to four of them in it (with two rows of two, each wave takes twice as many
+// codes apart: 2048 x 8192 -> 28672 782 us, this 645; its products are 72 % of the SIMDs' cycles, at a clock of 1.76 GHz).
+// 4 bits: 2048 x 8192 -> 28672 277 us, 3.5 PFLOP/s, the matrix unit busy for 43 % of the cycles, at 1.9 GHz; 64 x 5120 -> 27648 gated 22.2 us, 3.6 TB/s.
 template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
   // Stages on their way to registers: two where the results leave room, with their loads dealt to three quarters of a stage (us, one on its way and
