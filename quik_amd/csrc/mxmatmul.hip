@@ -773,8 +773,15 @@ __global__ __launch_bounds__(256) void mx_join_kernel(MxArgs p) {
   if (at >= p.M * quads) return;
   const int64_t m = at / quads, n = at % quads * 4;
   const float *from = p.partial + m * pitch + n;
+  const int64_t part = p.M * pitch;
   f32x4 v = *reinterpret_cast<const f32x4 *>(from);
-  for (int i = 1; i < p.splits; ++i) v += *reinterpret_cast<const f32x4 *>(from + i * p.M * pitch);
+  int i = 1;
+  for (; i + 2 < p.splits; i += 3) {  // (three requested together)
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(from + i * part), b = *reinterpret_cast<const f32x4 *>(from + (i + 1) * part),
+                c = *reinterpret_cast<const f32x4 *>(from + (i + 2) * part);
+    v = v + a + b + c;
+  }
+  for (; i < p.splits; ++i) v += *reinterpret_cast<const f32x4 *>(from + i * part);
   const float row = p.row ? p.row[m] : 1.0f;
   for (int r = 0; r < 4 && n + r < p.N; ++r) {
     float y = p.row ? v[r] * row : v[r];
@@ -858,30 +865,33 @@ struct TilePlan {
   int rows, cols, slots;
   double one, full, round;
 };
-constexpr TilePlan kPlans[2][4] = {{{32, 128, 3, 0.45, 1.2, 2.0}, {64, 128, 2, 0.58, 0.98, 2.0}, {128, 128, 2, 0.76, 1.5, 2.0}, {256, 256, 1, 1.75, 2.0, 5.0}},
+constexpr TilePlan kPlans[2][4] = {{{32, 128, 3, 0.5, 1.2, 2.0}, {64, 128, 2, 0.58, 0.98, 2.0}, {128, 128, 2, 0.76, 1.5, 2.0}, {256, 256, 1, 1.75, 2.0, 5.0}},
                                    {{32, 128, 2, 0.85, 1.5, 2.0}, {64, 128, 2, 1.08, 1.8, 2.0}, {128, 128, 1, 1.6, 1.65, 2.0}, {128, 256, 1, 2.35, 2.8, 4.0}}};
 struct Choice {
   int plan, splits;
 };
-// The cheapest tiles and K split: the rounds of workgroups, no less than the weights from memory, and for a split the second launch and its sums, written
-// and read.  us, as the rule has it and measured (the next best measured): 64 x 4096 -> 4096, 32 rows, 11.1, 10.8 (64 rows, K in 4: 12.1); 64 x 13824 -> 5120, 64
-// rows, K in 6, 17.3, 17.0 (32 rows 18.5); 300 x 4544 -> 4544, 64 rows, 14.9, 14.9 (128 rows 18.2); 777 x 5120 -> 5120, 128 rows, 34.5, 29.7 (64 rows 33.2);
-// 2048 x 4096 -> 4096, 128 rows, 28.5, 28.7 (256 rows 34.2); 2048 x 8192 -> 28672, 256 rows, 278, 277 (128 rows 333);
-// 8 bit: 300 x 4544 -> 4544, 64 rows, 23.9, 23.6 (128 rows 29.0), 777 x 5120 -> 5120, 128 x 256, 53.5, 53.1 (64 rows 58.7), 1024 x 4096 -> 4096, 128 x 128, 32.1,
-// 32.0 (64 rows 36.3), 2048 x 8192 -> 28672, 128 x 256, 658, 645 (128 x 128 757).
+// The cheapest tiles and K split: the rounds of workgroups, no less than the weights from memory (of whose rate each CU has its share), and for a split the
+// second launch and its sums, written and read (from the cache that all dies share); a part is four stages at least (64 x 4096 -> 4096, in parts of two 14.5,
+// of four 11.1).  us, as the rule has it and measured (the next best measured):
+// 64 x 13824 -> 5120, 64 rows, K in 6, 16.9, 17.2 (32 rows, K in 3: 18.5); 64 x 8192 -> 8192, 64 rows, K in 4, 16.4, 16.1 (32 rows, K in 2: 16.8); 32 x 28672 -> 8192, 32 rows, K in
+// 4, 35, 30.1 (in 3, 192 workgroups: 42.2); 64 x 4096 -> 11008, 32 rows, 12.5, 11.3 (64 rows 13.0); 128 x 5120 -> 13824, 64 rows, 16.1, 18.8 (128 rows 22.2); 300 x 4544 -> 4544,
+// 64 rows, 14.9, 15.3 (128 rows 18.1); 300 x 13824 -> 5120, 128 rows, K in 2, 31, 32.0 (64 rows 37.6); 777 x 5120 -> 5120, 128 rows, 34.5, 30.0 (64 rows 33.6); 2048 x 8192 ->
+// 28672, 256 rows, 278, 277 (128 rows 333).  8 bit: 300 x 4544 -> 4544, 64 rows, 23.9, 23.6 (128 rows 29.0); 300 x 13824 -> 5120, 128 x 256, K in 4, 48, 54.1 (128 x 128 55.7);
+// 777 x 5120 -> 5120, 128 x 256, 53.5, 53.1 (64 rows 58.7); 1024 x 4096 -> 4096, 128 x 128, 32.1, 32.0 (64 rows 36.3); 2048 x 8192 -> 28672, 128 x 256, 658, 645 (128 x 128 757).
 Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
   Choice best{1, 1};
   double least = 1e30;
   const int64_t cus = num_cus(), stages = (K + 255) / 256;
-  const double weights = static_cast<double>(N) * static_cast<double>(K) * 0.53125 / 4.6e6 + 1.0;
+  const double weights = static_cast<double>(N) * static_cast<double>(K) * 0.53125 / 4.6e6;
   for (int i = 0; i < 4; ++i) {
     const TilePlan &t = kPlans[x_bits == 8][i];
     const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
-    for (int s = 1; s <= (may_split ? 16 : 1) && (s == 1 || 2 * s <= stages); ++s) {
+    for (int s = 1; s <= (may_split ? 16 : 1) && (s == 1 || 4 * s <= stages); ++s) {
       const int64_t groups = tiles * s, rounds = groups / (cus * t.slots), rest = groups % (cus * t.slots), deep = (stages + s - 1) / s;
       double us = static_cast<double>(rounds) * (static_cast<double>(deep) * t.full + t.round);
       if (rest) us += static_cast<double>(deep) * (rest <= cus ? t.one : t.full) + t.round;
-      us = (us > weights ? us : weights) + 2.5 + (s > 1 ? 3.5 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8e-6 / 5.0 : 0.0);
+      const double share = 1.05 * static_cast<double>(groups) / static_cast<double>(cus), stream = weights / (share < 1.0 ? share : 1.0) + 1.0;
+      us = (us > stream ? us : stream) + 2.5 + (s > 1 ? 3.5 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 1.1e-6 : 0.0);
       if (us < least) {
         least = us;
         best = Choice{i, s};
