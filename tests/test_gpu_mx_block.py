@@ -255,3 +255,36 @@ def test_tokens_and_rows_of_a_product_past_one_launch(bits):
     assert torch.equal(out[-40:], ms().matmul(kind(x[-40:].clone()), s[-40:].clone(), w, ws)) and not out[:-40].any()
     del x, s, out
     torch.cuda.empty_cache()
+
+
+def test_tokens_past_one_launch():
+    n = (2 ** 31 - 1) // 256 + 6
+    gen = torch.Generator(DEV).manual_seed(4)
+    x = torch.randn(n, 1, 2, device=DEV, generator=gen).half()
+    cos, sin = torch.full((3, 1), 0.6, device=DEV), torch.full((3, 1), 0.8, device=DEV)
+    cos[2], sin[2] = 0.0, 1.0
+    positions, slots = torch.zeros(n, dtype=torch.int64, device=DEV), torch.full((n,), -1, dtype=torch.int64, device=DEV)
+    positions[-4:], slots[-4:] = 2, torch.arange(4, device=DEV)
+    cache = [torch.full(s, 9, dtype=torch.uint8, device=DEV) for s in ((6, 1, 1), (6, 1, 1), (6, 1, 1), (6, 1, 1))]
+    out = ms().rotate_to_cache(x, x, x, cos, sin, positions, slots, *cache)
+    tail = [torch.full_like(t, 9) for t in cache]
+    assert torch.equal(out[-9:], ms().rotate_to_cache(x[-9:], x[-9:], x[-9:], cos, sin, positions[-9:], slots[-9:], *tail))
+    assert all(torch.equal(a, b) for a, b in zip(cache, tail)) and (cache[0][:4] != 9).any() and all((t[4:] == 9).all() for t in cache)
+    a, b = x[:1000, 0].double().unbind(1)
+    assert (out[:1000, 0].double() - torch.stack((0.6 * a - 0.8 * b, 0.6 * b + 0.8 * a), 1)).abs().max() <= 2.0 ** -10 * 4
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_the_sum_over_one_of_its_terms(over, bits):
+    """The C entry point takes x or the residual as the place of their sum; bf16 rows of tiny numbers are read again for their squares."""
+    from quik_amd import _lib as L
+    x, r, w = torch.randn(5, 200, device=DEV).bfloat16(), torch.randn(5, 200, device=DEV).bfloat16(), torch.rand(200, device=DEV).bfloat16()
+    x[3], r[3] = x[3] * 2.0 ** -70, r[3] * 2.0 ** -70
+    want = ms().rms_norm_quantize(x, w, 0.0, r, bits)
+    q, s, f = (torch.empty_like(t) for t in want[:3])
+    place = x if over == "x" else r
+    L.check(L.load().quik_mx_rms_norm_quantize(L.ptr(x), 200, L.ptr(r), 200, L.ptr(w), 0.0, L.dtype_id(x, "norm", allow_bf16=True), 5, 200, bits, L.ptr(place),
+                                               L.ptr(q), L.ptr(s), L.ptr(f), L.stream()), "norm")
+    for a, b in zip((q, s, f, place), want):
+        assert torch.equal(a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b)

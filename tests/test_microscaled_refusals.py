@@ -204,3 +204,12 @@ def test_heads_shapes_types_and_layouts():
                          ({"k_cache": c8.transpose(0, 1)}, "contiguous")):
         with pytest.raises(RuntimeError, match=word):
             ms.rotate_to_cache(**{**good, **change})
+
+
+def test_the_typed_stub_describes_the_module():
+    import ast
+    import inspect
+    import pathlib
+    stub = ast.parse((pathlib.Path(quik.__file__).parent / "_C" / "microscaled.pyi").read_text())
+    given = {f.name: [a.arg for a in f.args.args] for f in stub.body if isinstance(f, ast.FunctionDef)}
+    assert given == {name: list(inspect.signature(getattr(ms, name)).parameters) for name in ms.__all__}
