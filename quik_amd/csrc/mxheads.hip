@@ -183,7 +183,9 @@ int launch_heads(const HeadArgs &p, int64_t tokens, bool wide, hipStream_t st) {
   HeadArgs a = p;
   constexpr int kGroups = 256 / L;
   const int64_t most = (p.q_heads + 2 * static_cast<int64_t>(p.kv_heads) + kGroups - 1) / kGroups, wanted = (4 * num_cus() + tokens - 1) / tokens;
-  a.splits = static_cast<int>(wanted < most ? wanted : most);
+  // A workgroup per round of heads where all of them run at once; more than that wait for their token's position and angles once more each (us, the heads of a
+  // token dealt to four per CU, and one round each: 300 tokens of 64 + 2 * 8 heads of 128 7.8, 5.8; 1024 of 40 + 2 * 40 12.3, 17.0).
+  a.splits = static_cast<int>(tokens * most <= 8 * num_cus() || wanted >= most ? most : wanted);
   const int64_t per_launch = (INT32_MAX / 256) / a.splits;
   for (int64_t first = 0; first < tokens; first += per_launch) {
     const int64_t n = tokens - first < per_launch ? tokens - first : per_launch;

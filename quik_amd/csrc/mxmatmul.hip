@@ -38,12 +38,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t mx_bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 
-// a pointer that is the same for the wave, in scalar registers
-__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))), hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)));
-  return reinterpret_cast<const uint8_t *>(hi << 32 | lo);
-}
 // one byte per lane: it lands in the low byte of the four at LDS address m0 + 4 i (the others are not to be read)
 __device__ __forceinline__ void dma_load_u8(const void *sbase, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" : : "s"(lds_addr), "v"(voff), "s"(sbase) : "memory", "m0");
