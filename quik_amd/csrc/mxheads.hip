@@ -49,7 +49,10 @@ __device__ __forceinline__ void put(const float (&v)[8], int left, uint8_t *code
 
 // L lanes per head, the power of two from four per block up.  WHOLE: every column turns, in chunks of eight that turn with each other, at 16-byte
 // addresses; the other instance takes every size, element by element where a column's fellow is concerned.
-template <bool BF16, int L, bool WHOLE>
+// FOLD: a token's angles are multiplied with the norms' weights before its heads, for workgroups that go through many (us, as numbers are normed and
+// this: 4096 tokens of 64 + 2 * 8 heads of 128, five rounds of heads each, 46.1, 41.3; of 32 + 2 * 32 46.0, 42.1; 300
+// tokens, one round, 5.9, 7.1).
+template <bool BF16, int L, bool WHOLE, bool FOLD>
 __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
   constexpr int kGroups = 256 / L;
   const int64_t token = blockIdx.x / static_cast<uint32_t>(p.splits);
@@ -94,6 +97,23 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
       }
     }
   }
+  float weight_q[FOLD ? 2 : 1][8], weight_k[FOLD ? 2 : 1][8];
+  if constexpr (FOLD) {
+    auto weigh = [&](const uint16_t *gain, float (&to)[2][8]) {
+      alignas(16) uint16_t g[8] = {}, h[8] = {};
+      if (gain && left > 0) {
+        load_eight<true>(gain + 8 * c, left, g);
+        load_eight<true>(gain + with[0], 8, h);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        to[0][e] = gain ? own[e] * to_f32<BF16>(g[e]) : own[e];
+        to[1][e] = gain ? other[e] * to_f32<BF16>(h[e]) : other[e];
+      }
+    };
+    weigh(p.q_gain, weight_q);
+    weigh(p.k_gain, weight_k);
+  }
   const int all = p.q_heads + 2 * p.kv_heads;
   const int64_t base_q = token * p.pitch_q, base_k = token * p.pitch_k, base_v = token * p.pitch_v;
   for (int item = split * kGroups + threadIdx.x / L; item < all; item += p.splits * kGroups) {
@@ -137,7 +157,7 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
         if (square == 0.0f && p.eps == 0.0f) f = 0.0f;  // (a head of zeros)
         if (!(square < __builtin_inff())) f = __builtin_nanf("");
         alignas(16) uint16_t g[8] = {}, h[8] = {};
-        if (left > 0) {
+        if (!FOLD && left > 0) {
           load_eight<WHOLE>(gain + 8 * c, left, g);
           if constexpr (WHOLE) {
             load_eight<true>(gain + with[0], 8, h);
@@ -148,13 +168,14 @@ __global__ __launch_bounds__(256) void mx_heads_kernel(HeadArgs p) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = v[e] * lift * f * to_f32<BF16>(g[e]);
-          t[e] = t[e] * lift * f * to_f32<BF16>(h[e]);
+          v[e] = v[e] * lift * f * (FOLD ? 1.0f : to_f32<BF16>(g[e]));
+          t[e] = t[e] * lift * f * (FOLD ? 1.0f : to_f32<BF16>(h[e]));
         }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float turn = v[e] * own[e] + t[e] * other[e];
+        const float a = FOLD ? (is_q ? weight_q[0][e] : weight_k[0][e]) : own[e], b = FOLD ? (is_q ? weight_q[FOLD][e] : weight_k[FOLD][e]) : other[e];
+        const float turn = v[e] * a + t[e] * b;
         v[e] = WHOLE || (e < left && (8 * c + e < turned || !known)) ? turn : v[e];  // (a column that stays is not added 0 * t: t may be an infinity)
       }
       if constexpr (!WHOLE) {
@@ -190,8 +211,10 @@ int launch_heads(const HeadArgs &p, int64_t tokens, bool wide, hipStream_t st) {
   for (int64_t first = 0; first < tokens; first += per_launch) {
     const int64_t n = tokens - first < per_launch ? tokens - first : per_launch;
     const dim3 grid(static_cast<unsigned>(n * a.splits));
-    if (wide) hipLaunchKernelGGL((mx_heads_kernel<BF16, L, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mx_heads_kernel<BF16, L, false>), grid, dim3(256), 0, st, a);
+    const bool fold = wide && (p.q_gain || p.k_gain) && most >= 4 * static_cast<int64_t>(a.splits);
+    if (fold) hipLaunchKernelGGL((mx_heads_kernel<BF16, L, true, true>), grid, dim3(256), 0, st, a);
+    else if (wide) hipLaunchKernelGGL((mx_heads_kernel<BF16, L, true, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mx_heads_kernel<BF16, L, false, false>), grid, dim3(256), 0, st, a);
     if (int rc = check_launch()) return rc;
     a.q += n * p.pitch_q, a.k += n * p.pitch_k, a.v += n * p.pitch_v;
     a.position += n, a.slot += n;

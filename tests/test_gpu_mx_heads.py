@@ -86,6 +86,40 @@ def test_heads(tokens, q_heads, kv_heads, size, half, k_bits, v_bits, norm, dtyp
         assert (t.view(torch.uint8).cpu()[rest] == fill).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("which", ["both", "q", "k"])
+def test_many_heads_of_many_tokens(which, dtype):
+    """So many that a workgroup goes through several rounds of heads; heads of zeros, of tiny numbers and without a number among them."""
+    tokens, q_heads, kv_heads, size, half = 1100, 40, 12, 128, 64
+    gen = torch.Generator().manual_seed(5)
+    qkv = torch.randn(tokens, q_heads + 2 * kv_heads, size, generator=gen).to(dtype)
+    qkv[3, 7], qkv[4, q_heads + 3], qkv[5, 9, 100], qkv[6, q_heads + 1, 2] = 0, 0, float("nan"), float("inf")
+    if dtype == torch.bfloat16:
+        qkv[7] *= 2.0 ** -120
+    q, k, v = qkv.split((q_heads, kv_heads, kv_heads), 1)
+    gains = [(1 + 0.2 * torch.randn(size, generator=gen)).to(dtype) if which in (name, "both") else None for name in "qk"]
+    cos, sin = table(50, half)
+    positions, slots = torch.randint(0, 50, (tokens,), generator=gen), torch.randperm(tokens + 3, generator=gen)[:tokens]
+    (kc, ks), (vc, vs) = empty_cache(tokens + 3, kv_heads, size, 8), empty_cache(tokens + 3, kv_heads, size, 4)
+    dev = [t.unflatten(1, (-1, size)) for t in qkv.flatten(1).to(DEV).split((q_heads * size, kv_heads * size, kv_heads * size), 1)]
+    out = ms().rotate_to_cache(*dev, cos.to(DEV), sin.to(DEV), positions.to(DEV), slots.to(DEV), kc, ks, vc, vs, *(None if g is None else g.to(DEV) for g in gains), 0.0)
+    bad = torch.zeros(tokens, q_heads, dtype=torch.bool)
+    bad[5, 9] = True
+    want, off = turned(q, gains[0], 1e-300, cos[positions], sin[positions])    # (eps 0; a head of zeros is zeros)
+    got = out.cpu().double()
+    if gains[0] is not None:
+        assert got[bad].isnan().all()
+    good = ~bad
+    assert ((got - want).abs() <= off + torch.finfo(dtype).eps / 2 * (want.abs() + off) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134))[good].all()
+    want, off = turned(k, gains[1], 1e-300, cos[positions], sin[positions])
+    keys, scales = kc.view(torch.uint8).cpu()[slots].view(kc.dtype), ks.cpu()[slots]
+    assert (scales[6, 1] == 255).any() if gains[1] is None else (scales[6, 1] == 255).all()
+    keep = torch.ones(tokens, kv_heads, dtype=torch.bool)
+    keep[6, 1] = False
+    check_cached(keys.view(torch.uint8)[keep].view(kc.dtype), scales[keep], want[keep], off[keep] + 2.0 ** -149, 8)
+    check_cached(vc.cpu()[slots], vs.cpu()[slots], v.double(), torch.zeros(()).double(), 4)
+
+
 def simple(tokens=4, heads=2, size=64, bits=8, dtype=torch.float16):
     gen = torch.Generator().manual_seed(1)
     q, k, v = (torch.randn(tokens, heads, size, generator=gen).to(dtype).to(DEV) for _ in range(3))
