@@ -9,7 +9,7 @@
 // All are bound by memory.  A block is four lanes of eight columns, 16 bytes of a 16-bit row each, and its largest magnitude two exchanges between
 // neighbouring lanes: there is nothing to wait for but the load, and a norm stores its codes before it knows the row's factor.
 // us, bytes per us against a copy's 5.1e6: quantize 2048 x 8192, 4 bits, 9.3, 4.6e6; silu_mul 2048 x 13824, 8 bits, 26.3, 5.4e6; norm with a residual 777 x 5120, 4 bits,
-// 8.2, 3.2e6 (one row per workgroup, all at once: loads, then stores), 8192 x 4096 39.3, 5.6e6; dequantize 32768 rows of 8 x 128, 8 bits, 18.6, 5.4e6.
+// 7.4, 3.5e6 (one row per workgroup, all at once: loads, then stores), 8192 x 4096 37.3, 5.9e6; dequantize 32768 rows of 8 x 128, 8 bits, 18.6, 5.4e6.
 #include "mx_format.h"
 #include "rows_math.h"
 
@@ -200,8 +200,10 @@ template <bool BF16, bool ADD, int BITS>
 int launch_norm(MxRows p, bool wide, hipStream_t st) {
   const int64_t lanes = lanes_of(p.cols), all = p.rows, most = 1 << 20;
   p.by_lanes = divide_by(lanes);
-  // (two or four chunks per thread, requested together, gain nothing: 777 x 5120 8.2, 8.4, 8.9 us, 2048 x 8192 20.1, 20.3, 21.1, 300 x 28672 13.5, 15.6, 17.3)
-  const int64_t threads = lanes < 1024 ? (lanes + 63) / 64 * 64 : 1024;
+  // One chunk per thread where so all rows run at once (2048 threads per CU); else two, one after the other (us, one and two: 777 x 5120 8.1, 7.4,
+  // 2048 x 8192 20.3, 19.1; 64 x 5120, which fits, 3.8, 4.3); two or four requested together gain nothing: 777 x 5120 8.2, 8.4, 8.9, 300 x 28672 13.5, 15.6, 17.3.
+  const int64_t one = (lanes + 63) / 64 * 64, two = ((lanes + 1) / 2 + 63) / 64 * 64;
+  const int64_t threads = lanes > 1024 ? 1024 : all > num_cus() * (2048 / one) ? two : one;
   for (int64_t first = 0; first < all; first += most) {
     p.rows = all - first < most ? all - first : most;
     const dim3 grid(static_cast<unsigned>(p.rows)), block(static_cast<unsigned>(threads));

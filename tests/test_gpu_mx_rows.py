@@ -129,7 +129,7 @@ def norm_reference(x, residual, gain, eps):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("with_residual", [False, True])
-@pytest.mark.parametrize("rows,cols", [(1, 2), (1, 64), (5, 34), (3, 250), (2, 4096), (37, 5120), (2, 8200), (1, 40000)])
+@pytest.mark.parametrize("rows,cols", [(1, 2), (1, 64), (5, 34), (3, 250), (2, 4096), (37, 5120), (2, 8200), (1, 40000), (800, 5120), (1030, 4114)])
 def test_norm(dtype, bits, with_residual, rows, cols):
     gen = torch.Generator().manual_seed(rows + cols)
     x = (torch.randn(rows, cols, generator=gen) * 3).to(dtype)
