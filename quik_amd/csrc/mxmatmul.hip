@@ -370,14 +370,18 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   const int m_tiles = static_cast<int>((p.M + S::kBM - 1) / S::kBM), n_tiles = static_cast<int>((p.N + kCols - 1) / kCols);
   const int all = static_cast<int>(gridDim.x), die = blockIdx.x & 7, run = all >> 3, rest = all & 7;
   const int unit = die * run + (die < rest ? die : rest) + static_cast<int>(blockIdx.x >> 3);
-  // (a division is vector code; its result, the same for all lanes, goes back to a scalar register)
-  const int tile = __builtin_amdgcn_readfirstlane(unit / p.splits), split = unit - tile * p.splits;
+  // (a division is some thirty vector instructions; its result, the same for all lanes, goes back to a scalar register)
+  int tile = unit, split = 0, first = 0, stages = all_stages;
+  if (p.splits > 1) {
+    tile = __builtin_amdgcn_readfirstlane(unit / p.splits), split = unit - tile * p.splits;
+    first = __builtin_amdgcn_readfirstlane(all_stages * split / p.splits);  // (at most 2^12 stages)
+    stages = __builtin_amdgcn_readfirstlane(all_stages * (split + 1) / p.splits);
+  }
   const int band = __builtin_amdgcn_readfirstlane(tile / (kBand * n_tiles)), in_band = tile - band * kBand * n_tiles;
   const int high = m_tiles - band * kBand < kBand ? m_tiles - band * kBand : kBand;
-  const int across = __builtin_amdgcn_readfirstlane(in_band / high);
+  const int across = __builtin_amdgcn_readfirstlane(high == 4 ? in_band >> 2 : high == 3 ? in_band / 3 : high == 2 ? in_band >> 1 : in_band);
+  static_assert(kBand == 4, "");
   const int64_t m0 = static_cast<int64_t>(band * kBand + in_band - across * high) * S::kBM, n0 = static_cast<int64_t>(across) * kCols;
-  const int first = __builtin_amdgcn_readfirstlane(all_stages * split / p.splits);  // (at most 2^12 stages)
-  const int stages = __builtin_amdgcn_readfirstlane(all_stages * (split + 1) / p.splits);
 
   const int64_t pitch_w = p.K / 2, pitch_x = p.K * XB / 8, left_m = p.M - 1 - m0, left_n = p.N - 1 - n0;
   const uint8_t *xbase = p.x + m0 * pitch_x, *wbase = p.w + n0 * pitch_w;
