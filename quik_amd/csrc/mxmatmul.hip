@@ -108,7 +108,7 @@ __device__ __forceinline__ int turn_of(int row) {
   return PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-// Up to 16 token rows (TR of them in LDS), on 16x16x128 instructions: the weights are the rows of the result tile, the tokens its columns.  A workgroup
+// Up to 32 token rows (TR of them in LDS, by sixteens), on 16x16x128 instructions: the weights are the rows of the result tile, the tokens its columns.  A workgroup
 // takes tiles of p.width <= 16 * FT result columns, which deals all of them evenly to the CUs; its W waves take blocks of STEPS * 128 columns of K in
 // turn and add their sums through LDS at a tile's end.  Operands and bytes come by direct copies, D - 1 blocks ahead and on into the next tile,
 // into a ring of the wave's own (no barrier but at a tile's end).  Up to eight rows of 8-bit codes are sixteen columns: their codes from 2 up, and behind
@@ -122,7 +122,7 @@ struct RingShape {
   static constexpr int kCW = FT * STEPS, kCX = TR * kPx / 64, kCSW = (16 * FT * STEPS + 63) / 64, kCSX = (TR * STEPS + 63) / 64;
   static constexpr int kCopies = kCW + kCX + kPlanes * (kCSW + kCSX);
   static constexpr int kAtX = kCW * 1024, kAtSW = kAtX + kCX * 1024, kAtSX = kAtSW + kPlanes * kCSW * 256, kStage = kAtSX + kPlanes * kCSX * 256;
-  static constexpr int kRed = W * FT * 1024, kLds = kRed + W * D * kStage;
+  static constexpr int kGroups = (TR + 15) / 16, kRed = W * FT * kGroups * 1024, kLds = kRed + W * D * kStage;
   static_assert(TR * kPx % 64 == 0 && kCopies * (D - 1) < 64, "");
 };
 
@@ -131,6 +131,7 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
   using S = RingShape<XB, TR, FT, W, D, STEPS, TAIL>;
   static_assert(!GATED || FT == 4, "");  // (a block of 32 results)
   constexpr bool kBoth = XB == 8 && TR == 8;
+  constexpr int kGroups = S::kGroups;  // of sixteen rows
   extern __shared__ float red[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
   const int nb = static_cast<int>(p.K / kMxBlock), steps = (nb + 3) / 4, blocks = (steps + STEPS - 1) / STEPS;
@@ -225,20 +226,24 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
   const uint32_t turn = col < 8 ? 0 : kBelow;
   int stage = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    f32x4 acc[FT];
+    f32x4 acc[FT][kGroups];
 #pragma unroll
-    for (int f = 0; f < FT; ++f) acc[f] = f32x4{0, 0, 0, 0};
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) acc[f][g] = f32x4{0, 0, 0, 0};
     for (int blk = wave; blk < blocks; blk += W) {
       copy_next(stage == 0 ? D - 1 : stage - 1);
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::kCopies * (D - 1)));
       asm volatile("" ::: "memory");
       const uint8_t *from = ring + stage * S::kStage;
       // a row's bytes of all steps; whole planes: of this lane's group
-      uint32_t sw[FT][STEPS], sx[STEPS];
+      uint32_t sw[FT][STEPS], sx[kGroups][STEPS];
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         const int plane = TAIL ? kg : 0;
-        sx[s] = *reinterpret_cast<const uint32_t *>(from + S::kAtSX + plane * S::kCSX * 256 + (token * STEPS + s) * 4);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          sx[g][s] = *reinterpret_cast<const uint32_t *>(from + S::kAtSX + plane * S::kCSX * 256 + ((token + 16 * g) * STEPS + s) * 4);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
           sw[f][s] = *reinterpret_cast<const uint32_t *>(from + S::kAtSW + plane * S::kCSW * 256 + ((16 * f + col) * STEPS + s) * 4);
@@ -246,24 +251,26 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         if (blk * STEPS + s >= steps) break;
-        Operand<XB> x;
+        Operand<XB> x[kGroups], below[kGroups];
 #pragma unroll
-        for (int h = 0; h < XB / 4; ++h) {
-          const int piece = XB == 4 ? 4 * s + kg : 8 * s + 4 * h + kg;
-          x.v[h] = *reinterpret_cast<const u32x4 *>(from + S::kAtX + (token * S::kPx + (piece ^ turn_of<S::kPx>(token))) * 16);
-          if constexpr (TAIL) {
-            const int b = 4 * (blk * STEPS + s) + (XB == 4 ? kg : 2 * h + (kg >> 1));
-            if (b >= nb) x.v[h] = u32x4{0, 0, 0, 0};
+        for (int g = 0; g < kGroups; ++g) {
+          const int row = token + 16 * g;
+#pragma unroll
+          for (int h = 0; h < XB / 4; ++h) {
+            const int piece = XB == 4 ? 4 * s + kg : 8 * s + 4 * h + kg;
+            x[g].v[h] = *reinterpret_cast<const u32x4 *>(from + S::kAtX + (row * S::kPx + (piece ^ turn_of<S::kPx>(row))) * 16);
+            if constexpr (TAIL) {
+              const int b = 4 * (blk * STEPS + s) + (XB == 4 ? kg : 2 * h + (kg >> 1));
+              if (b >= nb) x[g].v[h] = u32x4{0, 0, 0, 0};
+            }
           }
-        }
-        const uint32_t by_x = TAIL ? sx[s] : sx[s] >> (8 * kg);
-        Operand<XB> below;
-        if constexpr (XB == 8) {
+          if constexpr (XB == 8) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t v = x.v[i / 4][i % 4];
-            if constexpr (!kBoth) below.v[i / 4][i % 4] = small_of(v);
-            x.v[i / 4][i % 4] = kBoth ? part_of(v, turn) : large_of(v);
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t v = x[g].v[i / 4][i % 4];
+              if constexpr (!kBoth) below[g].v[i / 4][i % 4] = small_of(v);
+              x[g].v[i / 4][i % 4] = kBoth ? part_of(v, turn) : large_of(v);
+            }
           }
         }
 #pragma unroll
@@ -271,25 +278,32 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
           Operand<4> w;
           w.v[0] = *reinterpret_cast<const u32x4 *>(from + ((16 * f + col) * S::kPw + ((4 * s + kg) ^ turn_of<S::kPw>(col))) * 16);
           const uint32_t by_w = TAIL ? sw[f][s] : sw[f][s] >> (8 * kg);
-          acc[f] = mfma16<XB>(w, x, acc[f], by_w, by_x);
-          if constexpr (XB == 8 && !kBoth) acc[f] = mfma16<XB>(w, below, acc[f], by_w, by_x);
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            const uint32_t by_x = TAIL ? sx[g][s] : sx[g][s] >> (8 * kg);
+            acc[f][g] = mfma16<XB>(w, x[g], acc[f][g], by_w, by_x);
+            if constexpr (XB == 8 && !kBoth) acc[f][g] = mfma16<XB>(w, below[g], acc[f][g], by_w, by_x);
+          }
         }
       }
       stage = stage == D - 1 ? 0 : stage + 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wait only; this stage is copied to next: its reads are done)
     }
-    // the waves' sums: value r of lane l is column 16 f + 4 (l / 16) + r of token l % 16
+    // the waves' sums: value r of lane l is column 16 f + 4 (l / 16) + r of token 16 g + l % 16
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) red[((wave * FT + f) * 4 + r) * 64 + lane] = acc[f][r];
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[(((wave * FT + f) * kGroups + g) * 4 + r) * 64 + lane] = acc[f][g][r];
     __syncthreads();
     const int64_t n0 = static_cast<int64_t>(tile) * p.width;
     auto sum = [&](int m, int n) {
-      const int at = ((n >> 4) * 4 + (n & 3)) * 64 + ((n >> 2) & 3) * 16 + m;
+      const int at = (((n >> 4) * kGroups + (m >> 4)) * 4 + (n & 3)) * 64 + ((n >> 2) & 3) * 16 + (m & 15);
+      constexpr int kWave = FT * kGroups * 256;
       float v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v += kBoth ? red[i * FT * 256 + at] + red[i * FT * 256 + at + 8] : red[i * FT * 256 + at];
+      for (int i = 0; i < W; ++i) v += kBoth ? red[i * kWave + at] + red[i * kWave + at + 8] : red[i * kWave + at];
       return p.row ? v * p.row[m] : v;
     };
     if constexpr (GATED) {
@@ -321,7 +335,7 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no copy is under way when the workgroup's LDS goes to another)
 }
 
-// More token rows, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on stages of 256 columns: whole lines
+// More token rows than that, on 32x32x64 instructions: WM x WN waves side by side, each with RM x RN result tiles of 32 x 32, on stages of 256 columns: whole lines
 // of 128 bytes of the weights' rows (half lines cost as many requests again: 8192 x 8192 -> 8192 on stages of 128 columns 434 us).  LDS holds two
 // stages; one or two more are on their way to registers.  (Direct copies to LDS hold the wave that issues them until the CU has taken the ones before, some
 // 36 cycles per kilobyte, and its products with it; and they can start only when their place is free: 300 us.)
@@ -841,20 +855,25 @@ int deal_columns(int64_t N, int ft) {
   return static_cast<int>((N + rounds * cus - 1) / (rounds * cus));
 }
 
+int tiles_side_by_side(int64_t N) { return N > 16 * num_cus() ? 2 : 1; }
 // Two matrix tiles side by side where one would leave a second round of workgroups; then four waves with two blocks under way, not eight with one
 // (us: 1 x 8192 -> 28672 24.7, 25.4; 1 x 13824 -> 5120 8.8, 8.9; 16 rows of it 10.2, 10.4), but for up to eight rows of 8 bits, whose waves take their
 // codes apart meanwhile (1 x 8192 -> 28672 30.2, 27.3).  Gated the ring of two is the better one (1 x 5120 -> 27648 17.6, 20.5), and with one
 // tile (1 x 4096 -> 4096 4.2, 4.6).
 template <int XB, bool TAIL>
 int few_rows(MxArgs p, hipStream_t st) {
-  const int ft = p.N > 16 * num_cus() ? 2 : 1;
+  const int ft = tiles_side_by_side(p.N);
   p.width = deal_columns(p.N, ft);
   if (p.M <= 8) {
     if (ft == 2) return launch_ring<XB, 8, 2, (XB == 8 ? 8 : 4), (XB == 8 ? 2 : 3), 2, TAIL, false>(p, st);
     return launch_ring<XB, 8, 1, 8, 2, 2, TAIL, false>(p, st);
   }
-  if (ft == 2) return launch_ring<XB, 16, 2, 4, 3, 2, TAIL, false>(p, st);
-  return launch_ring<XB, 16, 1, 4, 2, 2, TAIL, false>(p, st);
+  if (p.M <= 16) {
+    if (ft == 2) return launch_ring<XB, 16, 2, 4, 3, 2, TAIL, false>(p, st);
+    return launch_ring<XB, 16, 1, 4, 2, 2, TAIL, false>(p, st);
+  }
+  if (ft == 2) return launch_ring<XB, 32, 2, 4, (XB == 8 ? 2 : 3), 2, TAIL, false>(p, st);
+  return launch_ring<XB, 32, 1, 4, 2, 2, TAIL, false>(p, st);
 }
 template <int XB, bool TAIL>
 int few_rows_gated(MxArgs p, hipStream_t st) {
@@ -873,6 +892,7 @@ constexpr TilePlan kPlans[2][4] = {{{32, 128, 3, 0.5, 1.2, 2.0}, {64, 128, 2, 0.
                                    {{32, 128, 2, 0.85, 1.5, 2.0}, {64, 128, 2, 1.08, 1.8, 2.0}, {128, 128, 1, 1.6, 1.65, 2.0}, {128, 256, 1, 2.35, 2.8, 4.0}}};
 struct Choice {
   int plan, splits;
+  double us;
 };
 // The cheapest tiles and K split: the rounds of workgroups, no less than the weights from memory (of whose rate each CU has its share), and for a split the
 // second launch and its sums, written and read (from the cache that all dies share); a part is four stages at least (64 x 4096 -> 4096, in parts of two 14.5,
@@ -883,10 +903,9 @@ struct Choice {
 // 28672, 256 rows, 278, 277 (128 rows 333).  8 bit: 300 x 4544 -> 4544, 64 rows, 23.9, 23.6 (128 rows 29.0); 300 x 13824 -> 5120, 128 x 256, K in 4, 48, 54.1 (128 x 128 55.7);
 // 777 x 5120 -> 5120, 128 x 256, 53.5, 53.1 (64 rows 58.7); 1024 x 4096 -> 4096, 128 x 128, 32.1, 32.0 (64 rows 36.3); 2048 x 8192 -> 28672, 128 x 256, 658, 645 (128 x 128 757).
 Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
-  Choice best{1, 1};
-  double least = 1e30;
+  Choice best{1, 1, 1e30};
   const int64_t cus = num_cus(), stages = (K + 255) / 256;
-  const double weights = static_cast<double>(N) * static_cast<double>(K) * 0.53125 / 4.6e6;
+  const double weights = static_cast<double>(N) * static_cast<double>(K) * 0.53125 / 5.0e6;
   for (int i = 0; i < 4; ++i) {
     const TilePlan &t = kPlans[x_bits == 8][i];
     const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
@@ -896,13 +915,22 @@ Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
       if (rest) us += static_cast<double>(deep) * (rest <= cus ? t.one : t.full) + t.round;
       const double share = 1.05 * static_cast<double>(groups) / static_cast<double>(cus), stream = weights / (share < 1.0 ? share : 1.0) + 1.0;
       us = (us > stream ? us : stream) + 2.5 + (s > 1 ? 3.5 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 1.1e-6 : 0.0);
-      if (us < least) {
-        least = us;
-        best = Choice{i, s};
-      }
+      if (us < best.us) best = Choice{i, s, us};
     }
   }
   return best;
+}
+// Up to 16 rows take the kernel of few rows, up to 32 where that is quicker: each CU takes the rows of its tiles' columns and all token rows through direct
+// copies, 32 bytes per ns of them and 3 us beside.  us, as the rule has it and measured (tiles): 24 x 4096 -> 4096 6.3, 5.0 (8.7), 17 x 13824 -> 5120 14.9, 11.0 (13.6), 24 x 5120 ->
+// 13824 13.0, 12.3 (17.3), 32 x 8192 -> 28672 35.1, 36 (30.0), 24 x 28672 -> 8192 33.4, 30.0 (28.3); 8 bit: 24 x 4096 -> 4096 8.3, 6.5 (10.1), 32 x 4096 -> 11008 14.4, 13.9 (15.8), 32 x 13824 ->
+// 5120 21.8, 18.8 (16.8).  (Gated, tiles of 32 results: 20 x 4096 -> 22016 19.0, tiles 15.3: up to 16 rows only.)
+bool by_ring(int64_t M, int64_t N, int64_t K, int x_bits) {
+  if (M <= 16) return true;
+  if (M > 32) return false;
+  const int ft = tiles_side_by_side(N), width = deal_columns(N, ft);
+  const int64_t tiles = (N + width - 1) / width, rounds = (tiles + num_cus() - 1) / num_cus();
+  const double bytes = static_cast<double>(rounds * K) * (width * 0.53125 + 32 * (x_bits / 8.0 + 1.0 / 32));
+  return 3.0 + bytes / 32e3 < choose(M, N, K, x_bits, true).us;
 }
 int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
 
@@ -961,7 +989,7 @@ bool by_fours(const uint8_t *xs, const uint8_t *ws, int64_t K) { return K % 128 
 using namespace quik;
 
 extern "C" int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t N, int64_t K) {
-  if (M <= 16 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX / 2 || K > 1 << 20) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX / 2 || K > 1 << 20 || by_ring(M, N, K, x_bits)) return 0;
   return partial_bytes(M, N, choose(M, N, K, x_bits, true).splits);
 }
 
@@ -975,7 +1003,7 @@ extern "C" int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale,
                  static_cast<float *>(workspace), 1};
   hipStream_t st = as_stream(stream);
   const bool fours = by_fours(x_scale, w_scale, K);
-  if (M <= 16) {
+  if (by_ring(M, N, K, x_bits)) {
     if (x_bits == 4) return fours ? few_rows<4, false>(p, st) : few_rows<4, true>(p, st);
     return fours ? few_rows<8, false>(p, st) : few_rows<8, true>(p, st);
   }
