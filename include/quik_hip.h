@@ -487,6 +487,9 @@ int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint
  * stream) then holds the sums of each part, which a second launch adds in order.  Bytes that such a call makes use of, 0: none.  With NULL or
  * fewer bytes K is not split: slower, the same result within its rounding. */
 int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t N, int64_t K);
+/* How such a call is cut (gated != 0: quik_mx_gated_matmul of N results): parts of K << 24 | rows << 12 | columns of one workgroup's results; 0 where there is
+ * nothing to do.  Parts 0: the kernel of few rows (8, 16, 32: how many it holds), whose waves take K in turn, and the columns that are dealt to it. */
+int quik_mx_matmul_tile(int x_bits, int gated, int64_t M, int64_t N, int64_t K, int64_t workspace_bytes);
 /* The first half of a gated feed-forward block in one launch: gate = x w[:inner]^T and up = x w[inner:]^T (times scale_row, rounded to dtype, which is all
  * that dtype is for), value = gate / (1 + exp(-gate)) * up, codes of q_bits: those of quik_mx_matmul and quik_mx_silu_mul_quantize one after the
  * other, up to the order of the sums over K.  w [2 inner, K/2], inner % 32 == 0. */

@@ -81,6 +81,7 @@ SIGNATURES = {
     "quik_mx_rotate_to_cache": (_int, [_vp, _vp]),
     "quik_mx_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
     "quik_mx_matmul_workspace_bytes": (_i64, [_int, _i64, _i64, _i64]),
+    "quik_mx_matmul_tile": (_int, [_int, _int, _i64, _i64, _i64, _i64]),
     "quik_mx_gated_matmul": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
 }
 

@@ -875,9 +875,10 @@ int few_rows(MxArgs p, hipStream_t st) {
   if (ft == 2) return launch_ring<XB, 32, 2, 4, (XB == 8 ? 2 : 3), 2, TAIL, false>(p, st);
   return launch_ring<XB, 32, 1, 4, 2, 2, TAIL, false>(p, st);
 }
+constexpr int kFewGated = 16;  // rows of a gated product that the kernel of few rows takes
 template <int XB, bool TAIL>
 int few_rows_gated(MxArgs p, hipStream_t st) {
-  p.width = 32;
+  p.width = kMxBlock;
   if (p.M <= 8) return launch_ring<XB, 8, 4, 4, 2, 2, TAIL, true>(p, st);
   return launch_ring<XB, 16, 4, 4, 2, 2, TAIL, true>(p, st);
 }
@@ -934,11 +935,21 @@ bool by_ring(int64_t M, int64_t N, int64_t K, int x_bits) {
 }
 int64_t partial_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * M * ((N + 3) / 4 * 4) * 4 : 0; }
 
+// the choice of a call with that much memory for the parts' sums
+Choice choose_within(int64_t M, int64_t N, int64_t K, int x_bits, int64_t workspace_bytes) {
+  const Choice c = choose(M, N, K, x_bits, true);
+  return workspace_bytes < partial_bytes(M, N, c.splits) ? choose(M, N, K, x_bits, false) : c;
+}
+// a gated product's, of `inner` results: K is not split, and tiles of 32 rows are those of 64
+int choose_gated(int64_t M, int64_t inner, int64_t K, int x_bits) {
+  const int plan = choose(M, 2 * inner, K, x_bits, false).plan;
+  return plan == 0 ? 1 : plan;
+}
+
 template <int XB>
 int many_rows(const MxArgs &p, int64_t workspace_bytes, hipStream_t st) {
   MxArgs q = p;
-  Choice c = choose(p.M, p.N, p.K, XB, true);
-  if (!p.partial || workspace_bytes < partial_bytes(p.M, p.N, c.splits)) c = choose(p.M, p.N, p.K, XB, false);
+  const Choice c = choose_within(p.M, p.N, p.K, XB, p.partial ? workspace_bytes : 0);
   q.splits = c.splits;
   if (c.plan == 0) return launch_tile<XB, 1, 1, 1, 4, false>(q, st);
   if constexpr (XB == 8) {
@@ -955,8 +966,8 @@ template <int XB>
 int many_rows_gated(const MxArgs &p, hipStream_t st) {
   MxArgs q = p;
   q.splits = 1;
-  const int plan = choose(p.M, 2 * p.N, p.K, XB, false).plan;
-  if (plan <= 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
+  const int plan = choose_gated(p.M, p.N, p.K, XB);
+  if (plan == 1) return launch_tile<XB, 1, 2, 2, 2, true>(q, st);
   if constexpr (XB == 8) {
     if (plan == 2) return launch_tile<8, 1, 4, 4, 1, true>(q, st);
     return launch_tile<8, 1, 4, 4, 2, true>(q, st);
@@ -993,6 +1004,17 @@ extern "C" int64_t quik_mx_matmul_workspace_bytes(int x_bits, int64_t M, int64_t
   return partial_bytes(M, N, choose(M, N, K, x_bits, true).splits);
 }
 
+extern "C" int quik_mx_matmul_tile(int x_bits, int gated, int64_t M, int64_t N, int64_t K, int64_t workspace_bytes) {
+  if ((x_bits != 4 && x_bits != 8) || M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX / 2 || K > 1 << 20) return 0;
+  if (gated ? M <= kFewGated : by_ring(M, N, K, x_bits)) {
+    const int rows = M <= 8 ? 8 : M <= 16 ? 16 : 32;
+    return rows << 12 | (gated ? kMxBlock : deal_columns(N, tiles_side_by_side(N)));
+  }
+  const Choice c = gated ? Choice{choose_gated(M, N, K, x_bits), 1, 0.0} : choose_within(M, N, K, x_bits, workspace_bytes);
+  const TilePlan &t = kPlans[x_bits == 8][c.plan];
+  return c.splits << 24 | t.rows << 12 | (gated ? t.cols / 2 : t.cols);
+}
+
 extern "C" int quik_mx_matmul(const void *x, int x_bits, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const float *scale_row,
                               const void *bias, int dtype, int64_t M, int64_t N, int64_t K, void *out, void *workspace, int64_t workspace_bytes,
                               void *stream) {
@@ -1021,7 +1043,7 @@ extern "C" int quik_mx_gated_matmul(const void *x, int x_bits, const uint8_t *x_
   const MxArgs p{static_cast<const uint8_t *>(x), x_scale, w, w_scale, scale_row, nullptr, q, q_scale, M, inner, K, dtype == QUIK_BF16, q_bits, 0, nullptr, 1};
   hipStream_t st = as_stream(stream);
   const bool fours = by_fours(x_scale, w_scale, K);
-  if (M <= 16) {
+  if (M <= kFewGated) {
     if (x_bits == 4) return fours ? few_rows_gated<4, false>(p, st) : few_rows_gated<4, true>(p, st);
     return fours ? few_rows_gated<8, false>(p, st) : few_rows_gated<8, true>(p, st);
   }
