@@ -878,6 +878,8 @@ class MicroscaledLinear4bit(torch.nn.Module):
             raise ValueError(f"MicroscaledLinear4bit: in_features must be a multiple of {microscaled.BLOCK}, got {in_features}")
         if act_bits not in (4, 8):
             raise ValueError(f"MicroscaledLinear4bit: act_bits must be 4 or 8, got {act_bits}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"MicroscaledLinear4bit: dtype must be torch.float16 or torch.bfloat16, got {dtype}")
         self.in_features = in_features
         self.out_features = out_features
         self.act_bits = act_bits
@@ -900,7 +902,11 @@ class MicroscaledLinear4bit(torch.nn.Module):
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self.dtype = fn(torch.empty(0, dtype=self.dtype)).dtype   # (.half(), .to(torch.bfloat16): the results' type goes with the bias)
+        dtype = fn(torch.empty(0, dtype=self.dtype)).dtype
+        if dtype in (torch.float16, torch.bfloat16):      # (.half(), .to(torch.bfloat16): the results' type goes with the bias)
+            self.dtype = dtype
+        elif self.bias is not None:                       # (.float(): there are no such results)
+            self.bias = self.bias.to(self.dtype)
         return self
 
     def _rows(self, x, scale, scale_row):

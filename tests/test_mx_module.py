@@ -1,0 +1,42 @@
+"""MicroscaledLinear4bit: which types it has, takes and gives, and what it is made of."""
+import pytest
+import torch
+
+import mx_plain as P
+from quik_amd.qlinear import MicroscaledLinear4bit
+
+DEV = "cuda:0"
+
+
+def ms():
+    from quik import microscaled
+    return microscaled
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.int8])
+def test_results_of_other_types_are_refused(dtype):
+    with pytest.raises(ValueError, match="dtype must be"):
+        MicroscaledLinear4bit(64, 32, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_module_that_is_cast_to_32_bits_keeps_its_type(bias, dtype):
+    mod = MicroscaledLinear4bit(64, 32, bias=bias, dtype=dtype)
+    if bias:
+        mod.bias.copy_(torch.arange(32) / 8)
+    mod.weight.fill_(0x12)
+    outer = torch.nn.Sequential(mod, torch.nn.Linear(32, 2)).float().double()
+    assert mod.dtype == dtype and outer[1].weight.dtype == torch.float64
+    assert mod.weight.dtype == mod.weight_scale.dtype == torch.uint8 and (mod.weight == 0x12).all()
+    if bias:
+        assert mod.bias.dtype == dtype and torch.equal(mod.bias, (torch.arange(32) / 8).to(dtype)) and "bias" in mod.state_dict()
+    assert mod.to(torch.bfloat16).dtype == torch.bfloat16 and mod.half().dtype == torch.float16 and (not bias or mod.bias.dtype == torch.float16)
+
+
+@pytest.mark.gpu
+def test_a_module_that_was_cast_to_32_bits_runs():
+    lin = torch.nn.Linear(64, 32, dtype=torch.bfloat16, device=DEV)
+    mod, x = MicroscaledLinear4bit.from_float(lin), torch.randn(3, 64, device=DEV).bfloat16()
+    want = mod(x)
+    assert torch.equal(mod.float()(x), want) and want.dtype == torch.bfloat16
