@@ -868,8 +868,8 @@ class MicroscaledLinear4bit(torch.nn.Module):
     """4-bit floating-point weights in blocks of 32 input columns with a power of two each (quik.microscaled), and activations in such blocks of
     `act_bits` (4 or 8).
 
-    weight [out, in/2] and weight_scale [out, in/32] are uint8.  forward(x) takes 16-bit activations of `dtype` and quantizes them; forward(q,
-    scale, scale_row) rows as microscaled.quantize, rms_norm_quantize and gated_matmul give them.  gated(...) takes the same where the
+    weight [out, in/2] and weight_scale [out, in/32] are uint8.  forward(x) takes 16-bit activations of `dtype`, the results' type (a module of bfloat16
+    those of float16 too), and quantizes them; forward(q, scale, scale_row) rows as microscaled.quantize, rms_norm_quantize and gated_matmul give them.  gated(...) takes the same where the
     weight is the gates' rows and behind them up's, and returns the activated rows (q, scale) for the next product.  No counterpart in the reference."""
 
     def __init__(self, in_features, out_features, act_bits=4, bias=False, dtype=torch.float16):
@@ -914,6 +914,9 @@ class MicroscaledLinear4bit(torch.nn.Module):
         if scale is None:
             if scale_row is not None:
                 raise ValueError("MicroscaledLinear4bit: scale_row belongs to rows of codes, which come with their scale")
+            if x.dtype == torch.bfloat16 and self.dtype == torch.float16:
+                raise ValueError("MicroscaledLinear4bit: activations are torch.bfloat16 and results torch.float16, whose range bfloat16's pass: "
+                                 "expected torch.float16, or a module of torch.bfloat16")
             rows = x.reshape(-1, x.shape[-1])
             if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
                 rows = rows.contiguous()

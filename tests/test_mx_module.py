@@ -40,3 +40,25 @@ def test_a_module_that_was_cast_to_32_bits_runs():
     mod, x = MicroscaledLinear4bit.from_float(lin), torch.randn(3, 64, device=DEV).bfloat16()
     want = mod(x)
     assert torch.equal(mod.float()(x), want) and want.dtype == torch.bfloat16
+
+
+def test_activations_of_a_wider_range_than_the_results_are_refused():
+    """A module of fp16 would turn results of bf16 activations into infinities; one of bf16 holds those of fp16."""
+    mod = MicroscaledLinear4bit(64, 64)
+    for call in (mod, mod.gated):
+        with pytest.raises(ValueError, match="bfloat16"):
+            call(torch.zeros(2, 64, dtype=torch.bfloat16))
+        with pytest.raises(RuntimeError, match="float16 or bfloat16|CUDA"):
+            call(torch.zeros(2, 64))
+
+
+@pytest.mark.gpu
+def test_activations_of_either_type():
+    lin = torch.nn.Linear(64, 32, dtype=torch.float16, device=DEV)
+    mod, x = MicroscaledLinear4bit.from_float(lin), torch.randn(3, 64, device=DEV).half()
+    with pytest.raises(ValueError, match="bfloat16"):
+        mod(x.bfloat16() * 2.0 ** 20)
+    assert mod(x).dtype == torch.float16
+    q, s = ms().quantize(x.bfloat16() * 2.0 ** 20)           # rows of codes have no type: what does not fit is the caller's
+    assert mod(q, s).dtype == torch.float16
+    assert mod.to(torch.bfloat16)(x.bfloat16() * 2.0 ** 20).isfinite().all() and mod(x).dtype == torch.bfloat16
