@@ -895,7 +895,7 @@ class MicroscaledLinear4bit(torch.nn.Module):
         w = module.weight
         dtype = w.dtype if w.dtype in (torch.float16, torch.bfloat16) else torch.float16
         mod = MicroscaledLinear4bit(module.in_features, module.out_features, act_bits, module.bias is not None, dtype).to(w.device)
-        mod.weight, mod.weight_scale = microscaled.quantize(w.detach().to(dtype), 4)
+        mod.weight, mod.weight_scale = microscaled.quantize(w.detach().to(dtype).contiguous(), 4)   # (a weight may be another's transpose)
         if module.bias is not None:
             mod.bias.copy_(module.bias)
         return mod

@@ -62,3 +62,16 @@ def test_activations_of_either_type():
     q, s = ms().quantize(x.bfloat16() * 2.0 ** 20)           # rows of codes have no type: what does not fit is the caller's
     assert mod(q, s).dtype == torch.float16
     assert mod.to(torch.bfloat16)(x.bfloat16() * 2.0 ** 20).isfinite().all() and mod(x).dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_a_weight_whose_columns_lie_apart(dtype):
+    """Another matrix' transpose (tied weights), and every other row of one."""
+    lin, w = torch.nn.Linear(96, 64, dtype=dtype, device=DEV), torch.randn(96, 64, dtype=dtype, device=DEV)
+    for weight in (w.t(), torch.randn(128, 96, dtype=dtype, device=DEV)[::2]):
+        lin.weight = torch.nn.Parameter(weight)
+        mod = MicroscaledLinear4bit.from_float(lin)
+        kind = torch.float16 if dtype == torch.float32 else dtype
+        c, e = P.codes(weight.to(kind).double().cpu(), 4)
+        assert torch.equal(P.unpack(mod.weight.cpu()), c) and torch.equal(mod.weight_scale.cpu().to(torch.int64), e)
