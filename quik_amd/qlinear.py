@@ -891,13 +891,20 @@ class MicroscaledLinear4bit(torch.nn.Module):
     @staticmethod
     @torch.no_grad()
     def from_float(module, act_bits=4):
-        """The nearest codes of a torch.nn.Linear on the GPU (an fp32 module's weight is rounded to fp16 first)."""
+        """The nearest codes of a torch.nn.Linear on the GPU (an fp32 module's weight and bias are rounded to fp16 first; one that has numbers beyond
+        its range is refused: they would be infinities, and a block with one NaNs)."""
         w = module.weight
         dtype = w.dtype if w.dtype in (torch.float16, torch.bfloat16) else torch.float16
+        rounded = {}
+        for name, t in (("weight", w), ("bias", module.bias)):
+            if t is not None:
+                rounded[name] = t.detach().to(dtype).contiguous()   # (a weight may be another's transpose)
+                if t.dtype != dtype and bool((t.isfinite() & ~rounded[name].isfinite()).any()):
+                    raise ValueError(f"MicroscaledLinear4bit: {name} has numbers beyond the range of {dtype}; a module of torch.bfloat16 holds them")
         mod = MicroscaledLinear4bit(module.in_features, module.out_features, act_bits, module.bias is not None, dtype).to(w.device)
-        mod.weight, mod.weight_scale = microscaled.quantize(w.detach().to(dtype).contiguous(), 4)   # (a weight may be another's transpose)
+        mod.weight, mod.weight_scale = microscaled.quantize(rounded["weight"], 4)
         if module.bias is not None:
-            mod.bias.copy_(module.bias)
+            mod.bias.copy_(rounded["bias"])
         return mod
 
     def _apply(self, fn, recurse=True):

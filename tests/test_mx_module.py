@@ -75,3 +75,23 @@ def test_a_weight_whose_columns_lie_apart(dtype):
         kind = torch.float16 if dtype == torch.float32 else dtype
         c, e = P.codes(weight.to(kind).double().cpu(), 4)
         assert torch.equal(P.unpack(mod.weight.cpu()), c) and torch.equal(mod.weight_scale.cpu().to(torch.int64), e)
+
+
+def test_numbers_beyond_the_range_of_the_type_are_refused():
+    for name in ("weight", "bias"):
+        lin = torch.nn.Linear(64, 32)
+        getattr(lin, name).data.view(-1)[5] = -7e4
+        with pytest.raises(ValueError, match=f"{name} has numbers beyond"):
+            MicroscaledLinear4bit.from_float(lin)
+
+
+@pytest.mark.gpu
+def test_the_largest_numbers_of_the_type_and_none_at_all():
+    lin = torch.nn.Linear(64, 4, device=DEV)
+    lin.weight.data[0, 3], lin.bias.data[1] = 65504.0, -65519.0      # (which rounds to fp16's last)
+    lin.weight.data[2, 40] = float("inf")                            # an infinity of the module's own: its block has no numbers
+    mod = MicroscaledLinear4bit.from_float(lin)
+    assert mod.bias[1] == -65504 and torch.equal(mod.weight_scale == 255, torch.tensor([[0, 0], [0, 0], [0, 1], [0, 0]], device=DEV) == 1)
+    lin = torch.nn.Linear(64, 4, device=DEV, dtype=torch.bfloat16)
+    lin.weight.data[0, 3] = 1e30
+    assert (MicroscaledLinear4bit.from_float(lin).weight_scale != 255).all()
