@@ -929,17 +929,21 @@ class MicroscaledLinear4bit(torch.nn.Module):
                 rows = rows.contiguous()
             x, scale = microscaled.quantize(rows, self.act_bits)
         else:
-            x, scale = x.reshape(-1, x.shape[-1]), scale.reshape(-1, scale.shape[-1])
-        return lead, x, scale
+            x, scale = x.reshape(-1, x.shape[-1]).contiguous(), scale.reshape(-1, scale.shape[-1]).contiguous()
+            if x.is_cuda and x.data_ptr() % 16:     # (a contiguous view that starts between)
+                x = x.clone()
+            if scale_row is not None:
+                scale_row = scale_row.contiguous()
+        return lead, x, scale, scale_row
 
     def forward(self, x, scale=None, scale_row=None):
-        lead, q, scale = self._rows(x, scale, scale_row)
+        lead, q, scale, scale_row = self._rows(x, scale, scale_row)
         out = microscaled.matmul(q, scale, self.weight, self.weight_scale, self.dtype, scale_row, self.bias)
         return out.reshape(*lead, self.out_features)
 
     def gated(self, x, scale=None, scale_row=None, bits=None):
         if self.bias is not None:
             raise ValueError("MicroscaledLinear4bit: the gated product has no bias")
-        lead, q, scale = self._rows(x, scale, scale_row)
+        lead, q, scale, scale_row = self._rows(x, scale, scale_row)
         q, scale = microscaled.gated_matmul(q, scale, self.weight, self.weight_scale, self.dtype, scale_row, self.act_bits if bits is None else bits)
         return q.reshape(*lead, q.shape[-1]), scale.reshape(*lead, scale.shape[-1])

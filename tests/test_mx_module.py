@@ -95,3 +95,23 @@ def test_the_largest_numbers_of_the_type_and_none_at_all():
     lin = torch.nn.Linear(64, 4, device=DEV, dtype=torch.bfloat16)
     lin.weight.data[0, 3] = 1e30
     assert (MicroscaledLinear4bit.from_float(lin).weight_scale != 255).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act_bits", [4, 8])
+def test_rows_of_codes_of_any_layout(act_bits):
+    """Codes that start between 16-byte borders, and codes, bytes and factors whose rows lie apart, are copied as activations are."""
+    lin = torch.nn.Linear(96, 64, bias=False, dtype=torch.float16, device=DEV)
+    mod, x, gain = MicroscaledLinear4bit.from_float(lin, act_bits), torch.randn(10, 96, device=DEV).half(), torch.ones(96, device=DEV).half()
+    q, s, row, _ = ms().rms_norm_quantize(x, gain, bits=act_bits)
+    raw = q.view(torch.uint8)
+    moved = torch.cat((raw.new_zeros(8), raw.flatten()))[8:].view(raw.shape).view(q.dtype)
+    assert moved.data_ptr() % 16 and moved.is_contiguous()
+    wide = torch.cat((raw, raw), 1)[:, raw.shape[1]:].view(q.dtype)
+    assert not wide.is_contiguous()
+    for call in (mod, lambda *a: torch.cat([t.view(torch.uint8) for t in mod.gated(*a)], 1)):
+        want = call(q, s, row)
+        assert torch.equal(call(moved, s, row), want)
+        assert torch.equal(call(wide, torch.cat((s, s), 1)[:, s.shape[1]:], torch.cat((row, row), 1)[:, 1:]), want)
+        assert torch.equal(call(q[::2], s[::2], row[::2]), want[::2])
+        assert torch.equal(call(q[1:], s[1:], row[1:]), want[1:])
