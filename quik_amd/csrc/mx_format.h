@@ -5,7 +5,7 @@
 // A block that holds a NaN or an infinity has codes 0 and the byte 255 (NaN): whatever it is multiplied by is a NaN.
 // Two 4-bit codes per byte, the even column in the low half.
 #pragma once
-#include "common.h"
+#include "rows_math.h"
 
 namespace quik {
 namespace {
@@ -87,8 +87,6 @@ inline Divide divide_by(int64_t d) {
 }
 
 // at the alignment of one element (global memory takes any)
-typedef uint32_t mx_loose4 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t mx_loose2 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t mx_loose1 __attribute__((aligned(1)));
 
 // the largest of four neighbouring lanes
@@ -104,7 +102,7 @@ template <bool WIDE>
 __device__ __forceinline__ void load_eight(const uint16_t *from, int left, uint16_t (&v)[8]) {
   if (WIDE || left == 8) {
     if constexpr (WIDE) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(from);
-    else *reinterpret_cast<mx_loose4 *>(v) = *reinterpret_cast<const mx_loose4 *>(from);
+    else *reinterpret_cast<loose4 *>(v) = *reinterpret_cast<const loose4 *>(from);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < left ? from[e] : 0;
@@ -114,7 +112,7 @@ template <bool WIDE>
 __device__ __forceinline__ void store_eight(uint16_t *to, int left, const uint16_t (&v)[8]) {
   if (WIDE || left == 8) {
     if constexpr (WIDE) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(v);
-    else *reinterpret_cast<mx_loose4 *>(to) = *reinterpret_cast<const mx_loose4 *>(v);
+    else *reinterpret_cast<loose4 *>(to) = *reinterpret_cast<const loose4 *>(v);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -144,7 +142,7 @@ __device__ __forceinline__ void store_block(const float (&v)[8], int left, uint8
   } else {
     const uint2 w = encode8(v, byte);
     if constexpr (WIDE) *reinterpret_cast<uint2 *>(codes) = w;
-    else if (left >= 8) *reinterpret_cast<mx_loose2 *>(codes) = mx_loose2{w.x, w.y};
+    else if (left >= 8) *reinterpret_cast<loose2 *>(codes) = loose2{w.x, w.y};
     else
       for (int e = 0; e < left; ++e) codes[e] = static_cast<uint8_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
   }

@@ -10,7 +10,6 @@
 // 4096 tokens of 40 + 2 * 40 heads of 128 fp16, keys 8 bit, values 4: 45.4 us for 195 MB, 4.3 TB/s of a copy's 5.1 (by single columns 73.9 us); 64 tokens of
 // 64 + 2 * 8 heads bf16 5.5 us, which is a launch and its loads' way.
 #include "mx_format.h"
-#include "rows_math.h"
 
 namespace quik {
 namespace {

@@ -12,7 +12,6 @@
 // (In one part sums were off by 1.5e-4 of their size, and the codes behind a gated product by 8e-4 in place of 2e-4.)
 // Columns behind the end of K: codes of x are made 0 in registers, the weights and bytes there are the row's last ones.
 #include "mx_format.h"
-#include "rows_math.h"
 
 #include <type_traits>
 
@@ -358,7 +357,8 @@ struct TileShape {
   static constexpr int kW = WM * WN, kBM = 32 * RM * WM, kBN = 32 * RN * WN, kT = 64 * kW;
   static constexpr int kPx = 2 * XB, kPw = 8;                         // 16-byte pieces of a row in a stage
   static constexpr int kCX = kBM * kPx / 64, kCW = kBN * kPw / 64;    // loads of 1 KB
-  static constexpr int kMyX = (kCX + kW - 1) / kW, kMyW = (kCW + kW - 1) / kW, kLoads = kMyX + kMyW;
+  static constexpr int kMyX = kCX / kW, kMyW = kCW / kW, kLoads = kMyX + kMyW;
+  static_assert(kCX % kW == 0 && kCW % kW == 0, "");
   static constexpr int kAtW = kCX * 1024, kStage = kAtW + kCW * 1024;
   static constexpr int kAtS = 2 * kStage, kRings = kAtS + (kBM + kBN) * 32;
   static constexpr int kPitch = RN * 64 + 16, kOut = kW * 32 * kPitch;  // (a wave's 32 rows on their way out)
@@ -373,7 +373,6 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   constexpr int kCols = GATED ? S::kBN / 2 : S::kBN;  // result columns per tile
   extern __shared__ float red[];
   uint8_t *lds = reinterpret_cast<uint8_t *>(red);
-  const uint32_t lds_at = lds_address(lds);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, kg = lane >> 5;
   const int wn = wave % WN, wm = wave / WN;
   const int nb = static_cast<int>(p.K / kMxBlock), all_stages = (nb + 7) / 8;
@@ -404,9 +403,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
   auto is_up = [](int R) { return GATED && R % (32 * RN) >= 16 * RN; };
   // this wave's loads: the row's offset and the piece of the stage that this lane takes, and where it goes
   uint32_t x_off[S::kMyX], w_off[S::kMyW];
-  auto nth = [&](int i, int all) { return all % S::kW == 0 ? wave + i * S::kW : (wave + i * S::kW) % all; };
-  auto x_row = [&](int i) { return nth(i, S::kCX) * (64 / S::kPx) + lane / S::kPx; };
-  auto w_row = [&](int i) { return nth(i, S::kCW) * 8 + (lane >> 3); };
+  auto nth = [&](int i) { return wave + i * S::kW; };
+  auto x_row = [&](int i) { return nth(i) * (64 / S::kPx) + lane / S::kPx; };
+  auto w_row = [&](int i) { return nth(i) * 8 + (lane >> 3); };
   const int x_piece = lane % S::kPx, w_piece = lane & 7;
 #pragma unroll
   for (int i = 0; i < S::kMyX; ++i) x_off[i] = static_cast<uint32_t>((x_row(i) < left_m ? x_row(i) : left_m) * pitch_x);
@@ -426,14 +425,14 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
       staged[i] = *reinterpret_cast<const u32x4 *>(xbase + stage * (S::kPx * 16) + (x_off[i] + static_cast<uint32_t>(piece) * 16));
     } else {
       const int last = nb - 1 - stage * 8, piece = w_piece < last ? w_piece : last;
-      const uint8_t *from = is_up(nth(i - S::kMyX, S::kCW) * 8) ? wbase + p.N * pitch_w : wbase;
+      const uint8_t *from = is_up(nth(i - S::kMyX) * 8) ? wbase + p.N * pitch_w : wbase;
       staged[i] = *reinterpret_cast<const u32x4 *>(from + stage * 128 + (w_off[i - S::kMyX] + static_cast<uint32_t>(piece) * 16));
     }
   };
   auto write = [&](const u32x4 (&staged)[S::kLoads], int stage, int i) {
     uint8_t *to = lds + ((stage - first) & 1) * S::kStage;
-    if (i < S::kMyX) *reinterpret_cast<u32x4 *>(to + x_to + (nth(i, S::kCX) - wave) * 1024) = staged[i];
-    else *reinterpret_cast<u32x4 *>(to + w_to + (nth(i - S::kMyX, S::kCW) - wave) * 1024) = staged[i];
+    if (i < S::kMyX) *reinterpret_cast<u32x4 *>(to + x_to + (nth(i) - wave) * 1024) = staged[i];
+    else *reinterpret_cast<u32x4 *>(to + w_to + (nth(i - S::kMyX) - wave) * 1024) = staged[i];
   };
   // exponent bytes: rows of x, then of w (a thread without a row of its own takes the last one too)
   const uint8_t *bytes_of[S::kRows];
@@ -714,7 +713,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
             const uint32_t o0 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[0]), 32)), o1 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine[1]), 32));
             const uint32_t lo = kg ? o1 : mine[0], hi = kg ? mine[1] : o0;  // group 0 stores columns 0 .. 15, group 1 the others
             const uint2 both = make_uint2((lo & 0xFFFFu) | hi << 16, lo >> 16 | (hi & 0xFFFF0000u));
-            if (there) *reinterpret_cast<mx_loose2 *>(static_cast<uint8_t *>(p.out) + block * 16 + 8 * kg) = mx_loose2{both.x, both.y};
+            if (there) *reinterpret_cast<loose2 *>(static_cast<uint8_t *>(p.out) + block * 16 + 8 * kg) = loose2{both.x, both.y};
           } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -753,7 +752,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxArgs p) {
           if (mm >= p.M || n >= p.N) continue;
           uint16_t *to = static_cast<uint16_t *>(p.out) + mm * p.N + n;
           if (n + 7 < p.N) {
-            *reinterpret_cast<mx_loose4 *>(to) = mx_loose4{w.x, w.y, w.z, w.w};
+            *reinterpret_cast<loose4 *>(to) = loose4{w.x, w.y, w.z, w.w};
           } else {
             const uint32_t h[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -848,7 +847,7 @@ int launch_tile(const MxArgs &p, hipStream_t st) {
   return QUIK_OK;
 }
 
-// Result columns per workgroup for up to 16 rows: the rounds that all CUs need with FT matrix tiles side by side, and the columns of a round
+// Result columns per workgroup of the kernel of few rows: the rounds that all CUs need with FT matrix tiles side by side, and the columns of a round
 // dealt to them evenly.
 int deal_columns(int64_t N, int ft) {
   const int64_t cus = num_cus(), most = 16 * ft, rounds = ((N + most - 1) / most + cus - 1) / cus;

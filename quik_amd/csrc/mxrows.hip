@@ -11,7 +11,6 @@
 // us, bytes per us against a copy's 5.1e6: quantize 2048 x 8192, 4 bits, 9.3, 4.6e6; silu_mul 2048 x 13824, 8 bits, 26.3, 5.4e6; norm with a residual 777 x 5120, 4 bits,
 // 7.4, 3.5e6 (one row per workgroup, all at once: loads, then stores), 8192 x 4096 37.3, 5.9e6; dequantize 32768 rows of 8 x 128, 8 bits, 18.6, 5.4e6.
 #include "mx_format.h"
-#include "rows_math.h"
 
 namespace quik {
 namespace {
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(256) void mx_read_kernel(MxRead p) {
         if constexpr (WIDE) {
           w[j] = *reinterpret_cast<const uint2 *>(q);
         } else if (left[j] == 8) {
-          const mx_loose2 t = *reinterpret_cast<const mx_loose2 *>(q);
+          const loose2 t = *reinterpret_cast<const loose2 *>(q);
           w[j] = make_uint2(t[0], t[1]);
         } else {
           for (int e = 0; e < left[j]; ++e) (e < 4 ? w[j].x : w[j].y) |= static_cast<uint32_t>(q[e]) << (8 * (e & 3));
