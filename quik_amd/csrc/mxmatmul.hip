@@ -347,8 +347,9 @@ __global__ __launch_bounds__(64 * W) void mx_ring_kernel(MxArgs p) {
 // Gated: a wave's tiles f < RN / 2 are gates, the others the same columns of up.
 // 8-bit rows: the codes of the next 64 columns are taken apart behind the products of these, five vector instructions per four codes, in the places where
 // the matrix unit is busy.  So a wave has one row of matrix tiles and up to four of them in it (with two rows of two, each wave takes twice as many
-// codes apart: 2048 x 8192 -> 28672 782 us, this 645; its products are 72 % of the SIMDs' cycles, at a clock of 1.76 GHz).
-// 4 bits: 2048 x 8192 -> 28672 277 us, 3.5 PFLOP/s, the matrix unit busy for 43 % of the cycles, at 1.9 GHz; 64 x 5120 -> 27648 gated 22.2 us, 3.6 TB/s.
+// codes apart: 2048 x 8192 -> 28672 782 us, this 637; its products are 75 % of the SIMDs' cycles, at a clock of 1.74 GHz).
+// 4 bits: 2048 x 8192 -> 28672 275 us, 3.5 PFLOP/s, the matrix unit busy for 48 % of the cycles, at 1.8 GHz (24576 columns, three full rounds of workgroups, 220:
+// 54 %, 1.7 GHz); 64 x 5120 -> 27648 gated 22.0 us, 3.6 TB/s.
 template <int XB, int RM, int RN, int WM, int WN>
 struct TileShape {
   // Stages on their way to registers: two where the results leave room, with their loads dealt to three quarters of a stage (us, one on its way and
@@ -897,11 +898,12 @@ struct Choice {
 // The cheapest tiles and K split: the rounds of workgroups, no less than the weights from memory (of whose rate each CU has its share), and for a split the
 // second launch and its sums, written and read (from the cache that all dies share); a part is four stages at least (64 x 4096 -> 4096, in parts of two 14.5,
 // of four 11.1).  us, as the rule has it and measured (the next best measured):
-// 64 x 13824 -> 5120, 64 rows, K in 6, 16.9, 17.2 (32 rows, K in 3: 18.5); 64 x 8192 -> 8192, 64 rows, K in 4, 16.4, 16.1 (32 rows, K in 2: 16.8); 32 x 28672 -> 8192, 32 rows, K in
-// 4, 35, 30.1 (in 3, 192 workgroups: 42.2); 64 x 4096 -> 11008, 32 rows, 12.5, 11.3 (64 rows 13.0); 128 x 5120 -> 13824, 64 rows, 16.1, 18.8 (128 rows 22.2); 300 x 4544 -> 4544,
-// 64 rows, 14.9, 15.3 (128 rows 18.1); 300 x 13824 -> 5120, 128 rows, K in 2, 31, 32.0 (64 rows 37.6); 777 x 5120 -> 5120, 128 rows, 34.5, 30.0 (64 rows 33.6); 2048 x 8192 ->
-// 28672, 256 rows, 278, 277 (128 rows 333).  8 bit: 300 x 4544 -> 4544, 64 rows, 23.9, 23.6 (128 rows 29.0); 300 x 13824 -> 5120, 128 x 256, K in 4, 48, 54.1 (128 x 128 55.7);
-// 777 x 5120 -> 5120, 128 x 256, 53.5, 53.1 (64 rows 58.7); 1024 x 4096 -> 4096, 128 x 128, 32.1, 32.0 (64 rows 36.3); 2048 x 8192 -> 28672, 128 x 256, 658, 645 (128 x 128 757).
+// 64 x 13824 -> 5120, 64 rows, K in 6, 16.8, 16.2 (32 rows, K in 3: 18.5); 64 x 8192 -> 8192, 64 rows, K in 4, 16.4, 15.5 (32 rows, K in 2: 16.8); 32 x 28672 -> 8192, 32 rows, K in
+// 4, 33.1, 29.6 (in 3, 192 workgroups: 42.2); 64 x 4096 -> 11008, 32 rows, 12.5, 9.9 (64 rows 13.0); 128 x 5120 -> 13824, 64 rows, 16.1, 17.2 (128 rows 22.2); 300 x 4544 -> 4544,
+// 64 rows, 14.9, 13.7 (128 rows 18.1); 300 x 13824 -> 5120, 128 rows, K in 2, 31.9, 31.3 (64 rows 37.6); 777 x 5120 -> 5120, 128 rows, 34.5, 28.8 (64 rows 33.6); 2048 x 8192 ->
+// 28672, 256 rows, 270.5, 275 (128 rows 333), 24576 columns 209.5, 220, 8192 x 8192 -> 8192 278.5, 282.  8 bit: 300 x 4544 -> 4544, 64 rows, 23.9, 22.6 (128 rows 29.0); 300 x 13824 ->
+// 5120, 128 x 256, K in 4, 49.7, 51.9 (128 x 128 55.7); 777 x 5120 -> 5120, 128 x 256, 53.5, 51.5 (64 rows 58.7); 1024 x 4096 -> 4096, 128 x 128, 30.9, 31.6 (64 rows 36.3); 2048 x
+// 8192 -> 28672, 128 x 256, 657.7, 637 (128 x 128 757).
 Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
   Choice best{1, 1, 1e30};
   const int64_t cus = num_cus(), stages = (K + 255) / 256;
@@ -921,9 +923,9 @@ Choice choose(int64_t M, int64_t N, int64_t K, int x_bits, bool may_split) {
   return best;
 }
 // Up to 16 rows take the kernel of few rows, up to 32 where that is quicker: each CU takes the rows of its tiles' columns and all token rows through direct
-// copies, 32 bytes per ns of them and 3 us beside.  us, as the rule has it and measured (tiles): 24 x 4096 -> 4096 6.3, 5.0 (8.7), 17 x 13824 -> 5120 14.9, 11.0 (13.6), 24 x 5120 ->
-// 13824 13.0, 12.3 (17.3), 32 x 8192 -> 28672 35.1, 36 (30.0), 24 x 28672 -> 8192 33.4, 30.0 (28.3); 8 bit: 24 x 4096 -> 4096 8.3, 6.5 (10.1), 32 x 4096 -> 11008 14.4, 13.9 (15.8), 32 x 13824 ->
-// 5120 21.8, 18.8 (16.8).  (Gated, tiles of 32 results: 20 x 4096 -> 22016 19.0, tiles 15.3: up to 16 rows only.)
+// copies, 32 bytes per ns of them and 3 us beside.  us, as the rule has it and measured (tiles): 24 x 4096 -> 4096 6.3, 4.9 (8.7), 17 x 13824 -> 5120 14.9, 11.1 (13.6), 24 x 5120 ->
+// 13824 13.0, 12.3 (17.3), 32 x 8192 -> 28672 35.6, 36 (27.4), 24 x 28672 -> 8192 33.5, 30.0 (28.6); 8 bit: 24 x 4096 -> 4096 8.3, 6.6 (10.1), 32 x 4096 -> 11008 14.4, 13.9 (15.8), 32 x 13824 ->
+// 5120 21.8, 18.8 (16.5).  (Gated, tiles of 32 results: 20 x 4096 -> 22016 19.0, tiles 15.3: up to 16 rows only.)
 bool by_ring(int64_t M, int64_t N, int64_t K, int x_bits) {
   if (M <= 16) return true;
   if (M > 32) return false;
